@@ -46,6 +46,10 @@ extern "C" {
 #define JO_BF16 2
 #define JO_E4M3 3 /* float8_e4m3fn */
 
+/* ---- 4-bit formats (e2m1 codes, two to a byte, even element low) ------ */
+#define JO_FP4_NV 0 /* blocks of 16: e4m3 block scales, an fp32 scale per row */
+#define JO_FP4_MX 1 /* blocks of 32: power-of-two (e8m0) block scales         */
+
 /* ---- norm codes (fused_norm_scale_shift.cu:153) ---------------------- */
 #define JO_NORM_LAYER 0
 #define JO_NORM_RMS 1
@@ -397,6 +401,107 @@ JO_API int jo_peer_wait(const uint64_t* flags, int world, int skip, uint64_t val
 /* cudaMemcpyAsync of `bytes` device bytes on `stream` (a peer's mapped memory
  * as the source: a copy-engine transfer over NVLink). */
 JO_API int jo_peer_copy(void* dst, const void* src, int64_t bytes, void* stream);
+
+/* ====================================================================== *
+ *  Attention layer of a batch of requests that share a long prefix
+ *  (no reference counterpart)
+ * ====================================================================== */
+
+/* Bytes of the block scales of a [rows, cols] matrix in a 4-bit format: tiles of
+ * 128 rows x 4 blocks, [ceil(rows/128), ceil(blocks/4), 32, 4, 4] bytes, where
+ * row m and block b of a tile sit at [m % 32, m / 32, b] (blocks of 16 elements
+ * for JO_FP4_NV, 32 for JO_FP4_MX).  -1: bad arguments. */
+JO_API int64_t jo_fp4_scale_bytes(int64_t rows, int64_t cols, int format);
+
+/* Rows to 4 bits.  x: F32/F16/BF16 [rows, cols], cols a multiple of 32; q: packed
+ * codes [rows, cols/2] bytes (row stride in bytes, a multiple of 8); block_scale:
+ * jo_fp4_scale_bytes(rows, cols, format) bytes, every one written (zero where there
+ * is no row or block); row_scale: fp32 [rows], JO_FP4_NV only.
+ *   JO_FP4_NV: r = max(amax(row), 1e-8) / 2688; s = e4m3((amax(block) / r) / 6);
+ *              code = e2m1(x / (s r)), 0 where s is 0; value = code * s * r
+ *   JO_FP4_MX: s = 2^clamp(floor(log2 amax(block)) - 2, -127, 127) (2^-127 for a
+ *              zero block); code = e2m1(x / s), saturating at 6; value = code * s
+ * with correctly rounded fp32 quotients and conversions to the nearest, ties to
+ * even.  A row (NV) or block (MX) with an infinity or a NaN becomes NaN: its scale is
+ * NaN and its codes are zero. */
+JO_API int jo_quant_fp4(void* q, int64_t q_row_stride, void* block_scale, float* row_scale, const void* x,
+                        int64_t x_row_stride, int64_t rows, int64_t cols, int format, int dtype, void* stream);
+
+/* The values of jo_quant_fp4's output, as F32/F16/BF16: code * s (* r), one fp32
+ * rounding of the product with r, one rounding to dtype. */
+JO_API int jo_dequant_fp4(void* out, int64_t out_row_stride, const void* q, int64_t q_row_stride,
+                          const void* block_scale, const float* row_scale, int64_t rows, int64_t cols, int format,
+                          int dtype, void* stream);
+
+/* Product of two matrices held in 4 bits, D[m,n] = out((sum_k A[m,k] * B[n,k]) *
+ * scale_b[n] * scale_a[m] (+ bias[n])): A [M, K] and B [N, K] (a Linear's weight as it
+ * is stored) are codes times block scales of one format, summed in fp32; scale_a /
+ * scale_b: fp32 row scales, NULL = 1; D row-major [M, N] (row stride ldd), F16/BF16,
+ * as is the bias (NULL = none).  lda, ldb: row strides in bytes, multiples of 16; K a
+ * multiple of 32, N and ldd of 8; every operand 16-byte aligned. */
+JO_API int jo_fp4_scaled_mm(void* d, int64_t ldd, const void* a, int64_t lda, const void* b, int64_t ldb,
+                            const void* block_a, const void* block_b, const float* scale_a, const float* scale_b,
+                            const void* bias, int64_t m, int64_t n, int64_t k, int format, int out_dtype,
+                            void* stream);
+
+/* Rotary position embedding by gathered table rows.  q: [tokens, q_heads,
+ * head_dim], k: [tokens, k_heads, head_dim] (k_heads == 0: q alone), element
+ * (t, h, d) at p[t*stride_t + h*stride_h + d]; an output may be its input.
+ * cos/sin: fp32 [table_rows, rot_dim/2] contiguous; positions: int32 or int64
+ * (index_bits 32 / 64) [tokens].  Of each head's first rot_dim elements the
+ * pairs (2i, 2i+1) (interleaved != 0) or (i, i + rot_dim/2) become
+ * (x0 c - x1 s, x0 s + x1 c); the other elements are copied.  fp32 math, one
+ * rounding.  inverse != 0: -sin, which is the gradient with respect to q and k.
+ * A position outside the tables gives NaN in the rotated elements (nothing is
+ * read out of range).  dtype: F32/F16/BF16; head_dim even, <= 256.  Rows that
+ * start on 16 bytes with rot_dim/2 a multiple of 8 (16-bit) are moved 16 bytes
+ * at a time, others element by element. */
+JO_API int jo_rotary_embed(void* q_out, int64_t qo_stride_t, int64_t qo_stride_h, const void* q, int64_t q_stride_t,
+                           int64_t q_stride_h, void* k_out, int64_t ko_stride_t, int64_t ko_stride_h, const void* k,
+                           int64_t k_stride_t, int64_t k_stride_h, const float* cos, const float* sin,
+                           int64_t table_rows, const void* positions, int index_bits, int64_t tokens,
+                           int64_t q_heads, int64_t k_heads, int64_t head_dim, int64_t rot_dim, int interleaved,
+                           int inverse, int dtype, void* stream);
+
+/* jo_rotary_embed for serving: the rotated keys and the values (copied) go to
+ * row slots[t] of k_cache / v_cache [cache_rows, k_heads, head_dim] (element
+ * (r, h, d) at p[r*stride_r + h*stride_h + d]), the rotated q to q_out.  slots
+ * has the positions' type.  A slot outside [0, cache_rows) (a padding token)
+ * writes neither cache; two tokens with one slot leave either's row. */
+JO_API int jo_rotary_embed_append(void* q_out, int64_t qo_stride_t, int64_t qo_stride_h, const void* q,
+                                  int64_t q_stride_t, int64_t q_stride_h, const void* k, int64_t k_stride_t,
+                                  int64_t k_stride_h, const void* v, int64_t v_stride_t, int64_t v_stride_h,
+                                  void* k_cache, int64_t kc_stride_r, int64_t kc_stride_h, void* v_cache,
+                                  int64_t vc_stride_r, int64_t vc_stride_h, int64_t cache_rows, const void* slots,
+                                  const float* cos, const float* sin, int64_t table_rows, const void* positions,
+                                  int index_bits, int64_t tokens, int64_t q_heads, int64_t k_heads, int64_t head_dim,
+                                  int64_t rot_dim, int interleaved, int dtype, void* stream);
+
+/* Attention of a batch of requests over a prefix that all of them share and, per
+ * request, its own cache rows.  q [batch, q_len, q_heads, head_dim]; k_prefix /
+ * v_prefix [prefix_len, kv_heads, head_dim]; k_own / v_own [batch, own_len, kv_heads,
+ * head_dim], of which request b has the first lens[b] (int32, device; clamped to
+ * 0..own_len) and nothing after them reaches a result, whatever it holds.  Element
+ * strides per dimension, the last dimension contiguous.  q head h reads k/v head
+ * h / (q_heads / kv_heads).  Every query sees the whole prefix; of its request's own
+ * rows query i sees all or, causal != 0, those up to lens[b] - q_len + i (the queries
+ * are the last q_len rows).  out [batch, q_len, q_heads, head_dim] contiguous, lse
+ * (natural log-sum-exp of the scaled scores) fp32 [batch, q_heads, q_len]; a query
+ * that sees nothing gives 0 and -inf.  dtype F16/BF16, head_dim 64 or 128.  Pointers
+ * and strides of q, k and v: multiples of 16 bytes.  workspace: 16-byte aligned,
+ * jo_shared_prefix_attention_workspace(...) bytes (-1: bad arguments). */
+JO_API int64_t jo_shared_prefix_attention_workspace(int64_t batch, int64_t q_len, int64_t q_heads, int64_t kv_heads,
+                                                    int64_t head_dim, int64_t prefix_len, int64_t own_len);
+JO_API int jo_shared_prefix_attention(void* out, float* lse, const void* q, int64_t q_stride_b, int64_t q_stride_t,
+                                      int64_t q_stride_h, const void* k_prefix, int64_t kp_stride_t,
+                                      int64_t kp_stride_h, const void* v_prefix, int64_t vp_stride_t,
+                                      int64_t vp_stride_h, const void* k_own, int64_t ko_stride_b,
+                                      int64_t ko_stride_t, int64_t ko_stride_h, const void* v_own,
+                                      int64_t vo_stride_b, int64_t vo_stride_t, int64_t vo_stride_h,
+                                      const int32_t* lens, int64_t batch, int64_t q_len, int64_t q_heads,
+                                      int64_t kv_heads, int64_t head_dim, int64_t prefix_len, int64_t own_len,
+                                      int causal, float scale, void* workspace, int64_t workspace_bytes, int dtype,
+                                      void* stream);
 
 #ifdef __cplusplus
 }

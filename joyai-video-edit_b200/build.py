@@ -6,7 +6,7 @@ Produces, inside ``joyomni_ops/`` next to this file:
   CUDA kernel, compiled with ``nvcc -gencode arch=compute_100a,code=sm_100a``;
   no torch dependency, static cudart.
 * ``_C.so`` -- the ``torch.ops.joyomni_ops`` registration shim
-  (``csrc/torch_shim.cpp``), linked against ``libjoyomni_b200.so`` through an
+  (``csrc/torch_shim*.cpp``), linked against ``libjoyomni_b200.so`` through an
   ``$ORIGIN`` rpath.
 
 Run ``python build.py`` (or ``__graft_entry__.build()``).  Object files go to
@@ -37,7 +37,9 @@ NVCC_FLAGS = ARCH + [
     f"-I{INCLUDE}", f"-I{CSRC}",
 ]
 CU_SOURCES = ["common.cu", "rows.cu", "rows_bf16.cu", "rows_f16.cu", "rows_f32.cu", "qkv.cu", "elementwise.cu",
-              "fp8_gemm.cu", "temb.cu", "host_io.cu", "attn.cu", "peer.cu"]
+              "fp8_gemm.cu", "temb.cu", "host_io.cu", "attn.cu", "peer.cu",
+              "rotary.cu", "fp4_quant.cu", "fp4_gemm.cu", "prefix_attn.cu"]
+SHIM_SOURCES = ["torch_shim.cpp", "torch_shim_prefix.cpp"]
 LIB = OUT / "libjoyomni_b200.so"
 SHIM = OUT / "_C.so"
 
@@ -59,7 +61,7 @@ def _stale(target: Path, deps: list[Path]) -> bool:
 
 
 def _headers() -> list[Path]:
-    return sorted(CSRC.glob("*.cuh")) + sorted(INCLUDE.glob("*.h"))
+    return sorted(CSRC.glob("*.cuh")) + sorted(CSRC.glob("*.h")) + sorted(INCLUDE.glob("*.h"))
 
 
 def build_lib(jobs: int = 8) -> Path:
@@ -82,28 +84,33 @@ def build_lib(jobs: int = 8) -> Path:
     return LIB
 
 
-def build_shim() -> Path:
+def build_shim(jobs: int = 8) -> Path:
     import torch
     from torch.utils import cpp_extension as ce
 
-    src = CSRC / "torch_shim.cpp"
-    if not _stale(SHIM, [src, LIB] + _headers()):
+    if not _stale(SHIM, [CSRC / s for s in SHIM_SOURCES] + [LIB] + _headers()):
         return SHIM
     inc = [f"-I{p}" for p in ce.include_paths("cuda")] + [f"-I{INCLUDE}"]
     libdirs = [p for p in ce.library_paths("cuda")]
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
-    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
-           "-DTORCH_EXTENSION_NAME=_C", "-w", *inc, str(src), "-o", str(SHIM),
-           *[f"-L{p}" for p in libdirs], f"-L{OUT}",
-           "-ljoyomni_b200", "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu",
-           "-Wl,-rpath,$ORIGIN"]
-    _run(cmd)
+    flags = ["-O2", "-std=c++17", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={abi}", "-DTORCH_EXTENSION_NAME=_C", "-w", *inc]
+    objs, todo = [], []
+    for name in SHIM_SOURCES:
+        src = CSRC / name
+        obj = BUILD / (src.stem + ".o")
+        objs.append(obj)
+        if _stale(obj, [src] + _headers()):
+            todo.append(["g++", *flags, "-c", str(src), "-o", str(obj)])
+    with cf.ThreadPoolExecutor(max_workers=jobs) as ex:
+        list(ex.map(_run, todo))
+    _run(["g++", "-shared", *map(str, objs), "-o", str(SHIM), *[f"-L{p}" for p in libdirs], f"-L{OUT}",
+          "-ljoyomni_b200", "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-Wl,-rpath,$ORIGIN"])
     return SHIM
 
 
 def build(jobs: int = 8) -> None:
     build_lib(jobs)
-    build_shim()
+    build_shim(jobs)
 
 
 def clean() -> None:

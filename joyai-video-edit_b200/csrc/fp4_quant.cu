@@ -1,0 +1,397 @@
+// Quantisation of rows to 4 bits (formats and layouts: fp4.cuh) and back.
+//
+//   JO_FP4_NV: r[m] = max(max|x[m, :]|, 1e-8) / (6 * 448)
+//              s[m, b] = e4m3((max|x[m, block b]| / r[m]) / 6)
+//              code = e2m1(x / (s r)), 0 where s is 0; value = code s r
+//   JO_FP4_MX: s[m, b] = 2^clamp(floor(log2 max|x[m, block b]|) - 2, -127, 127)
+//              code = e2m1(x / s), saturating at 6; value = code s
+//
+// Every quotient is the correctly rounded fp32 one and every conversion rounds to
+// the nearest, ties to even, so codes and scales follow from these lines bit for bit
+// (a zero's sign is not kept).  The row scale puts a row's largest block scale at the
+// top of e4m3's range; it multiplies the product's row like the per-token FP8 scale.
+//
+// A row (NV) or block (MX) that holds an infinity or a NaN gets a NaN scale and zero
+// codes: the whole row (block) is NaN after a product or jo_dequant_fp4.
+//
+// Bound: HBM (16-bit inputs: 2 bytes read and 0.5625 or 0.53 written per element).
+// A lane holds whole runs of 16 elements (32 bytes of a 16-bit row, one 256-bit
+// load), so a block's maximum needs no shuffle (MX: one) and its 16 codes leave as
+// one 8-byte store.  One pass: the row stays in registers between its maximum and
+// its codes.  `warps` warps share a row, each lane holding up to kRuns runs.
+#include <cuda_fp4.h>
+
+#include "fp4.cuh"
+#include "quant.cuh"
+
+namespace jo {
+namespace {
+
+// 32 bytes in one instruction, read once.
+__device__ __forceinline__ void ld_stream32(const void* p, uint32_t (&w)[8]) {
+  asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+               : "l"(p));
+}
+
+// A run of 16 consecutive elements of a row, as it lies in memory.
+template <typename T>
+struct Run {
+  static constexpr int kWords = 16 * sizeof(T) / 4;
+  uint32_t w[kWords];
+
+  // align: bytes that every run's address is a multiple of (32, 16 or less)
+  __device__ __forceinline__ void load(const T* p, int align) {
+    if (align == 32) {
+      uint32_t v[8];
+#pragma unroll
+      for (int i = 0; i < kWords / 8; ++i) {
+        ld_stream32(reinterpret_cast<const uint8_t*>(p) + 32 * i, v);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) w[8 * i + j] = v[j];
+      }
+    } else if (align == 16) {
+#pragma unroll
+      for (int i = 0; i < kWords / 4; ++i) {
+        const uint4 v = ld_stream(reinterpret_cast<const uint8_t*>(p) + 16 * i);
+        w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
+      }
+    } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) w[i] = __ldg(reinterpret_cast<const uint32_t*>(p) + i);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t lo = __ldg(reinterpret_cast<const unsigned short*>(p) + 2 * i);
+        const uint32_t hi = __ldg(reinterpret_cast<const unsigned short*>(p) + 2 * i + 1);
+        w[i] = lo | (hi << 16);
+      }
+    }
+  }
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) w[i] = 0;
+  }
+  // max|x| as the bits of a non-negative float, which order as integers do; an
+  // infinity or a NaN comes out at 0x7f800000 or above
+  __device__ __forceinline__ uint32_t amax_bits() const {
+    uint32_t m = 0;
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < kWords; ++i) m = max(m, w[i] & 0x7fffffffu);
+      return m;
+    } else {
+#pragma unroll
+      for (int i = 0; i < kWords; ++i) m = absmax16x2<T>(m, w[i]);
+      return __float_as_uint(bits16_to_f<T>(amax16_bits(m)));
+    }
+  }
+  __device__ __forceinline__ float2 pair(int i) const {
+    if constexpr (sizeof(T) == 4) {
+      return make_float2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
+    } else if constexpr (sizeof(T) == 2) {
+      return make_float2(bits16_to_f<T>(w[i] & 0xffffu), bits16_to_f<T>(w[i] >> 16));
+    }
+  }
+};
+
+__device__ __forceinline__ uint32_t e2m1x2(float2 v) {  // v.x in the low half of the byte
+  return (uint32_t)__nv_cvt_float2_to_fp4x2(v, __NV_E2M1, cudaRoundNearest);
+}
+
+// 16 codes of a run of a block with scale step d: e2m1 of the correctly rounded
+// x / d (quant.cuh; no code depends on a quotient below 2^-3).
+template <typename T>
+__device__ __forceinline__ uint2 codes_of(const Run<T>& r, float d) {
+  const float2 nd = f2(-d), rc = f2(__frcp_rn(d));
+  uint32_t c[2] = {0, 0};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) c[i / 4] |= e2m1x2(div2_ms(r.pair(i), nd, rc)) << (8 * (i % 4));
+  return make_uint2(c[0], c[1]);
+}
+// The same for a power-of-two step, whose reciprocal is exact.
+template <typename T>
+__device__ __forceinline__ uint2 codes_of_pow2(const Run<T>& r, float inv) {
+  uint32_t c[2] = {0, 0};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) c[i / 4] |= e2m1x2(__fmul2_rn(r.pair(i), f2(inv))) << (8 * (i % 4));
+  return make_uint2(c[0], c[1]);
+}
+
+struct QuantArgs {
+  uint8_t* q;
+  int64_t ldq;
+  uint8_t* bs;
+  float* rs;
+  const void* x;
+  int64_t ldx;
+  int64_t rows, rows_padded;
+  int runs;     // 16-element runs per row
+  int tiles_k;  // 512-byte scale tiles along K
+  int warps;    // per row
+  int align;
+};
+
+constexpr int kQuantThreads = 256;
+
+// kMaxThreads: 256 (up to 8 warps per row, registers to hold the runs) or 1024.
+template <typename T, bool kMx, int kRuns, int kMaxThreads>
+__global__ void __launch_bounds__(kMaxThreads) quant_fp4_kernel(const QuantArgs a) {
+  __shared__ uint32_t row_max[32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int rows_per_cta = blockDim.x / (32 * a.warps);
+  const int w = warp % a.warps;
+  const int64_t m = (int64_t)blockIdx.x * rows_per_cta + warp / a.warps;
+  pdl_wait();
+  pdl_trigger();
+  const bool live = m < a.rows;
+  Run<T> run[kRuns];
+  uint32_t top[kRuns];
+  uint32_t all = 0;
+  const T* xr = reinterpret_cast<const T*>(a.x) + m * a.ldx;
+#pragma unroll
+  for (int j = 0; j < kRuns; ++j) {
+    const int u = (j * a.warps + w) * 32 + lane;
+    if (live && u < a.runs)
+      run[j].load(xr + (int64_t)u * 16, a.align);
+    else
+      run[j].clear();
+  }
+#pragma unroll
+  for (int j = 0; j < kRuns; ++j) {
+    top[j] = run[j].amax_bits();
+    if constexpr (kMx)
+      top[j] = max(top[j], __shfl_xor_sync(0xffffffffu, top[j], 1));  // the other half of the block of 32
+    else
+      all = max(all, top[j]);
+  }
+  float rs = 0.f;
+  bool bad_row = false;
+  if constexpr (!kMx) {
+    all = __reduce_max_sync(0xffffffffu, all);
+    if (a.warps > 1) {  // one row per CTA
+      if (lane == 0) row_max[warp] = all;
+      __syncthreads();
+      all = __reduce_max_sync(0xffffffffu, lane < a.warps ? row_max[lane] : 0u);
+    }
+    bad_row = all >= 0x7f800000u;
+    rs = __fdiv_rn(fmaxf(__uint_as_float(all), 1e-8f), 6.f * kFp8Max);
+    if (live && w == 0 && lane == 0) a.rs[m] = bad_row ? __int_as_float(0x7fffffff) : rs;
+  }
+  if (m >= a.rows_padded) return;
+  constexpr int kLanes = kMx ? 8 : 4;  // lanes that share a 4-byte word of block scales
+#pragma unroll
+  for (int j = 0; j < kRuns; ++j) {
+    const int u = (j * a.warps + w) * 32 + lane;
+    uint32_t code = 0;  // the block scale's byte
+    uint2 c = make_uint2(0, 0);
+    if (live && u < a.runs) {
+      if constexpr (kMx) {
+        const uint32_t e = top[j] >> 23;
+        if (e == 255) {
+          code = 255;
+        } else {
+          code = e > 2 ? e - 2 : 0;
+          c = codes_of_pow2(run[j], __uint_as_float((254u - code) << 23));  // 2^-(code - 127)
+        }
+      } else if (!bad_row) {
+        const float t = __fdiv_rn(__fdiv_rn(__uint_as_float(top[j]), rs), 6.f);
+        code = (uint32_t)__nv_cvt_float_to_fp8(t, __NV_SATFINITE, __NV_E4M3);
+        if (code) c = codes_of(run[j], __fmul_rn(fp4_scale_value<false>((uint8_t)code), rs));
+      }
+      *reinterpret_cast<uint2*>(a.q + m * a.ldq + (int64_t)u * 8) = c;
+    }
+    // four block scales to a word
+    const int b = kMx ? u >> 1 : u;
+    uint32_t word = code << (8 * (b & 3));
+#pragma unroll
+    for (int o = kMx ? 2 : 1; o < kLanes; o <<= 1) word |= __shfl_xor_sync(0xffffffffu, word, o);
+    if ((lane & (kLanes - 1)) == 0 && (b >> 2) < a.tiles_k)
+      *reinterpret_cast<uint32_t*>(a.bs + fp4_scale_offset(m, b, a.tiles_k)) = word;
+  }
+}
+
+struct DequantArgs {
+  void* out;
+  int64_t ldo;
+  const uint8_t* q;
+  int64_t ldq;
+  const uint8_t* bs;
+  const float* rs;
+  int64_t total;  // runs
+  int runs, tiles_k;
+  int vec;  // elements per store
+};
+
+// Store 16 floats as T, `vec` elements at a time.
+template <typename T>
+__device__ __forceinline__ void store16(T* p, const float* f, int vec) {
+  if (vec == Elt<T>::kVec) {
+#pragma unroll
+    for (int i = 0; i < 16; i += Elt<T>::kVec) st_global(p + i, Elt<T>::pack(f + i));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) p[i] = Elt<T>::from_f(f[i]);
+  }
+}
+
+template <typename T, bool kMx>
+__global__ void __launch_bounds__(kQuantThreads) dequant_fp4_kernel(const DequantArgs a) {
+  pdl_wait();
+  pdl_trigger();
+  for (int64_t i = (int64_t)blockIdx.x * kQuantThreads + threadIdx.x; i < a.total;
+       i += (int64_t)gridDim.x * kQuantThreads) {
+    const int64_t m = i / a.runs;
+    const int u = (int)(i - m * a.runs);
+    const uint2 c = __ldg(reinterpret_cast<const uint2*>(a.q + m * a.ldq + (int64_t)u * 8));
+    const float s = fp4_scale_value<kMx>(__ldg(a.bs + fp4_scale_offset(m, kMx ? u >> 1 : u, a.tiles_k)));
+    const float r = kMx ? 1.f : __ldg(a.rs + m);
+    const uint32_t w[2] = {c.x, c.y};
+    float f[16];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const __half2_raw h = __nv_cvt_fp4x2_to_halfraw2((__nv_fp4x2_storage_t)((w[j / 4] >> (8 * (j % 4))) & 0xffu), __NV_E2M1);
+      const float2 v = __half22float2(__half2(h));
+      f[2 * j] = kMx ? v.x * s : __fmul_rn(v.x * s, r);  // code * s is exact
+      f[2 * j + 1] = kMx ? v.y * s : __fmul_rn(v.y * s, r);
+    }
+    store16(reinterpret_cast<T*>(a.out) + m * a.ldo + (int64_t)u * 16, f, a.vec);
+  }
+}
+
+template <typename T, bool kMx, int kRuns>
+int launch_quant(const QuantArgs& a, cudaStream_t st) {
+  const int per_cta = a.warps > 1 ? 1 : kQuantThreads / 32;
+  const int64_t grid = cdiv(a.rows_padded, per_cta);
+  const auto kern = a.warps <= kQuantThreads / 32 ? quant_fp4_kernel<T, kMx, kRuns, kQuantThreads>
+                                                  : quant_fp4_kernel<T, kMx, kRuns, 1024>;
+  if (cudaError_t e = launch_pdl(kern, dim3((unsigned)grid), dim3((unsigned)(32 * a.warps * per_cta)), 0, st, a))
+    return launch_failed(e, "quant_fp4");
+  return after_launch("quant_fp4_kernel");
+}
+
+template <typename T, bool kMx>
+int dispatch_quant(QuantArgs a, const DeviceInfo* di, cudaStream_t st) {
+  // A row's runs in warps-full: as few warps per row as still give every SM 32
+  // warps, each lane with up to 6 runs in flight (fp32: 4).
+  const int full = (int)cdiv(a.runs, 32);
+  constexpr int kMost = sizeof(T) == 4 ? 4 : 6;
+  int runs = 1;
+  for (int r : {2, 4, 6})
+    if (r <= kMost && (a.rows * cdiv(full, r) >= (int64_t)32 * di->sm_count || cdiv(full, runs) > 32)) runs = r;
+  if (runs > full) runs = full <= 1 ? 1 : full <= 2 ? 2 : full <= 4 ? 4 : 6;
+  a.warps = (int)cdiv(full, runs);
+  if (a.warps > 32) return fail(JO_ERR_SHAPE, "quant_fp4: rows of at most %d elements", 32 * 32 * 16 * kMost);
+  switch (runs) {
+    case 1: return launch_quant<T, kMx, 1>(a, st);
+    case 2: return launch_quant<T, kMx, 2>(a, st);
+    case 4: return launch_quant<T, kMx, 4>(a, st);
+    default:
+      if constexpr (kMost == 6) return launch_quant<T, kMx, 6>(a, st);
+      return launch_quant<T, kMx, 4>(a, st);
+  }
+}
+
+int check_fp4(const char* op, const void* q, int64_t ldq, const void* bs, const void* rs, int64_t rows, int64_t cols,
+              int format, int dtype) {
+  if (format != JO_FP4_NV && format != JO_FP4_MX) return fail(JO_ERR_INVALID, "%s: unknown 4-bit format %d", op, format);
+  if (dtype != JO_F32 && dtype != JO_F16 && dtype != JO_BF16)
+    return fail(JO_ERR_DTYPE, "%s: values must be fp32, fp16 or bf16", op);
+  if (rows < 0 || cols < 0) return fail(JO_ERR_SHAPE, "%s: negative size", op);
+  if (cols % 32 || cols == 0) return fail(JO_ERR_SHAPE, "%s: the row length must be a positive multiple of 32", op);
+  if (cols > INT32_MAX || rows > INT32_MAX) return fail(JO_ERR_SHAPE, "%s: size too large", op);
+  if (rows == 0) return JO_OK;
+  if (!q || !bs || (format == JO_FP4_NV && !rs)) return fail(JO_ERR_INVALID, "%s: null operand", op);
+  if (ldq < cols / 2 || ldq % 8 || (reinterpret_cast<uintptr_t>(q) & 7))
+    return fail(JO_ERR_ALIGN, "%s: packed rows must start on 8 bytes and not overlap", op);
+  if (!aligned16(bs)) return fail(JO_ERR_ALIGN, "%s: block scales must be 16-byte aligned", op);
+  return JO_OK;
+}
+
+}  // namespace
+}  // namespace jo
+
+using namespace jo;
+
+extern "C" {
+
+int64_t jo_fp4_scale_bytes(int64_t rows, int64_t cols, int format) {
+  if (rows < 0 || cols < 0 || (format != JO_FP4_NV && format != JO_FP4_MX)) return -1;
+  return cdiv(rows, 128) * fp4_tiles_k(cols, format) * 512;
+}
+
+int jo_quant_fp4(void* q, int64_t q_row_stride, void* block_scale, float* row_scale, const void* x,
+                 int64_t x_row_stride, int64_t rows, int64_t cols, int format, int dtype, void* stream) {
+  const char* op = "quant_fp4";
+  const DeviceInfo* di;
+  if (int s = device_info(&di)) return s;
+  if (int s = check_fp4(op, q, q_row_stride, block_scale, row_scale, rows, cols, format, dtype)) return s;
+  if (rows == 0) return JO_OK;
+  if (!x) return fail(JO_ERR_INVALID, "%s: null operand", op);
+  if (rows > 1 && x_row_stride < cols) return fail(JO_ERR_SHAPE, "%s: row stride smaller than the row", op);
+  const int64_t esize = dtype == JO_F32 ? 4 : 2;
+  QuantArgs a{};
+  a.q = (uint8_t*)q;
+  a.ldq = q_row_stride;
+  a.bs = (uint8_t*)block_scale;
+  a.rs = row_scale;
+  a.x = x;
+  a.ldx = x_row_stride;
+  a.rows = rows;
+  a.rows_padded = cdiv(rows, 128) * 128;
+  a.runs = (int)(cols / 16);
+  a.tiles_k = (int)fp4_tiles_k(cols, format);
+  const uint64_t at = reinterpret_cast<uintptr_t>(x) | (uint64_t)(rows > 1 ? x_row_stride * esize : 0);
+  a.align = at % 32 == 0 ? 32 : at % 16 == 0 ? 16 : (int)esize;
+  if (at % esize) return fail(JO_ERR_ALIGN, "%s: x must be aligned to its elements", op);
+  cudaStream_t st = (cudaStream_t)stream;
+  const bool mx = format == JO_FP4_MX;
+  switch (dtype) {
+    case JO_F32: return mx ? dispatch_quant<float, true>(a, di, st) : dispatch_quant<float, false>(a, di, st);
+    case JO_F16: return mx ? dispatch_quant<__half, true>(a, di, st) : dispatch_quant<__half, false>(a, di, st);
+    default:
+      return mx ? dispatch_quant<__nv_bfloat16, true>(a, di, st) : dispatch_quant<__nv_bfloat16, false>(a, di, st);
+  }
+}
+
+int jo_dequant_fp4(void* out, int64_t out_row_stride, const void* q, int64_t q_row_stride, const void* block_scale,
+                   const float* row_scale, int64_t rows, int64_t cols, int format, int dtype, void* stream) {
+  const char* op = "dequant_fp4";
+  const DeviceInfo* di;
+  if (int s = device_info(&di)) return s;
+  if (int s = check_fp4(op, q, q_row_stride, block_scale, row_scale, rows, cols, format, dtype)) return s;
+  if (rows == 0) return JO_OK;
+  if (!out) return fail(JO_ERR_INVALID, "%s: null operand", op);
+  if (rows > 1 && out_row_stride < cols) return fail(JO_ERR_SHAPE, "%s: row stride smaller than the row", op);
+  const int64_t esize = dtype == JO_F32 ? 4 : 2;
+  DequantArgs a{};
+  a.out = out;
+  a.ldo = out_row_stride;
+  a.q = (const uint8_t*)q;
+  a.ldq = q_row_stride;
+  a.bs = (const uint8_t*)block_scale;
+  a.rs = row_scale;
+  a.runs = (int)(cols / 16);
+  a.tiles_k = (int)fp4_tiles_k(cols, format);
+  a.total = rows * a.runs;
+  const uint64_t at = reinterpret_cast<uintptr_t>(out) | (uint64_t)(rows > 1 ? out_row_stride * esize : 0);
+  if (at % esize) return fail(JO_ERR_ALIGN, "%s: out must be aligned to its elements", op);
+  a.vec = at % 16 == 0 ? (int)(16 / esize) : 1;
+  auto launch = [&](auto kern) -> int {
+    const int64_t cap = (int64_t)di->sm_count * occupancy((const void*)kern, kQuantThreads, 0);
+    const int64_t need = cdiv(a.total, kQuantThreads);
+    if (cudaError_t e = launch_pdl(kern, dim3((unsigned)(need < cap ? need : cap)), dim3(kQuantThreads), 0,
+                                   (cudaStream_t)stream, a))
+      return launch_failed(e, op);
+    return after_launch("dequant_fp4_kernel");
+  };
+  const bool mx = format == JO_FP4_MX;
+  switch (dtype) {
+    case JO_F32: return mx ? launch(dequant_fp4_kernel<float, true>) : launch(dequant_fp4_kernel<float, false>);
+    case JO_F16: return mx ? launch(dequant_fp4_kernel<__half, true>) : launch(dequant_fp4_kernel<__half, false>);
+    default:
+      return mx ? launch(dequant_fp4_kernel<__nv_bfloat16, true>) : launch(dequant_fp4_kernel<__nv_bfloat16, false>);
+  }
+}
+
+}  // extern "C"

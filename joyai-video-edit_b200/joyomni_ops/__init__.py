@@ -13,7 +13,11 @@ built extension raises ImportError exactly like the reference.
 New fused ops on the same path live in the same namespace
 (``qkv_norm_rope_pack``, ``gated_residual``, ``gated_residual_norm_scale_shift``,
 ``gelu_tanh``, ``silu_mul``, ``timestep_embedding``, ``timestep_mlp``, ``rmsnorm_quant_fp8``,
-``norm_scale_shift_quant_fp8``).
+``norm_scale_shift_quant_fp8``), as do the operators of an attention layer whose
+requests share a long prefix: matrices in 4 bits and their product (``quant_fp4``,
+``dequant_fp4``, ``fp4_scaled_mm``, ``fp4_linear``), the rotary embedding
+(``rotary_embed``, ``rotary_embed_backward``, ``rotary_embed_append``) and
+``shared_prefix_attention``; ``joyomni_ops.prefix`` runs them together.
 """
 import glob
 import os
@@ -56,6 +60,15 @@ __all__ = [
     "gelu_quant_fp8",
     "attn_merge",
     "gated_residual_norm_scale_shift_quant_fp8",
+    # attention layer of a batch of requests that share a long prefix
+    "quant_fp4",
+    "dequant_fp4",
+    "fp4_scaled_mm",
+    "fp4_linear",
+    "rotary_embed",
+    "rotary_embed_backward",
+    "rotary_embed_append",
+    "shared_prefix_attention",
     "library_path",
 ]
 
@@ -218,6 +231,51 @@ def _fake_rmsnorm_quant_fp8(x, weight, eps):
 def _fake_norm_scale_shift_quant_fp8(x, gamma, beta, scale, shift, norm_type, eps):
     return (x.new_empty(x.shape, dtype=torch.float8_e4m3fn),
             x.new_empty((x.shape[0], 1), dtype=torch.float32))
+
+
+_FP4_FORMATS = {"nvfp4": 0, "mxfp4": 1}  # JO_FP4_NV, JO_FP4_MX
+_FP4_BLOCK = (16, 32)
+_FP4_SCALE = (torch.float8_e4m3fn, torch.float8_e8m0fnu)
+
+
+@torch.library.register_fake("joyomni_ops::quant_fp4")
+def _fake_quant_fp4(x, format):
+    m, k = x.shape
+    blocks = k // _FP4_BLOCK[format]
+    return (x.new_empty((m, k // 2), dtype=torch.uint8),
+            x.new_empty(((m + 127) // 128, (blocks + 3) // 4, 32, 4, 4), dtype=_FP4_SCALE[format]),
+            x.new_empty((m if format == 0 else 0, 1), dtype=torch.float32))
+
+
+@torch.library.register_fake("joyomni_ops::dequant_fp4")
+def _fake_dequant_fp4(q, block_scale, row_scale, dtype):
+    return q.new_empty((q.shape[0], 2 * q.shape[1]), dtype=dtype)
+
+
+@torch.library.register_fake("joyomni_ops::fp4_scaled_mm")
+def _fake_fp4_scaled_mm(mat_a, mat_b, block_a, block_b, scales_a, scales_b, out_dtype, bias=None):
+    return mat_a.new_empty((mat_a.shape[0], mat_b.shape[0]), dtype=out_dtype)
+
+
+@torch.library.register_fake("joyomni_ops::fp4_linear")
+def _fake_fp4_linear(x, mat_b, block_b, scales_b, bias=None):
+    return x.new_empty((x.shape[0], mat_b.shape[0]))
+
+
+@torch.library.register_fake("joyomni_ops::rotary_embed")
+def _fake_rotary_embed(q, k, cos, sin, positions, interleaved, inverse):
+    return q.new_empty(q.shape), q.new_empty(k.shape if k is not None else (0,))
+
+
+@torch.library.register_fake("joyomni_ops::rotary_embed_append")
+def _fake_rotary_embed_append(q, k, v, cos, sin, positions, slots, k_cache, v_cache, interleaved):
+    return q.new_empty(q.shape)
+
+
+@torch.library.register_fake("joyomni_ops::shared_prefix_attention")
+def _fake_shared_prefix_attention(q, k_prefix, v_prefix, k_own, v_own, lens, causal, scale):
+    b, n, h, _ = q.shape
+    return q.new_empty(q.shape), q.new_empty((b, h, n), dtype=torch.float32)
 
 
 # ---------------------------------------------------------------- wrappers (reference signatures)
@@ -384,3 +442,88 @@ def rmsnorm_quant_fp8(x, weight, eps=1e-6):
 def norm_scale_shift_quant_fp8(x, gamma, beta, scale, shift, norm_type="layer", eps=1e-6):
     """(q e4m3 [M, N], scale fp32 [M, 1]) of bf16(Norm(x)*(1+scale)+shift)."""
     return _ops.norm_scale_shift_quant_fp8(x, gamma, beta, scale, shift, _norm_code(norm_type), eps)
+
+
+# ---------------------------------------------------------------- attention over a shared prefix
+def _fp4_code(format: str) -> int:
+    return _FP4_FORMATS.get(format, -1)  # an unknown name becomes -1, which the op rejects
+
+
+def quant_fp4(x, format="nvfp4"):
+    """Rows of x [M, K] (bf16, fp16 or fp32; K a multiple of 32) in 4 bits: (q, block_scale, row_scale).
+
+    q: uint8 [M, K/2], two e2m1 codes to a byte (the even element low).  "nvfp4": blocks of 16 with e4m3
+    block scales and an fp32 row scale [M, 1]; "mxfp4": blocks of 32 with power-of-two block scales,
+    row_scale None.  block_scale: tiles [ceil(M/128), ceil(blocks/4), 32, 4, 4], where row m and block b of
+    a tile sit at [m % 32, m // 32, b].  The rounding rules stand in ``include/joyomni_b200.h``."""
+    q, block, row = _ops.quant_fp4(x, _fp4_code(format))
+    return q, block, row if row.shape[0] == x.shape[0] and block.dtype == torch.float8_e4m3fn else None
+
+
+def dequant_fp4(q, block_scale, row_scale=None, dtype=torch.bfloat16):
+    """The values that quant_fp4's output stands for, [M, K] of dtype."""
+    return _ops.dequant_fp4(q, block_scale, row_scale, dtype)
+
+
+def fp4_scaled_mm(mat_a, mat_b, block_a, block_b, scales_a, scales_b, out_dtype, bias: Optional[torch.Tensor] = None):
+    """(A @ B^T) * scales_b * scales_a (+ bias) of two matrices in 4 bits, A [M, K] and B [N, K] as quant_fp4
+    gives them (codes, block scales, row scales), summed in fp32: [M, N] of out_dtype (bf16 or fp16)."""
+    return _ops.fp4_scaled_mm(mat_a, mat_b, block_a, block_b, scales_a, scales_b, out_dtype, bias)
+
+
+def fp4_linear(x, mat_b, block_b, scales_b=None, bias: Optional[torch.Tensor] = None):
+    """A Linear layer in 4 bits: quant_fp4 of x [M, K] in the weight's format, then fp4_scaled_mm with the
+    weight (mat_b, block_b, scales_b = quant_fp4(weight [N, K])); [M, N] of x's dtype (bf16 or fp16)."""
+    return _ops.fp4_linear(x, mat_b, block_b, scales_b, bias)
+
+
+class _RotaryEmbed(torch.autograd.Function):
+    """rotary_embed with its gradient; the tables and positions have none."""
+
+    @staticmethod
+    def forward(ctx, q, k, cos, sin, positions, interleaved):
+        ctx.save_for_backward(cos, sin, positions)
+        ctx.interleaved = interleaved
+        qo, ko = _ops.rotary_embed(q, k, cos, sin, positions, interleaved, False)
+        return qo, ko if k is not None else None
+
+    @staticmethod
+    def backward(ctx, dq, dk):
+        cos, sin, positions = ctx.saved_tensors
+        dq, dk = rotary_embed_backward(dq, dk, cos, sin, positions, ctx.interleaved)
+        return dq, dk, None, None, None, None
+
+
+def rotary_embed(q, k, cos, sin, positions, interleaved=False):
+    """Rotary position embedding of q [T, H, D] and k [T, HK, D] (or None): the tables' rows cos/sin (fp32
+    [P, R/2]) at positions (int [T]) rotate the first R elements of each head, in pairs (2i, 2i+1) if
+    interleaved, else (i, i + R/2); the other elements are copied.  fp32 math, one rounding.  Differentiable
+    in q and k.  A position outside the tables gives NaN.  Returns (q, k) (k None if it was)."""
+    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+        return _RotaryEmbed.apply(q, k, cos, sin, positions, interleaved)
+    qo, ko = _ops.rotary_embed(q, k, cos, sin, positions, interleaved, False)
+    return qo, ko if k is not None else None
+
+
+def rotary_embed_backward(dq, dk, cos, sin, positions, interleaved=False):
+    """Gradients with respect to rotary_embed's q and k from those of its outputs: the inverse rotation."""
+    qo, ko = _ops.rotary_embed(dq, dk, cos, sin, positions, interleaved, True)
+    return qo, ko if dk is not None else None
+
+
+def rotary_embed_append(q, k, v, cos, sin, positions, slots, k_cache, v_cache, interleaved=False):
+    """rotary_embed for serving: returns the rotated q [T, H, D] and writes the rotated k and v [T, HK, D] into
+    rows slots [T] (the positions' dtype) of k_cache / v_cache [rows, HK, D].  A slot outside the cache (a
+    padding token, -1) writes nothing; slots that repeat leave one of their rows."""
+    return _ops.rotary_embed_append(q, k, v, cos, sin, positions, slots, k_cache, v_cache, interleaved)
+
+
+def shared_prefix_attention(q, k_prefix, v_prefix, k_own, v_own, lens, causal=True, scale=None):
+    """Attention of q [B, L, H, D] over a prefix that all requests share (k_prefix / v_prefix [P, HK, D]) and
+    each request's own rows (the first lens [B] (int32) of k_own / v_own [B, S, HK, D]; what lies after them
+    is not used, whatever it holds).  Every query sees the whole prefix; causal: the L queries are the last
+    rows of their request, so query i sees own rows up to lens - L + i.  H a multiple of HK, D 64 or 128,
+    bf16 or fp16; scale: 1/sqrt(D) by default.  Returns (out [B, L, H, D], lse fp32 [B, H, L], the natural
+    log-sum-exp of the scaled scores); a query that sees nothing gives 0 and -inf."""
+    return _ops.shared_prefix_attention(q, k_prefix, v_prefix, k_own, v_own, lens, causal,
+                                        q.shape[-1] ** -0.5 if scale is None else scale)

@@ -22,6 +22,7 @@ JO_ERR_UNSUPPORTED = -6
 
 JO_F32, JO_F16, JO_BF16, JO_E4M3 = 0, 1, 2, 3
 JO_NORM_LAYER, JO_NORM_RMS = 0, 1
+JO_FP4_NV, JO_FP4_MX = 0, 1
 
 
 class JoView4(C.Structure):
@@ -71,6 +72,15 @@ SIGNATURES = {
     "jo_gelu_quant_fp8": [P, I64, P, P, I64, I64, I64, I32, P],
     "jo_gated_residual_norm_scale_shift_quant_fp8": [P, I64, P, I64, P, P, I64, P, I64, P, I64, I64, P, P, P, P,
                                                      I64, I64, I64, I64, I32, I32, F32, P],
+    "jo_fp4_scale_bytes": [I64, I64, I32],
+    "jo_quant_fp4": [P, I64, P, P, P, I64, I64, I64, I32, I32, P],
+    "jo_dequant_fp4": [P, I64, P, I64, P, P, I64, I64, I32, I32, P],
+    "jo_fp4_scaled_mm": [P, I64, P, I64, P, I64, P, P, P, P, P, I64, I64, I64, I32, I32, P],
+    "jo_rotary_embed": [P, I64, I64] * 4 + [P, P, I64, P, I32, I64, I64, I64, I64, I64, I32, I32, I32, P],
+    "jo_rotary_embed_append": [P, I64, I64] * 6 + [I64, P, P, P, I64, P, I32, I64, I64, I64, I64, I64, I32, I32, P],
+    "jo_shared_prefix_attention_workspace": [I64] * 7,
+    "jo_shared_prefix_attention": [P, P] + [P, I64, I64, I64] + [P, I64, I64] * 2 + [P, I64, I64, I64] * 2
+                                  + [P] + [I64] * 7 + [I32, F32, P, I64, I32, P],
     "jo_ipc_alloc": [I64, PP],
     "jo_ipc_free": [P],
     "jo_ipc_handle": [P, P],
@@ -81,7 +91,8 @@ SIGNATURES = {
     "jo_peer_copy": [P, P, I64, P],
 }
 JO_IPC_HANDLE_BYTES = 64
-_RESTYPES = {"jo_status_name": C.c_char_p, "jo_last_error": C.c_char_p, "jo_launch_count": C.c_uint64}
+_RESTYPES = {"jo_status_name": C.c_char_p, "jo_last_error": C.c_char_p, "jo_launch_count": C.c_uint64,
+             "jo_fp4_scale_bytes": C.c_int64, "jo_shared_prefix_attention_workspace": C.c_int64}
 
 _lib = None
 
