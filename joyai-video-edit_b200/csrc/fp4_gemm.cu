@@ -2,80 +2,664 @@
 //
 //   D[m, n] = out((sum_k A[m, k] B[n, k]) * scale_b[n] * scale_a[m] (+ bias[n]))
 //
-// with A and B the codes times their block scales, summed in fp32.
-#include <cuda_fp4.h>
-
+// with A and B the codes times their block scales.  The block scales enter the tensor
+// cores' product itself: tcgen05.mma.kind::mxf4nvf4.block_scale multiplies each run of
+// 16 (or 32) products by the two scales, which it reads from tensor memory, and sums in
+// fp32; the row scales and the bias are applied in the epilogue.
+//
+// Both kernels stream K in blocks of 128 bytes (256 elements, one 128-byte swizzle row)
+// through a ring of mbarrier stages: codes by 2-D TMA, scale tiles (512 bytes per 128
+// rows x 4 blocks, as they lie) by 3-D TMA, then tcgen05.cp (32 lanes x 128 bits, to all
+// four lane quadrants) of each scale tile and four products of K = 64.  One thread issues
+// both; the tensor-core pipe runs them in order, so nothing waits in between.  Rows and
+// blocks past the end arrive as zero from the TMA.
+//
+//   fp4_gemm_pair_kernel   256 x 256 tiles on CTA pairs (cta_group::2)
+//   fp4_gemm_rows_kernel   for few rows of A: 128 rows of B x up to 128 rows of A, K split
+//                          over a cluster
+//
+// Every mbarrier wait is bounded (pipeline.cuh), as in the FP8 product.
 #include "fp4.cuh"
+#include "tcgen05.cuh"
 
 namespace jo {
 namespace {
 
-struct Fp4Operand {
-  const uint8_t* q;
-  int64_t ld;
-  const uint8_t* bs;
-  const float* rs;  // null: 1
+constexpr int kKBytes = 128;                // of K per stage
+constexpr int kKElems = 2 * kKBytes;        // 256
+constexpr int kSteps = 4;                   // products of K = 64 per stage
+constexpr int kChunk = 512;                 // bytes of a scale tile
+
+template <bool kMx>
+struct Fmt {
+  static constexpr int kTiles = kMx ? 2 : 4;  // scale tiles per 128 rows and stage
+  static constexpr int kScale = kTiles * kChunk;
+  static constexpr int kCols = kTiles * 4;  // tensor-memory columns of 128 rows' scales of a stage
 };
+
+// Instruction descriptor, block-scaled: e2m1 x e2m1, both K-major; the scale ids pick the
+// byte pair of each 32-bit tensor-memory cell that a K = 64 product of blocks of 32 uses.
+template <bool kMx>
+__device__ __forceinline__ constexpr uint32_t fp4_idesc(int m, int n, int id) {
+  return ((uint32_t)id << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)kMx << 23) |
+         ((uint32_t)(m >> 4) << 24) | ((uint32_t)id << 29);
+}
+// Scale tile in shared memory: 32 rows of 16 bytes, no swizzle, 8-row groups 128 B apart.
+__device__ __forceinline__ uint64_t scale_desc(uint32_t saddr) {
+  return (uint64_t)((saddr >> 4) & 0x3FFF) | (uint64_t)(128 >> 4) << 32 | (uint64_t)1 << 46;
+}
+template <bool kPair>
+__device__ __forceinline__ void scale_copy(uint32_t taddr, uint64_t desc) {
+  if constexpr (kPair)
+    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+  else
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+#define JO_FP4_MMA(GROUP, VEC)                                                                              \
+  asm volatile(                                                                                             \
+      "{\n\t.reg .pred p;\n\t"                                                                              \
+      "setp.ne.b32 p, %6, 0;\n\t"                                                                           \
+      "tcgen05.mma.cta_group::" GROUP ".kind::mxf4nvf4.block_scale.scale_vec::" VEC                         \
+      " [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),                                                    \
+      "l"(ad), "l"(bd), "r"(idesc), "r"(sfa), "r"(sfb), "r"((uint32_t)accumulate)                           \
+      : "memory")
+template <bool kPair, bool kMx>
+__device__ __forceinline__ void fp4_mma(uint32_t d, uint64_t ad, uint64_t bd, uint32_t idesc, uint32_t sfa,
+                                        uint32_t sfb, bool accumulate) {
+  if constexpr (kPair && kMx)
+    JO_FP4_MMA("2", "2X");
+  else if constexpr (kPair)
+    JO_FP4_MMA("2", "4X");
+  else if constexpr (kMx)
+    JO_FP4_MMA("1", "2X");
+  else
+    JO_FP4_MMA("1", "4X");
+}
+#undef JO_FP4_MMA
+
+// One stage: scales to tensor memory at `sf` (A's, then B's), then its products.  gb: 128-row
+// groups of B's scales.
+template <bool kPair, bool kMx>
+__device__ __forceinline__ void stage_products(uint32_t acc, uint32_t a0, uint32_t b0, uint32_t sa0, uint32_t sb0,
+                                               uint32_t sf, int m, int n, int gb, int steps, bool first) {
+  using F = Fmt<kMx>;
+#pragma unroll
+  for (int j = 0; j < F::kTiles; ++j) {
+    scale_copy<kPair>(sf + j * 4, scale_desc(sa0 + j * kChunk));
+    for (int g = 0; g < gb; ++g)
+      scale_copy<kPair>(sf + F::kCols + j * 4 * gb + g * 4, scale_desc(sb0 + g * F::kScale + j * kChunk));
+  }
+#pragma unroll
+  for (int kk = 0; kk < kSteps; ++kk) {
+    if (kk >= steps) break;
+    const int j = kMx ? kk >> 1 : kk;
+    fp4_mma<kPair, kMx>(acc, sw128_desc(a0 + kk * 32), sw128_desc(b0 + kk * 32),
+                        fp4_idesc<kMx>(m, n, kMx ? 2 * (kk & 1) : 0), sf + j * 4, sf + F::kCols + j * 4 * gb,
+                        !(first && kk == 0));
+  }
+}
+
 struct Fp4GemmArgs {
   void* d;
   int64_t ldd;
-  Fp4Operand a, b;
+  const float* sa;  // null: 1
+  const float* sb;
   const void* bias;
-  int m, n, k, tiles_k;
+  int m, n, k;
+  int tiles_m, tiles_n;
+  unsigned int* fault;
 };
 
-constexpr int kTile = 64, kDepth = 32;
+__device__ __forceinline__ int steps_of(int k, int kb) { return min(kSteps, (k - kb * kKElems + 63) / 64); }
+
+// ------------------------------------------------------------------ CTA pairs
+// As the FP8 product's pair kernel (CTA rank r of a (2,1,1) cluster loads A rows and B rows
+// [128 r, 128 r + 128) of a 256 x 256 tile, the leader issues for both), with, per stage, the
+// scales of the CTA's own 128 rows of A and of all 256 rows of B, which each CTA's half of
+// the product needs whole.
+//
+// Tensor memory: two accumulators of 256 columns and two stages of scales (2 x 48 columns)
+// are more than the 512 there are, so the accumulators overlap by 96 columns, at 0 and 160,
+// the scales at 416.  An epilogue first takes its accumulator's overlapped columns into
+// registers; the next tile's products start then, while it works on the other 160.
+constexpr int kAccStep = 160, kOverlap = 96, kScaleCol = 416;
+constexpr int kPairM = 256, kPairN = 256;
+constexpr int kEpiWarps = 8;
+constexpr int kPairThreads = 64 + 32 * kEpiWarps;
 
 template <bool kMx>
-__device__ __forceinline__ void stage(float (*dst)[kTile + 1], const Fp4Operand& o, int row0, int rows, int k0, int tiles_k) {
-  // 64 rows x 32 elements; thread: 8 elements (4 bytes) of one row
-  const int r = threadIdx.x >> 2, c = (threadIdx.x & 3) * 8, row = row0 + r;
-  uint32_t w = 0;
-  float s = 0.f;
-  if (row < rows) {
-    w = *reinterpret_cast<const uint32_t*>(o.q + row * o.ld + (k0 + c) / 2);
-    s = fp4_scale_value<kMx>(o.bs[fp4_scale_offset(row, (k0 + c) / (kMx ? 32 : 16), tiles_k)]);
-  }
+struct PairSmem {
+  using F = Fmt<kMx>;
+  static constexpr int kStages = kMx ? 6 : 5;
+  static constexpr int kOp = 128 * kKBytes;  // 16 KB of codes
+  static constexpr int kStage = 2 * kOp + 3 * F::kScale;
+  static constexpr int kA = 0, kB = kStages * kOp;
+  static constexpr int kSA = 2 * kStages * kOp, kSB = kSA + kStages * F::kScale;
+  static constexpr int kBars = kSB + kStages * 2 * F::kScale;
+  static constexpr int kBytes = kBars + 256 + 1024 /*align*/;
+};
+
+// 16 columns of a row: scales, bias, rounding, two 16-byte stores.
+template <typename OutT>
+__device__ __forceinline__ void store16(const Fp4GemmArgs& g, const uint32_t* r, int n0, float s_a, bool row_ok,
+                                        OutT* drow) {
+  const OutT* bias = reinterpret_cast<const OutT*>(g.bias);
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const __half2_raw h = __nv_cvt_fp4x2_to_halfraw2((__nv_fp4x2_storage_t)((w >> (8 * j)) & 0xffu), __NV_E2M1);
-    const float2 v = __half22float2(__half2(h));
-    dst[c + 2 * j][r] = v.x * s;
-    dst[c + 2 * j + 1][r] = v.y * s;
+  for (int h = 0; h < 2; ++h) {
+    const int n = n0 + 8 * h;
+    if (n >= g.n) break;
+    float o[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e] = __uint_as_float(r[8 * h + e]);
+    if (g.sb) {
+      const float4 s0 = __ldg(reinterpret_cast<const float4*>(g.sb + n));
+      const float4 s1 = __ldg(reinterpret_cast<const float4*>(g.sb + n + 4));
+      const float s[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
+#pragma unroll
+      for (int e = 0; e < 8; ++e) o[e] *= s[e];
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e] *= s_a;
+    if (bias) {
+      float b[8];
+      Elt<OutT>::unpack(__ldg(reinterpret_cast<const uint4*>(bias + n)), b);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) o[e] += b[e];
+    }
+    if (row_ok) st_global(drow + n, Elt<OutT>::pack(o));
   }
 }
 
 template <typename OutT, bool kMx>
-__global__ void __launch_bounds__(256) fp4_gemm_kernel(const Fp4GemmArgs g) {
-  __shared__ float sa[kDepth][kTile + 1], sb[kDepth][kTile + 1];
-  const int m0 = blockIdx.y * kTile, n0 = blockIdx.x * kTile;
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  float acc[4][4] = {};
-  for (int k0 = 0; k0 < g.k; k0 += kDepth) {
-    stage<kMx>(sa, g.a, m0, g.m, k0, g.tiles_k);
-    stage<kMx>(sb, g.b, n0, g.n, k0, g.tiles_k);
-    __syncthreads();
-#pragma unroll 8
-    for (int k = 0; k < kDepth; ++k)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(sa[k][ty * 4 + i], sb[k][tx * 4 + j], acc[i][j]);
-    __syncthreads();
+__global__ void __launch_bounds__(kPairThreads, 1)
+    fp4_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                         const __grid_constant__ CUtensorMap map_sa, const __grid_constant__ CUtensorMap map_sb,
+                         const Fp4GemmArgs args) {
+  using S = PairSmem<kMx>;
+  using F = Fmt<kMx>;
+  constexpr int kStages = S::kStages;
+  unsigned int* const fault = args.fault;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw_base = smem_u32(smem_raw);
+  const uint32_t base = (raw_base + 1023u) & ~1023u;  // identical offsets in both CTAs
+  uint8_t* gbase = smem_raw + (base - raw_base);
+  const uint32_t bars = base + S::kBars;
+  auto full_bar = [&](int s) { return bars + 8u * s; };
+  auto empty_bar = [&](int s) { return bars + 8u * (kStages + s); };
+  const uint32_t tfull = bars + 8u * (2 * kStages), drained = tfull + 8, done = tfull + 16;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gbase + (tfull + 24 - base));
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_rank();
+  const bool leader = rank == 0;
+  const int cluster = (int)(blockIdx.x >> 1), nclusters = (int)(gridDim.x >> 1);
+  const int num_tiles = args.tiles_m * args.tiles_n;
+  const int kblocks = (args.k + kKElems - 1) / kKElems;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(full_bar(s), 1);
+      mbar_init(empty_bar(s), 1);
+    }
+    mbar_init(tfull, 1);
+    mbar_init(drained, 2 * kEpiWarps * 32);  // the epilogue threads of both CTAs
+    mbar_init(done, 1);
+    mbar_init_fence();
   }
-  for (int i = 0; i < 4; ++i) {
-    const int m = m0 + ty * 4 + i;
-    if (m >= g.m) break;
-    for (int j = 0; j < 4; ++j) {
-      const int n = n0 + tx * 4 + j;
-      if (n >= g.n) break;
-      float v = acc[i][j];
-      if (g.b.rs) v *= g.b.rs[n];
-      if (g.a.rs) v *= g.a.rs[m];
-      if (g.bias) v += Elt<OutT>::to_f(reinterpret_cast<const OutT*>(g.bias)[n]);
-      reinterpret_cast<OutT*>(g.d)[m * g.ldd + n] = Elt<OutT>::from_f(v);
+  if (warp == 1) {  // same warp in both CTAs: the pair allocation is collective
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                 "r"(512)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  __syncthreads();
+  cluster_sync();  // both CTAs' barriers initialised before any cross-CTA signal
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  pdl_wait();
+  pdl_trigger();
+
+  if (warp == 0) {
+    if (lane == 0) {
+      // ---------------- TMA producer (both CTAs)
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      int issued = 0;
+      for (int tile = cluster; tile < num_tiles && ok; tile += nclusters) {
+        const int tm = tile / args.tiles_n, tn = tile - tm * args.tiles_n;
+        for (int kb = 0; kb < kblocks; ++kb) {
+          if (!mbar_wait(empty_bar(stage), phase ^ 1u, fault)) {
+            ok = false;
+            break;
+          }
+          const uint32_t fb = cluster_addr(full_bar(stage), 0);
+          if (leader) mbar_expect_tx(full_bar(stage), 2 * S::kStage);
+          tma_load_2d_pair(base + S::kA + stage * S::kOp, &map_a, kb * kKBytes, tm * kPairM + (int)rank * 128, fb);
+          tma_load_2d_pair(base + S::kB + stage * S::kOp, &map_b, kb * kKBytes, tn * kPairN + (int)rank * 128, fb);
+          tma_load_3d_pair(base + S::kSA + stage * F::kScale, &map_sa, 0, kb * F::kTiles, tm * 2 + (int)rank, fb);
+          tma_load_3d_pair(base + S::kSB + stage * 2 * F::kScale, &map_sb, 0, kb * F::kTiles, tn * 2, fb);
+          ++issued;
+          if (++stage == kStages) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+      }
+      // drain (leader): the pair's copies into every issued stage must have landed (the
+      // leader's full barriers count both CTAs' bytes); the peer is held by the final
+      // cluster barrier until then
+      if (leader)
+        for (int j = max(0, issued - kStages); j < issued; ++j)
+          mbar_wait(full_bar(j % kStages), (j / kStages) & 1, fault);
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && leader) {
+      // ---------------- MMA issuer (leader CTA only)
+      int stage = 0;
+      uint32_t phase = 0;
+      int count = 0;  // stages so far: scales alternate between two column sets
+      bool ok = true;
+      int i = 0;
+      for (int tile = cluster; tile < num_tiles && ok; tile += nclusters, ++i) {
+        if (i > 0 && !mbar_wait(drained, (i - 1) & 1, fault)) break;
+        tc_fence_after();
+        const uint32_t acc = tmem + (i & 1) * kAccStep;
+        for (int kb = 0; kb < kblocks; ++kb, ++count) {
+          if (!mbar_wait(full_bar(stage), phase, fault)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          stage_products<true, kMx>(acc, base + S::kA + stage * S::kOp, base + S::kB + stage * S::kOp,
+                                    base + S::kSA + stage * F::kScale, base + S::kSB + stage * 2 * F::kScale,
+                                    tmem + kScaleCol + (count & 1) * 3 * F::kCols, kPairM, kPairN, 2,
+                                    steps_of(args.k, kb), kb == 0);
+          // the stage is reusable in both CTAs once these products have read it
+          tc_commit_pair(empty_bar(stage));
+          tc_commit_pair(cluster_addr(empty_bar(stage), 1));
+          if (++stage == kStages) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+        tc_commit_pair(tfull);  // accumulator complete, in both CTAs
+        tc_commit_pair(cluster_addr(tfull, 1));
+      }
+      // TMEM is freed below and the peer's shared memory is read by these products: wait
+      // until every one of them has retired
+      tc_commit_pair(done);
+      mbar_wait(done, 0, fault);
+    }
+  } else {
+    // ---------------- epilogue: warps 2..9 of both CTAs; warp w: lanes 32*(w%4).., and of
+    // both parts of the accumulator's columns the half (w-2)/4
+    const int q = warp & 3, half = (warp - 2) >> 2;
+    OutT* D = reinterpret_cast<OutT*>(args.d);
+    int i = 0;
+    for (int tile = cluster; tile < num_tiles; tile += nclusters, ++i) {
+      const int tm = tile / args.tiles_n, tn = tile - tm * args.tiles_n;
+      if (!mbar_wait(tfull, i & 1, fault)) break;
+      tc_fence_after();
+      const int row = tm * kPairM + (int)rank * 128 + q * 32 + lane;
+      const bool row_ok = row < args.m;
+      const float s_a = row_ok && args.sa ? __ldg(args.sa + row) : 1.f;
+      OutT* drow = D + (int64_t)(row_ok ? row : 0) * args.ldd;
+      const bool odd = i & 1;
+      const uint32_t t_acc = tmem + ((uint32_t)(q * 32) << 16) + (odd ? kAccStep : 0);
+      const int c0 = (odd ? 0 : kAccStep) + half * (kOverlap / 2);      // shared with the other accumulator
+      const int c1 = (odd ? kOverlap : 0) + half * (kAccStep / 2);      // this one's alone
+      {
+        uint32_t r[48];
+#pragma unroll
+        for (int j = 0; j < 3; ++j) tmem_ld16(t_acc + c0 + 16 * j, r + 16 * j);
+#pragma unroll
+        for (int j = 0; j < 3; ++j) tmem_ld_wait(r + 16 * j);
+        tc_fence_before();
+        if (leader)
+          mbar_arrive(drained);
+        else
+          mbar_arrive_cluster(cluster_addr(drained, 0));
+#pragma unroll
+        for (int j = 0; j < 3; ++j)
+          store16<OutT>(args, r + 16 * j, tn * kPairN + c0 + 16 * j, s_a, row_ok, drow);
+      }
+#pragma unroll 1
+      for (int j = 0; j < 5; ++j) {
+        uint32_t r[16];
+        tmem_ld16(t_acc + c1 + 16 * j, r);
+        tmem_ld_wait(r);
+        store16<OutT>(args, r, tn * kPairN + c1 + 16 * j, s_a, row_ok, drow);
+      }
+      tc_fence_before();
     }
   }
+  __syncthreads();
+  // neither CTA leaves while the other may still signal its barriers or have its shared
+  // memory read by the pair's products
+  cluster_sync();
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+  }
+}
+
+// ------------------------------------------------------------------ few rows
+// B (the weight) takes the tensor cores' 128 rows and A's rows their columns, kCols of them,
+// so a single token costs 16 columns and not 128 rows (kCols < 128 serves one tile of at
+// most kCols rows: a tile's scales start at a 128-row group).  The CTAs of a cluster take
+// contiguous parts of K of one tile; each then receives, from every CTA of the cluster by
+// distributed shared memory, its share of the columns, and adds the parts in the CTAs'
+// order: one result whatever the timing.
+constexpr int kRowsThreads = 192;
+constexpr int kMaxSplit = 8;
+
+template <bool kMx, int kCols>
+struct RowsSmem {
+  using F = Fmt<kMx>;
+  static constexpr int kB = 128 * kKBytes;    // the weight's codes
+  static constexpr int kA = kCols * kKBytes;  // kCols rows of A
+  static constexpr int kStage = kB + kA + 2 * F::kScale;
+  static constexpr int kPart = 128 * kCols * 4;  // received parts
+  static constexpr int kStages = (int)((227 * 1024 - 2048 - kPart) / kStage) < 8
+                                     ? (int)((227 * 1024 - 2048 - kPart) / kStage)
+                                     : 8;
+  static constexpr int kOffB = 0, kOffA = kStages * kB, kOffSB = kOffA + kStages * kA;
+  static constexpr int kOffSA = kOffSB + kStages * F::kScale;
+  static constexpr int kOffPart = kOffSA + kStages * F::kScale;
+  static constexpr int kBars = kOffPart + kPart;
+  static constexpr int kBytes = kBars + 256 + 1024;
+  static constexpr int kTmem = kCols + 64 <= 128 ? 128 : 256;  // accumulator, two stages of scales
+};
+
+template <typename OutT>
+__device__ __forceinline__ void store_one(const Fp4GemmArgs& g, float v, int m, int n, float s_b, float bias) {
+  v *= s_b;
+  if (g.sa) v *= __ldg(g.sa + m);
+  reinterpret_cast<OutT*>(g.d)[(int64_t)m * g.ldd + n] = Elt<OutT>::from_f(v + bias);
+}
+
+template <typename OutT, bool kMx, int kCols>
+__global__ void __launch_bounds__(kRowsThreads, 1)
+    fp4_gemm_rows_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                         const __grid_constant__ CUtensorMap map_sa, const __grid_constant__ CUtensorMap map_sb,
+                         const Fp4GemmArgs args, const int split) {
+  using S = RowsSmem<kMx, kCols>;
+  using F = Fmt<kMx>;
+  constexpr int kStages = S::kStages;
+  static_assert(kStages >= 3, "ring too short");
+  unsigned int* const fault = args.fault;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw_base = smem_u32(smem_raw);
+  const uint32_t base = (raw_base + 1023u) & ~1023u;
+  uint8_t* gbase = smem_raw + (base - raw_base);
+  const uint32_t bars = base + S::kBars;
+  auto full_bar = [&](int s) { return bars + 8u * s; };
+  auto empty_bar = [&](int s) { return bars + 8u * (kStages + s); };
+  const uint32_t tfull = bars + 8u * (2 * kStages);
+  const uint32_t tmem_slot = tfull + 8;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = split > 1 ? (int)cluster_rank() : 0;
+  const int tn = (int)blockIdx.x / split, tm = (int)blockIdx.y;
+  const int kblocks = (args.k + kKElems - 1) / kKElems;
+  const int kb0 = kblocks * rank / split, kb1 = kblocks * (rank + 1) / split;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(full_bar(s), 1);
+      mbar_init(empty_bar(s), 1);
+    }
+    mbar_init(tfull, 1);
+    mbar_init_fence();
+  }
+  if (warp == 1) tmem_alloc(tmem_slot, S::kTmem);
+  __syncthreads();
+  if (split > 1) cluster_sync();  // every CTA of the cluster runs before any part is sent
+  tc_fence_after();
+  const uint32_t tmem = *reinterpret_cast<uint32_t*>(gbase + (tmem_slot - base));
+  pdl_wait();
+  pdl_trigger();
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int stage = 0, issued = 0;
+      uint32_t phase = 0;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (!mbar_wait(empty_bar(stage), phase ^ 1u, fault)) break;
+        mbar_expect_tx(full_bar(stage), S::kStage);
+        tma_load_2d(base + S::kOffB + stage * S::kB, &map_b, kb * kKBytes, tn * 128, full_bar(stage));
+        tma_load_3d(base + S::kOffSB + stage * F::kScale, &map_sb, 0, kb * F::kTiles, tn, full_bar(stage));
+        tma_load_2d(base + S::kOffA + stage * S::kA, &map_a, kb * kKBytes, tm * kCols, full_bar(stage));
+        tma_load_3d(base + S::kOffSA + stage * F::kScale, &map_sa, 0, kb * F::kTiles, tm, full_bar(stage));
+        ++issued;
+        if (++stage == kStages) stage = 0, phase ^= 1u;
+      }
+      for (int j = max(0, issued - kStages); j < issued; ++j)
+        mbar_wait(full_bar(j % kStages), (j / kStages) & 1, fault);
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (!mbar_wait(full_bar(stage), phase, fault)) break;
+        tc_fence_after();
+        const uint32_t sf = tmem + kCols + ((kb - kb0) & 1) * 2 * F::kCols;
+        const uint32_t sb0 = base + S::kOffSB + stage * F::kScale, sa0 = base + S::kOffSA + stage * F::kScale;
+#pragma unroll
+        for (int j = 0; j < F::kTiles; ++j) {
+          scale_copy<false>(sf + j * 4, scale_desc(sb0 + j * kChunk));
+          scale_copy<false>(sf + F::kCols + j * 4, scale_desc(sa0 + j * kChunk));
+        }
+        const uint32_t b0 = base + S::kOffB + stage * S::kB, a0 = base + S::kOffA + stage * S::kA;
+        const int steps = steps_of(args.k, kb);
+#pragma unroll
+        for (int kk = 0; kk < kSteps; ++kk) {
+          if (kk >= steps) break;
+          const int j = kMx ? kk >> 1 : kk;
+          fp4_mma<false, kMx>(tmem, sw128_desc(b0 + kk * 32), sw128_desc(a0 + kk * 32),
+                              fp4_idesc<kMx>(128, kCols, kMx ? 2 * (kk & 1) : 0), sf + j * 4,
+                              sf + F::kCols + j * 4, kb != kb0 || kk != 0);
+        }
+        tc_commit(empty_bar(stage));
+        if (++stage == kStages) stage = 0, phase ^= 1u;
+      }
+      tc_commit(tfull);  // also after a failed wait: everything issued has retired
+      mbar_wait(tfull, 0, fault);
+    }
+  } else {
+    // ---------------- epilogue: thread = row of B (tensor-memory lane), columns = rows of A
+    const int q = warp & 3, nl = q * 32 + lane, n = tn * 128 + nl;
+    const uint32_t t_row = tmem + ((uint32_t)(q * 32) << 16);
+    const bool live = n < args.n;
+    const float s_b = live && args.sb ? __ldg(args.sb + n) : 1.f;
+    const float bias = live && args.bias ? Elt<OutT>::to_f(reinterpret_cast<const OutT*>(args.bias)[n]) : 0.f;
+    const bool ok = mbar_wait(tfull, 0, fault);
+    tc_fence_after();
+    const int share = kCols / split;  // columns that each CTA of the cluster adds up
+#pragma unroll 1
+    for (int c = 0; c < kCols && ok; c += 16) {
+      uint32_t r[16];
+      if (kb1 > kb0) {
+        tmem_ld16(t_row + c, r);
+        tmem_ld_wait(r);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) r[e] = 0;
+      }
+      if (split == 1) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int m = tm * kCols + c + e;
+          if (live && m < args.m) store_one<OutT>(args, __uint_as_float(r[e]), m, n, s_b, bias);
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int to = (c + e) / share;
+          const uint32_t at = base + S::kOffPart + (uint32_t)((rank * share + (c + e) - to * share) * 128 + nl) * 4;
+          asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr(at, to)), "r"(r[e]) : "memory");
+        }
+      }
+    }
+    tc_fence_before();
+  }
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_free(tmem, S::kTmem);
+  }
+  if (split > 1) {
+    cluster_sync();  // every part has arrived, and nothing reaches another CTA any more
+    const int share = kCols / split;
+    const float* part = reinterpret_cast<const float*>(gbase + S::kOffPart);
+    for (int j = threadIdx.x; j < share * 128; j += kRowsThreads) {
+      const int nl = j & 127, c = j >> 7, n = tn * 128 + nl, m = tm * kCols + rank * share + c;
+      if (n >= args.n || m >= args.m) continue;
+      float v = 0.f;
+      for (int r = 0; r < split; ++r) v += part[(r * share + c) * 128 + nl];
+      const float s_b = args.sb ? __ldg(args.sb + n) : 1.f;
+      const float bias = args.bias ? Elt<OutT>::to_f(reinterpret_cast<const OutT*>(args.bias)[n]) : 0.f;
+      store_one<OutT>(args, v, m, n, s_b, bias);
+    }
+  }
+}
+
+// ------------------------------------------------------------------ host side
+int make_code_map(CUtensorMap* map, const void* ptr, int64_t rows, int64_t kbytes, int64_t ld, int box_rows) {
+  auto fn = tensor_map_encoder();
+  if (!fn) return fail(JO_ERR_CUDA, "fp4_scaled_mm: cuTensorMapEncodeTiled unavailable");
+  cuuint64_t dims[2] = {(cuuint64_t)kbytes, (cuuint64_t)rows};
+  cuuint64_t strides[1] = {(cuuint64_t)ld};
+  cuuint32_t box[2] = {(cuuint32_t)kKBytes, (cuuint32_t)box_rows};
+  cuuint32_t estr[2] = {1, 1};
+  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(ptr), dims, strides, box, estr,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(JO_ERR_CUDA, "fp4_scaled_mm: cuTensorMapEncodeTiled failed (%d)", (int)r);
+  return JO_OK;
+}
+// Scale tiles [groups of 128 rows][tiles along K][512 bytes].
+int make_scale_map(CUtensorMap* map, const void* ptr, int64_t groups, int64_t tiles_k, int box_tiles, int box_groups) {
+  auto fn = tensor_map_encoder();
+  if (!fn) return fail(JO_ERR_CUDA, "fp4_scaled_mm: cuTensorMapEncodeTiled unavailable");
+  cuuint64_t dims[3] = {kChunk / 4, (cuuint64_t)tiles_k, (cuuint64_t)groups};
+  cuuint64_t strides[2] = {kChunk, (cuuint64_t)tiles_k * kChunk};
+  cuuint32_t box[3] = {kChunk / 4, (cuuint32_t)box_tiles, (cuuint32_t)box_groups};
+  cuuint32_t estr[3] = {1, 1, 1};
+  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 3, const_cast<void*>(ptr), dims, strides, box, estr,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(JO_ERR_CUDA, "fp4_scaled_mm: cuTensorMapEncodeTiled failed (%d)", (int)r);
+  return JO_OK;
+}
+
+struct Operands {
+  const void* a;
+  const void* b;
+  const void* block_a;
+  const void* block_b;
+  int64_t lda, ldb;
+};
+
+template <bool kMx>
+int make_maps(CUtensorMap* maps, const Operands& o, const Fp4GemmArgs& g, int rows_a, int rows_b, int groups_b) {
+  using F = Fmt<kMx>;
+  const int64_t tk = fp4_tiles_k(g.k, kMx ? JO_FP4_MX : JO_FP4_NV);
+  if (int s = make_code_map(&maps[0], o.a, g.m, g.k / 2, o.lda, rows_a)) return s;
+  if (int s = make_code_map(&maps[1], o.b, g.n, g.k / 2, o.ldb, rows_b)) return s;
+  if (int s = make_scale_map(&maps[2], o.block_a, cdiv(g.m, 128), tk, F::kTiles, 1)) return s;
+  return make_scale_map(&maps[3], o.block_b, cdiv(g.n, 128), tk, F::kTiles, groups_b);
+}
+
+template <typename OutT, bool kMx>
+int launch_pair(const Operands& o, Fp4GemmArgs g, cudaStream_t st, const DeviceInfo* di) {
+  const char* op = "fp4_scaled_mm";
+  using S = PairSmem<kMx>;
+  auto kern = fp4_gemm_pair_kernel<OutT, kMx>;
+  static std::atomic<uint64_t> reserved{0};
+  if (int s = reserve_smem((const void*)kern, S::kBytes, reserved, di, op)) return s;
+  cudaLaunchConfig_t cfg = {};
+  cfg.blockDim = dim3(kPairThreads, 1, 1);
+  cfg.dynamicSmemBytes = S::kBytes;
+  cfg.stream = st;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = 2;
+  at[0].val.clusterDim.y = 1;
+  at[0].val.clusterDim.z = 1;
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // see launch_pdl
+  at[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  static std::atomic<int> resident[64];  // CTA pairs held at once, per device (0 = not asked yet)
+  int pairs = resident[di->ordinal].load(std::memory_order_relaxed);
+  if (!pairs) {
+    cfg.gridDim = dim3(2, 1, 1);
+    cfg.numAttrs = 1;
+    if (cudaOccupancyMaxActiveClusters(&pairs, (const void*)kern, &cfg) != cudaSuccess || pairs < 1) {
+      cudaGetLastError();
+      return fail(JO_ERR_CUDA, "%s: no resident CTA pair", op);
+    }
+    resident[di->ordinal].store(pairs, std::memory_order_relaxed);
+  }
+  g.tiles_m = (int)cdiv(g.m, kPairM);
+  g.tiles_n = (int)cdiv(g.n, kPairN);
+  if ((int64_t)g.tiles_m * g.tiles_n > INT32_MAX) return fail(JO_ERR_SHAPE, "%s: too many tiles", op);
+  CUtensorMap maps[4];
+  if (int s = make_maps<kMx>(maps, o, g, 128, 128, 2)) return s;
+  const int tiles = g.tiles_m * g.tiles_n;
+  cfg.gridDim = dim3(2 * (unsigned)(tiles < pairs ? tiles : pairs), 1, 1);
+  cfg.numAttrs = 2;
+  if (cudaError_t e = cudaLaunchKernelEx(&cfg, kern, maps[0], maps[1], maps[2], maps[3], g)) return launch_failed(e, op);
+  return after_launch("fp4_gemm_pair_kernel");
+}
+
+template <typename OutT, bool kMx, int kCols>
+int launch_rows(const Operands& o, Fp4GemmArgs g, cudaStream_t st, const DeviceInfo* di) {
+  const char* op = "fp4_scaled_mm";
+  using S = RowsSmem<kMx, kCols>;
+  auto kern = fp4_gemm_rows_kernel<OutT, kMx, kCols>;
+  static std::atomic<uint64_t> reserved{0};
+  if (int s = reserve_smem((const void*)kern, S::kBytes, reserved, di, op)) return s;
+  g.tiles_m = (int)cdiv(g.m, kCols);
+  g.tiles_n = (int)cdiv(g.n, 128);
+  if (kCols < 128 && g.tiles_m > 1) return fail(JO_ERR_SHAPE, "%s: %d rows in a tile of %d", op, g.m, kCols);
+  if (g.tiles_m > 65535 || (int64_t)g.tiles_n * kMaxSplit > INT32_MAX) return fail(JO_ERR_SHAPE, "%s: too many tiles", op);
+  // K in as many parts as still leave two stages each, until every SM has a CTA
+  const int64_t tiles = (int64_t)g.tiles_m * g.tiles_n, kblocks = cdiv(g.k, kKElems);
+  int split = 1;
+  while (split < kMaxSplit && tiles * split * 2 <= di->sm_count && kblocks >= split * 4) split *= 2;
+  CUtensorMap maps[4];
+  if (int s = make_maps<kMx>(maps, o, g, kCols, 128, 1)) return s;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(g.tiles_n * split), (unsigned)g.tiles_m, 1);
+  cfg.blockDim = dim3(kRowsThreads, 1, 1);
+  cfg.dynamicSmemBytes = S::kBytes;
+  cfg.stream = st;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = (unsigned)split;
+  at[1].val.clusterDim.y = 1;
+  at[1].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 2;
+  if (cudaError_t e = cudaLaunchKernelEx(&cfg, kern, maps[0], maps[1], maps[2], maps[3], g, split))
+    return launch_failed(e, op);
+  return after_launch("fp4_gemm_rows_kernel");
+}
+
+template <typename OutT, bool kMx>
+int dispatch(const Operands& o, const Fp4GemmArgs& g, cudaStream_t st, const DeviceInfo* di) {
+  // CTA pairs where their 256 x 256 tiles keep most SMs busy
+  const int64_t pair_tiles = cdiv(g.m, kPairM) * cdiv(g.n, kPairN);
+  if (g.m > 128 && pair_tiles * 2 * 2 >= di->sm_count) return launch_pair<OutT, kMx>(o, g, st, di);
+  if (g.m <= 16) return launch_rows<OutT, kMx, 16>(o, g, st, di);
+  if (g.m <= 32) return launch_rows<OutT, kMx, 32>(o, g, st, di);
+  if (g.m <= 64) return launch_rows<OutT, kMx, 64>(o, g, st, di);
+  return launch_rows<OutT, kMx, 128>(o, g, st, di);
 }
 
 }  // namespace
@@ -96,7 +680,8 @@ int jo_fp4_scaled_mm(void* d, int64_t ldd, const void* a, int64_t lda, const voi
   if (out_dtype != JO_BF16 && out_dtype != JO_F16) return fail(JO_ERR_DTYPE, "%s: out dtype must be bf16/fp16", op);
   if (m == 0 || n == 0) return JO_OK;
   if (k == 0 || k % 32) return fail(JO_ERR_SHAPE, "%s: K must be a positive multiple of 32", op);
-  if (m > INT32_MAX || n > INT32_MAX || k > INT32_MAX) return fail(JO_ERR_SHAPE, "%s: size too large", op);
+  const int64_t most = INT32_MAX - 512;
+  if (m > most || n > most || k > most) return fail(JO_ERR_SHAPE, "%s: size too large", op);
   if (!d || !a || !b || !block_a || !block_b) return fail(JO_ERR_INVALID, "%s: null operand", op);
   if (lda < k / 2 || ldb < k / 2 || ldd < n) return fail(JO_ERR_SHAPE, "%s: leading dimension smaller than the row", op);
   if (lda % 16 || ldb % 16 || n % 8 || ldd % 8)
@@ -104,25 +689,22 @@ int jo_fp4_scaled_mm(void* d, int64_t ldd, const void* a, int64_t lda, const voi
   if (!aligned16(d) || !aligned16(a) || !aligned16(b) || !aligned16(block_a) || !aligned16(block_b) ||
       (scale_b && !aligned16(scale_b)) || (bias && !aligned16(bias)))
     return fail(JO_ERR_ALIGN, "%s: operands must be 16-byte aligned", op);
-  Fp4GemmArgs g{d, ldd, {(const uint8_t*)a, lda, (const uint8_t*)block_a, scale_a},
-                {(const uint8_t*)b, ldb, (const uint8_t*)block_b, scale_b}, bias, (int)m, (int)n, (int)k,
-                (int)fp4_tiles_k(k, format)};
-  const dim3 grid((unsigned)cdiv(n, kTile), (unsigned)cdiv(m, kTile));
-  if (grid.y > 65535) return fail(JO_ERR_SHAPE, "%s: size too large", op);
+  Fp4GemmArgs g{};
+  g.d = d;
+  g.ldd = ldd;
+  g.sa = scale_a;
+  g.sb = scale_b;
+  g.bias = bias;
+  g.m = (int)m;
+  g.n = (int)n;
+  g.k = (int)k;
+  g.fault = di->fault;
+  const Operands o{a, b, block_a, block_b, lda, ldb};
   cudaStream_t st = (cudaStream_t)stream;
   const bool mx = format == JO_FP4_MX;
-  if (out_dtype == JO_BF16) {
-    if (mx)
-      fp4_gemm_kernel<__nv_bfloat16, true><<<grid, 256, 0, st>>>(g);
-    else
-      fp4_gemm_kernel<__nv_bfloat16, false><<<grid, 256, 0, st>>>(g);
-  } else {
-    if (mx)
-      fp4_gemm_kernel<__half, true><<<grid, 256, 0, st>>>(g);
-    else
-      fp4_gemm_kernel<__half, false><<<grid, 256, 0, st>>>(g);
-  }
-  return after_launch("fp4_gemm_kernel");
+  if (out_dtype == JO_BF16)
+    return mx ? dispatch<__nv_bfloat16, true>(o, g, st, di) : dispatch<__nv_bfloat16, false>(o, g, st, di);
+  return mx ? dispatch<__half, true>(o, g, st, di) : dispatch<__half, false>(o, g, st, di);
 }
 
 }  // extern "C"
