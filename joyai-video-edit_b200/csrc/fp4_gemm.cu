@@ -11,7 +11,9 @@
 // through a ring of mbarrier stages: codes by 2-D TMA, scale tiles (512 bytes per 128
 // rows x 4 blocks, as they lie) by 3-D TMA, then tcgen05.cp (32 lanes x 128 bits, to all
 // four lane quadrants) of each scale tile and four products of K = 64.  One thread issues
-// both; the tensor-core pipe runs them in order, so nothing waits in between.  Rows and
+// both; the tensor-core pipe runs them in order, so nothing waits in between.  The issuing
+// warp stays converged and elects the thread at each stage: its addresses are then
+// warp-uniform values, which the instructions' operands need anyway.  Rows and
 // blocks past the end arrive as zero from the TMA.
 //
 //   fp4_gemm_pair_kernel   256 x 256 tiles on CTA pairs (cta_group::2)
@@ -77,25 +79,26 @@ __device__ __forceinline__ void fp4_mma(uint32_t d, uint64_t ad, uint64_t bd, ui
 }
 #undef JO_FP4_MMA
 
-// One stage: scales to tensor memory at `sf` (A's, then B's), then its products.  gb: 128-row
-// groups of B's scales.
-template <bool kPair, bool kMx>
-__device__ __forceinline__ void stage_products(uint32_t acc, uint32_t a0, uint32_t b0, uint32_t sa0, uint32_t sb0,
-                                               uint32_t sf, int m, int n, int gb, int steps, bool first) {
+// One stage: scales to tensor memory at `sf` (A's, then B's), then its products.  ad, bd:
+// descriptors of the stage's codes; sad, sbd: of its scales; kGroups: 128-row groups of B's
+// scales.  `steps` < 4 only in the last stage.
+template <bool kPair, bool kMx, int kM, int kN, int kGroups>
+__device__ __forceinline__ void stage_products(uint32_t acc, uint64_t ad, uint64_t bd, uint64_t sad, uint64_t sbd,
+                                               uint32_t sf, int steps, bool first) {
   using F = Fmt<kMx>;
 #pragma unroll
   for (int j = 0; j < F::kTiles; ++j) {
-    scale_copy<kPair>(sf + j * 4, scale_desc(sa0 + j * kChunk));
-    for (int g = 0; g < gb; ++g)
-      scale_copy<kPair>(sf + F::kCols + j * 4 * gb + g * 4, scale_desc(sb0 + g * F::kScale + j * kChunk));
+    scale_copy<kPair>(sf + j * 4, sad + j * (kChunk >> 4));
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g)
+      scale_copy<kPair>(sf + F::kCols + (j * kGroups + g) * 4, sbd + ((g * F::kScale + j * kChunk) >> 4));
   }
 #pragma unroll
   for (int kk = 0; kk < kSteps; ++kk) {
-    if (kk >= steps) break;
     const int j = kMx ? kk >> 1 : kk;
-    fp4_mma<kPair, kMx>(acc, sw128_desc(a0 + kk * 32), sw128_desc(b0 + kk * 32),
-                        fp4_idesc<kMx>(m, n, kMx ? 2 * (kk & 1) : 0), sf + j * 4, sf + F::kCols + j * 4 * gb,
-                        !(first && kk == 0));
+    if (kk < steps)
+      fp4_mma<kPair, kMx>(acc, ad + 2 * kk, bd + 2 * kk, fp4_idesc<kMx>(kM, kN, kMx ? 2 * (kk & 1) : 0), sf + j * 4,
+                          sf + F::kCols + j * 4 * kGroups, !(first && kk == 0));
   }
 }
 
@@ -122,6 +125,7 @@ __device__ __forceinline__ int steps_of(int k, int kb) { return min(kSteps, (k -
 // are more than the 512 there are, so the accumulators overlap by 96 columns, at 0 and 160,
 // the scales at 416.  An epilogue first takes its accumulator's overlapped columns into
 // registers; the next tile's products start then, while it works on the other 160.
+// Results leave by TMA, 32 rows x 64 columns at a time from a staging box per warp.
 constexpr int kAccStep = 160, kOverlap = 96, kScaleCol = 416;
 constexpr int kPairM = 256, kPairN = 256;
 constexpr int kEpiWarps = 8;
@@ -130,43 +134,58 @@ constexpr int kPairThreads = 64 + 32 * kEpiWarps;
 template <bool kMx>
 struct PairSmem {
   using F = Fmt<kMx>;
-  static constexpr int kStages = kMx ? 6 : 5;
+  static constexpr int kStages = 5;
   static constexpr int kOp = 128 * kKBytes;  // 16 KB of codes
   static constexpr int kStage = 2 * kOp + 3 * F::kScale;
   static constexpr int kA = 0, kB = kStages * kOp;
   static constexpr int kSA = 2 * kStages * kOp, kSB = kSA + kStages * F::kScale;
-  static constexpr int kBars = kSB + kStages * 2 * F::kScale;
+  static constexpr int kBox = 32 * 128;  // an epilogue warp's staging box: 32 rows x 64 columns
+  static constexpr int kOut = (kSB + kStages * 2 * F::kScale + 1023) / 1024 * 1024;
+  static constexpr int kBars = kOut + kEpiWarps * kBox;
   static constexpr int kBytes = kBars + 256 + 1024 /*align*/;
 };
 
-// 16 columns of a row: scales, bias, rounding, two 16-byte stores.
+// 32 accumulator columns of this lane's row: scales, bias, rounding, four 16-byte chunks into
+// the warp's staging box (row = lane, 128-byte swizzle) from chunk `c0` on.
 template <typename OutT>
-__device__ __forceinline__ void store16(const Fp4GemmArgs& g, const uint32_t* r, int n0, float s_a, bool row_ok,
-                                        OutT* drow) {
+__device__ __forceinline__ void stage32(const Fp4GemmArgs& g, const uint32_t* r, int n0, float s_a, uint8_t* box, int lane,
+                                        int c0) {
   const OutT* bias = reinterpret_cast<const OutT*>(g.bias);
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
+  for (int h = 0; h < 4; ++h) {
     const int n = n0 + 8 * h;
-    if (n >= g.n) break;
     float o[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) o[e] = __uint_as_float(r[8 * h + e]);
-    if (g.sb) {
-      const float4 s0 = __ldg(reinterpret_cast<const float4*>(g.sb + n));
-      const float4 s1 = __ldg(reinterpret_cast<const float4*>(g.sb + n + 4));
-      const float s[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
+    if (n < g.n) {  // N is a multiple of 8; columns past it are not stored
+      if (g.sb) {
+        const float4 s0 = __ldg(reinterpret_cast<const float4*>(g.sb + n));
+        const float4 s1 = __ldg(reinterpret_cast<const float4*>(g.sb + n + 4));
+        const float s[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
 #pragma unroll
-      for (int e = 0; e < 8; ++e) o[e] *= s[e];
+        for (int e = 0; e < 8; ++e) o[e] *= s[e];
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) o[e] *= s_a;
+      if (bias) {
+        float b[8];
+        Elt<OutT>::unpack(__ldg(reinterpret_cast<const uint4*>(bias + n)), b);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[e] += b[e];
+      }
     }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) o[e] *= s_a;
-    if (bias) {
-      float b[8];
-      Elt<OutT>::unpack(__ldg(reinterpret_cast<const uint4*>(bias + n)), b);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) o[e] += b[e];
-    }
-    if (row_ok) st_global(drow + n, Elt<OutT>::pack(o));
+    *reinterpret_cast<uint4*>(box + lane * 128 + (((c0 + h) ^ (lane & 7)) << 4)) = Elt<OutT>::pack(o);
+  }
+}
+// The warp's staging box, filled by all lanes, to rows [m0, m0 + 32) x columns [n0, n0 + 64)
+// of D (what lies outside D is clipped by the TMA).
+__device__ __forceinline__ void store_box(const CUtensorMap* map, const Fp4GemmArgs& g, uint32_t box, int n0, int m0,
+                                          int lane) {
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  __syncwarp();
+  if (lane == 0 && n0 < g.n && m0 < g.m) {
+    tma_store_2d(map, box, n0, m0);
+    bulk_commit();
   }
 }
 
@@ -174,7 +193,7 @@ template <typename OutT, bool kMx>
 __global__ void __launch_bounds__(kPairThreads, 1)
     fp4_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                          const __grid_constant__ CUtensorMap map_sa, const __grid_constant__ CUtensorMap map_sb,
-                         const Fp4GemmArgs args) {
+                         const __grid_constant__ CUtensorMap map_d, const Fp4GemmArgs args) {
   using S = PairSmem<kMx>;
   using F = Fmt<kMx>;
   constexpr int kStages = S::kStages;
@@ -189,7 +208,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   const uint32_t tfull = bars + 8u * (2 * kStages), drained = tfull + 8, done = tfull + 16;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gbase + (tfull + 24 - base));
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = warp_index(), lane = threadIdx.x & 31;
   const uint32_t rank = cluster_rank();
   const bool leader = rank == 0;
   const int cluster = (int)(blockIdx.x >> 1), nclusters = (int)(gridDim.x >> 1);
@@ -254,85 +273,108 @@ __global__ void __launch_bounds__(kPairThreads, 1)
           mbar_wait(full_bar(j % kStages), (j / kStages) & 1, fault);
     }
   } else if (warp == 1) {
-    if (lane == 0 && leader) {
+    if (leader) {
       // ---------------- MMA issuer (leader CTA only)
+      const uint64_t ad = sw128_desc(base + S::kA), bd = sw128_desc(base + S::kB);
+      const uint64_t sad = scale_desc(base + S::kSA), sbd = scale_desc(base + S::kSB);
       int stage = 0;
       uint32_t phase = 0;
       int count = 0;  // stages so far: scales alternate between two column sets
       bool ok = true;
       int i = 0;
       for (int tile = cluster; tile < num_tiles && ok; tile += nclusters, ++i) {
-        if (i > 0 && !mbar_wait(drained, (i - 1) & 1, fault)) break;
+        if (i > 0 && !(ok = __all_sync(0xffffffffu, mbar_wait(drained, (i - 1) & 1, fault)))) break;
         tc_fence_after();
         const uint32_t acc = tmem + (i & 1) * kAccStep;
         for (int kb = 0; kb < kblocks; ++kb, ++count) {
-          if (!mbar_wait(full_bar(stage), phase, fault)) {
-            ok = false;
-            break;
-          }
+          if (!(ok = __all_sync(0xffffffffu, mbar_wait(full_bar(stage), phase, fault)))) break;
           tc_fence_after();
-          stage_products<true, kMx>(acc, base + S::kA + stage * S::kOp, base + S::kB + stage * S::kOp,
-                                    base + S::kSA + stage * F::kScale, base + S::kSB + stage * 2 * F::kScale,
-                                    tmem + kScaleCol + (count & 1) * 3 * F::kCols, kPairM, kPairN, 2,
-                                    steps_of(args.k, kb), kb == 0);
-          // the stage is reusable in both CTAs once these products have read it
-          tc_commit_pair(empty_bar(stage));
-          tc_commit_pair(cluster_addr(empty_bar(stage), 1));
+          if (elect_one()) {
+            stage_products<true, kMx, kPairM, kPairN, 2>(
+                acc, ad + stage * (S::kOp >> 4), bd + stage * (S::kOp >> 4), sad + stage * (F::kScale >> 4),
+                sbd + stage * (2 * F::kScale >> 4), tmem + kScaleCol + (count & 1) * 3 * F::kCols,
+                steps_of(args.k, kb), kb == 0);
+            // the stage is reusable in both CTAs once these products have read it
+            tc_commit_pair(empty_bar(stage));
+            tc_commit_pair(cluster_addr(empty_bar(stage), 1));
+            if (kb == kblocks - 1) {  // accumulator complete, in both CTAs
+              tc_commit_pair(tfull);
+              tc_commit_pair(cluster_addr(tfull, 1));
+            }
+          }
+          __syncwarp();
           if (++stage == kStages) {
             stage = 0;
             phase ^= 1u;
           }
         }
-        tc_commit_pair(tfull);  // accumulator complete, in both CTAs
-        tc_commit_pair(cluster_addr(tfull, 1));
       }
       // TMEM is freed below and the peer's shared memory is read by these products: wait
       // until every one of them has retired
-      tc_commit_pair(done);
+      if (elect_one()) tc_commit_pair(done);
+      __syncwarp();
       mbar_wait(done, 0, fault);
     }
   } else {
-    // ---------------- epilogue: warps 2..9 of both CTAs; warp w: lanes 32*(w%4).., and of
-    // both parts of the accumulator's columns the half (w-2)/4
+    // ---------------- epilogue: warps 2..9 of both CTAs; warp w: lanes 32*(w%4).., and the
+    // half (w-2)/4 of the accumulator's columns, as two boxes of 64
     const int q = warp & 3, half = (warp - 2) >> 2;
-    OutT* D = reinterpret_cast<OutT*>(args.d);
+    uint8_t* const box = gbase + S::kOut + (warp - 2) * S::kBox;
+    const uint32_t box_addr = base + S::kOut + (warp - 2) * S::kBox;
+    auto refill = [&]() {  // the last box has left the staging buffer
+      if (lane == 0) bulk_wait_read_all();
+      __syncwarp();
+    };
+    auto drained_by_us = [&]() {
+      tc_fence_before();
+      if (leader)
+        mbar_arrive(drained);
+      else
+        mbar_arrive_cluster(cluster_addr(drained, 0));
+    };
     int i = 0;
     for (int tile = cluster; tile < num_tiles; tile += nclusters, ++i) {
       const int tm = tile / args.tiles_n, tn = tile - tm * args.tiles_n;
-      if (!mbar_wait(tfull, i & 1, fault)) break;
+      if (!__all_sync(0xffffffffu, mbar_wait(tfull, i & 1, fault))) break;
       tc_fence_after();
-      const int row = tm * kPairM + (int)rank * 128 + q * 32 + lane;
-      const bool row_ok = row < args.m;
-      const float s_a = row_ok && args.sa ? __ldg(args.sa + row) : 1.f;
-      OutT* drow = D + (int64_t)(row_ok ? row : 0) * args.ldd;
-      const bool odd = i & 1;
-      const uint32_t t_acc = tmem + ((uint32_t)(q * 32) << 16) + (odd ? kAccStep : 0);
-      const int c0 = (odd ? 0 : kAccStep) + half * (kOverlap / 2);      // shared with the other accumulator
-      const int c1 = (odd ? kOverlap : 0) + half * (kAccStep / 2);      // this one's alone
-      {
-        uint32_t r[48];
-#pragma unroll
-        for (int j = 0; j < 3; ++j) tmem_ld16(t_acc + c0 + 16 * j, r + 16 * j);
-#pragma unroll
-        for (int j = 0; j < 3; ++j) tmem_ld_wait(r + 16 * j);
-        tc_fence_before();
-        if (leader)
-          mbar_arrive(drained);
-        else
-          mbar_arrive_cluster(cluster_addr(drained, 0));
-#pragma unroll
-        for (int j = 0; j < 3; ++j)
-          store16<OutT>(args, r + 16 * j, tn * kPairN + c0 + 16 * j, s_a, row_ok, drow);
-      }
+      const int m0 = tm * kPairM + (int)rank * 128 + q * 32, row = m0 + lane;
+      const float s_a = row < args.m && args.sa ? __ldg(args.sa + row) : 1.f;
+      const int odd = i & 1;
+      const uint32_t t_acc = tmem + ((uint32_t)(q * 32) << 16) + odd * kAccStep;
+      const int n0 = tn * kPairN;
+      if (half == odd) {
+        // none of this half's columns is the other accumulator's
+        drained_by_us();
 #pragma unroll 1
-      for (int j = 0; j < 5; ++j) {
-        uint32_t r[16];
-        tmem_ld16(t_acc + c1 + 16 * j, r);
-        tmem_ld_wait(r);
-        store16<OutT>(args, r, tn * kPairN + c1 + 16 * j, s_a, row_ok, drow);
+        for (int c = half * 128; c < half * 128 + 128; c += 64) {
+          uint32_t r[64];
+          tmem_ld64(t_acc + c, r);
+          refill();
+          stage32<OutT>(args, r, n0 + c, s_a, box, lane, 0);
+          stage32<OutT>(args, r + 32, n0 + c + 32, s_a, box, lane, 4);
+          store_box(&map_d, args, box_addr, n0 + c, m0, lane);
+        }
+      } else {
+        // of [160, 256) (even) or [0, 96) (odd): 64 columns that are a box, 32 of the other box
+        const int whole = odd ? 0 : 192, part = odd ? 64 : 160, rest = odd ? 96 : 128;
+        uint32_t r[64], p[32];
+        tmem_ld32(t_acc + part, p);
+        tmem_ld64(t_acc + whole, r);
+        drained_by_us();
+        refill();
+        stage32<OutT>(args, r, n0 + whole, s_a, box, lane, 0);
+        stage32<OutT>(args, r + 32, n0 + whole + 32, s_a, box, lane, 4);
+        store_box(&map_d, args, box_addr, n0 + whole, m0, lane);
+        uint32_t o[32];
+        tmem_ld32(t_acc + rest, o);
+        refill();
+        stage32<OutT>(args, p, n0 + part, s_a, box, lane, odd ? 0 : 4);
+        stage32<OutT>(args, o, n0 + rest, s_a, box, lane, odd ? 4 : 0);
+        store_box(&map_d, args, box_addr, n0 + (odd ? part : rest), m0, lane);
       }
       tc_fence_before();
     }
+    refill();
   }
   __syncthreads();
   // neither CTA leaves while the other may still signal its barriers or have its shared
@@ -399,7 +441,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
   const uint32_t tfull = bars + 8u * (2 * kStages);
   const uint32_t tmem_slot = tfull + 8;
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = warp_index(), lane = threadIdx.x & 31;
   const int rank = split > 1 ? (int)cluster_rank() : 0;
   const int tn = (int)blockIdx.x / split, tm = (int)blockIdx.y;
   const int kblocks = (args.k + kKElems - 1) / kKElems;
@@ -439,35 +481,26 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
         mbar_wait(full_bar(j % kStages), (j / kStages) & 1, fault);
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      int stage = 0;
-      uint32_t phase = 0;
-      for (int kb = kb0; kb < kb1; ++kb) {
-        if (!mbar_wait(full_bar(stage), phase, fault)) break;
-        tc_fence_after();
-        const uint32_t sf = tmem + kCols + ((kb - kb0) & 1) * 2 * F::kCols;
-        const uint32_t sb0 = base + S::kOffSB + stage * F::kScale, sa0 = base + S::kOffSA + stage * F::kScale;
-#pragma unroll
-        for (int j = 0; j < F::kTiles; ++j) {
-          scale_copy<false>(sf + j * 4, scale_desc(sb0 + j * kChunk));
-          scale_copy<false>(sf + F::kCols + j * 4, scale_desc(sa0 + j * kChunk));
-        }
-        const uint32_t b0 = base + S::kOffB + stage * S::kB, a0 = base + S::kOffA + stage * S::kA;
-        const int steps = steps_of(args.k, kb);
-#pragma unroll
-        for (int kk = 0; kk < kSteps; ++kk) {
-          if (kk >= steps) break;
-          const int j = kMx ? kk >> 1 : kk;
-          fp4_mma<false, kMx>(tmem, sw128_desc(b0 + kk * 32), sw128_desc(a0 + kk * 32),
-                              fp4_idesc<kMx>(128, kCols, kMx ? 2 * (kk & 1) : 0), sf + j * 4,
-                              sf + F::kCols + j * 4, kb != kb0 || kk != 0);
-        }
+    const uint64_t bd = sw128_desc(base + S::kOffB), ad = sw128_desc(base + S::kOffA);
+    const uint64_t sbd = scale_desc(base + S::kOffSB), sad = scale_desc(base + S::kOffSA);
+    int stage = 0;
+    uint32_t phase = 0;
+    for (int kb = kb0; kb < kb1; ++kb) {
+      if (!__all_sync(0xffffffffu, mbar_wait(full_bar(stage), phase, fault))) break;
+      tc_fence_after();
+      if (elect_one()) {
+        stage_products<false, kMx, 128, kCols, 1>(
+            tmem, bd + stage * (S::kB >> 4), ad + stage * (S::kA >> 4), sbd + stage * (F::kScale >> 4),
+            sad + stage * (F::kScale >> 4), tmem + kCols + ((kb - kb0) & 1) * 2 * F::kCols, steps_of(args.k, kb),
+            kb == kb0);
         tc_commit(empty_bar(stage));
-        if (++stage == kStages) stage = 0, phase ^= 1u;
       }
-      tc_commit(tfull);  // also after a failed wait: everything issued has retired
-      mbar_wait(tfull, 0, fault);
+      __syncwarp();
+      if (++stage == kStages) stage = 0, phase ^= 1u;
     }
+    if (elect_one()) tc_commit(tfull);  // also after a failed wait: everything issued has retired
+    __syncwarp();
+    mbar_wait(tfull, 0, fault);
   } else {
     // ---------------- epilogue: thread = row of B (tensor-memory lane), columns = rows of A
     const int q = warp & 3, nl = q * 32 + lane, n = tn * 128 + nl;
@@ -555,6 +588,21 @@ int make_scale_map(CUtensorMap* map, const void* ptr, int64_t groups, int64_t ti
   return JO_OK;
 }
 
+// D [m, n], stored in boxes of 32 rows x 64 columns.
+int make_out_map(CUtensorMap* map, const Fp4GemmArgs& g, bool bf16) {
+  auto fn = tensor_map_encoder();
+  if (!fn) return fail(JO_ERR_CUDA, "fp4_scaled_mm: cuTensorMapEncodeTiled unavailable");
+  cuuint64_t dims[2] = {(cuuint64_t)g.n, (cuuint64_t)g.m};
+  cuuint64_t strides[1] = {(cuuint64_t)g.ldd * 2};
+  cuuint32_t box[2] = {64, 32};
+  cuuint32_t estr[2] = {1, 1};
+  const CUresult r = fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, g.d, dims,
+                        strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(JO_ERR_CUDA, "fp4_scaled_mm: cuTensorMapEncodeTiled failed (%d)", (int)r);
+  return JO_OK;
+}
+
 struct Operands {
   const void* a;
   const void* b;
@@ -606,12 +654,13 @@ int launch_pair(const Operands& o, Fp4GemmArgs g, cudaStream_t st, const DeviceI
   g.tiles_m = (int)cdiv(g.m, kPairM);
   g.tiles_n = (int)cdiv(g.n, kPairN);
   if ((int64_t)g.tiles_m * g.tiles_n > INT32_MAX) return fail(JO_ERR_SHAPE, "%s: too many tiles", op);
-  CUtensorMap maps[4];
+  CUtensorMap maps[5];
   if (int s = make_maps<kMx>(maps, o, g, 128, 128, 2)) return s;
+  if (int s = make_out_map(&maps[4], g, std::is_same<OutT, __nv_bfloat16>::value)) return s;
   const int tiles = g.tiles_m * g.tiles_n;
   cfg.gridDim = dim3(2 * (unsigned)(tiles < pairs ? tiles : pairs), 1, 1);
   cfg.numAttrs = 2;
-  if (cudaError_t e = cudaLaunchKernelEx(&cfg, kern, maps[0], maps[1], maps[2], maps[3], g)) return launch_failed(e, op);
+  if (cudaError_t e = cudaLaunchKernelEx(&cfg, kern, maps[0], maps[1], maps[2], maps[3], maps[4], g)) return launch_failed(e, op);
   return after_launch("fp4_gemm_pair_kernel");
 }
 
