@@ -126,7 +126,7 @@ __device__ __forceinline__ int steps_of(int k, int kb) { return min(kSteps, (k -
 // the scales at 416.  An epilogue first takes its accumulator's overlapped columns into
 // registers; the next tile's products start then, while it works on the other 160.
 // Results leave by TMA, 32 rows x 64 columns at a time from a staging box per warp.
-constexpr int kAccStep = 160, kOverlap = 96, kScaleCol = 416;
+constexpr int kAccStep = 160, kScaleCol = 416;
 constexpr int kPairM = 256, kPairN = 256;
 constexpr int kEpiWarps = 8;
 constexpr int kPairThreads = 64 + 32 * kEpiWarps;

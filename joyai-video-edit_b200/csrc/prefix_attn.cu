@@ -252,7 +252,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
   auto v_full = [&](int s) { return bars + 32 + 8u * (2 * kStages + s); };
   auto v_empty = [&](int s) { return bars + 32 + 8u * (3 * kStages + s); };
   const uint32_t tmem_slot = bars + 32 + 8u * (4 * kStages);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = warp_index(), lane = threadIdx.x & 31;
 
   pdl_wait();  // lens, q, k and v may be the previous kernel's
   pdl_trigger();
@@ -309,35 +309,43 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
       for (int j = max(0, vn - kStages); j < vn; ++j) mbar_wait(v_full(j % kStages), (j / kStages) & 1, a.fault);
     }
   } else if (warp == 5) {
-    if (lane == 0) {
-      // ---------------- MMA issuer
-      constexpr uint32_t idesc_s = attn_idesc<T>(kTileKeys, false), idesc_o = attn_idesc<T>(D, true);
-      bool ok = mbar_wait(q_full, 0, a.fault);
-      int s = 0;
-      uint32_t phase = 0;
-      for (int t = 0; t < n && ok; ++t) {
-        if (!(ok = mbar_wait(k_full(s), phase, a.fault))) break;
-        tc_fence_after();
-        const uint32_t k0 = base + S::kK + s * S::kTile, v0 = base + S::kV + s * S::kTile;
+    // ---------------- MMA issuer: the warp stays converged and elects one thread per tile
+    constexpr uint32_t idesc_s = attn_idesc<T>(kTileKeys, false), idesc_o = attn_idesc<T>(D, true);
+    const uint64_t qd = sw128_desc(base + S::kQ), kd0 = sw128_desc(base + S::kK);
+    const uint64_t vd0 = sw128_desc_mn(base + S::kV, kBox);
+    bool ok = __all_sync(0xffffffffu, mbar_wait(q_full, 0, a.fault));
+    int s = 0;
+    uint32_t phase = 0;
+    for (int t = 0; t < n && ok; ++t) {
+      if (!(ok = __all_sync(0xffffffffu, mbar_wait(k_full(s), phase, a.fault)))) break;
+      tc_fence_after();
+      if (elect_one()) {
+        const uint64_t kd = kd0 + s * (S::kTile >> 4);
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
-          const uint32_t off = (kk / 4) * kBox + (kk % 4) * 32;
-          tc_mma_f16_ss(tmem, sw128_desc(base + S::kQ + off), sw128_desc(k0 + off), idesc_s, kk != 0);
+          const int off = ((kk / 4) * kBox + (kk % 4) * 32) >> 4;
+          tc_mma_f16_ss(tmem, qd + off, kd + off, idesc_s, kk != 0);
         }
         tc_commit(k_empty(s));
         tc_commit(s_full);
-        if (!(ok = mbar_wait(v_full(s), phase, a.fault))) break;
-        if (!(ok = mbar_wait(p_full, t & 1, a.fault))) break;
-        tc_fence_after();
+      }
+      __syncwarp();
+      if (!(ok = __all_sync(0xffffffffu, mbar_wait(v_full(s), phase, a.fault)))) break;
+      if (!(ok = __all_sync(0xffffffffu, mbar_wait(p_full, t & 1, a.fault)))) break;
+      tc_fence_after();
+      if (elect_one()) {
+        const uint64_t vd = vd0 + s * (S::kTile >> 4);
 #pragma unroll
         for (int kk = 0; kk < kTileKeys / 16; ++kk)
-          tc_mma_f16_ts(tmem_o, tmem + kk * 8, sw128_desc_mn(v0 + kk * 2048, kBox), idesc_o, t != 0 || kk != 0);
+          tc_mma_f16_ts(tmem_o, tmem + kk * 8, vd + kk * (2048 >> 4), idesc_o, t != 0 || kk != 0);
         tc_commit(v_empty(s));
-        if (++s == kStages) s = 0, phase ^= 1u;
       }
-      tc_commit(o_full);  // also after a failed wait: everything issued has retired
-      mbar_wait(o_full, 0, a.fault);
+      __syncwarp();
+      if (++s == kStages) s = 0, phase ^= 1u;
     }
+    if (elect_one()) tc_commit(o_full);  // also after a failed wait: everything issued has retired
+    __syncwarp();
+    mbar_wait(o_full, 0, a.fault);
   } else {
     // ---------------- softmax: thread r owns query row r (tensor-memory lane r)
     const int r = threadIdx.x;
