@@ -19,24 +19,27 @@
 // log2-sum-exps.
 //
 // Rows.  All queries that read one k/v head can share its keys whatever request they
-// belong to, so over the prefix a row of the 128-row tensor-core tile is any (request,
-// query, q head of the k/v head's group): the prefix is read once per 128 such rows,
-// not once per request.  Two plans (plan_attention):
+// belong to, so over the prefix a row of a tensor-core tile is any (request, query, q head
+// of the k/v head's group): the prefix is read once for up to 256 such rows, not once per
+// request.  Two plans (plan_attention):
 //   packed  row tiles run across requests; the prefix and each request's own rows are
 //           separate work items, joined afterwards;
-//   fused   row tiles stay within a request and walk the prefix, then its own rows;
-//           taken when that costs hardly more tiles (many queries per request).
-// Where there are fewer items than the GPU holds, their keys are split and joined.
+//   fused   row tiles stay within a request and walk the prefix, then its own rows.
+// Where the items do not fill the GPU evenly, the last ones' keys are split and joined.
 //
-// One item = one CTA of 6 warps, two CTAs per SM so that one's softmax runs while the
-// other's products do:
-//   warp 4  TMA producer: K and V tiles of 128 rows (128-byte swizzle);
-//   warp 5  tcgen05.mma issuer: S = Q K^T (128 x 128, both operands in shared memory),
-//           then O += P V with P from tensor memory and V as it lies ([keys, D], the
-//           MN-major operand); owns the 256 tensor-memory columns (S and, in its place,
-//           P as 16-bit pairs; O);
-//   warps 0-3  load Q, then per tile: S from tensor memory (one row per thread), the
-//           running maximum and sum, P back to tensor memory, O rescaled in place.
+// One CTA per SM walks over the items with two streams, each with its own S, P and O in
+// tensor memory, so that one stream's softmax runs while the other's products do:
+//   an item of more than 128 rows: the streams take its two halves, and share every K and
+//   V tile (64 KB per tile of 128 keys would otherwise exceed what an SM can take in);
+//   an item of up to 128 rows (single tokens): the streams take alternate key tiles of the
+//   same rows and are joined at the end.
+// Warps 0-3 and 4-7: softmax of stream 0 and 1, one row per thread (tensor-memory lane):
+//   S from tensor memory, the running maximum and sum, P back in place of S in two halves
+//   (the product may start on the first), O rescaled in place; Q and the results.
+// Warp 8: TMA producer of K and V tiles of 128 rows (128-byte swizzle) into one ring, in
+//   the order of their first use; it runs ahead across items.
+// Warp 9: tcgen05.mma issuer: S = Q K^T (both operands in shared memory), O += P V with P
+//   from tensor memory and V as it lies ([keys, D], the MN-major operand).
 //
 // P is rounded to q's 16-bit type for the tensor cores (its error averages out over the
 // keys: 2^-9 relative for bf16, like the output's own rounding); l sums the unrounded p.
@@ -45,11 +48,12 @@
 namespace jo {
 namespace {
 
-constexpr int kTileRows = 128;  // queries per tile (UMMA M)
-constexpr int kTileKeys = 128;  // keys per tile (UMMA N of S, K of P V)
-constexpr int kSoftmaxThreads = 128;
-constexpr int kAttnThreads = 192;
-constexpr int kTmemColsAttn = 256;  // S / P: 0..127, O: 128..128+D-1
+constexpr int kTileRows = 128;           // rows per stream (UMMA M)
+constexpr int kItemRows = 2 * kTileRows;  // rows per item at most
+constexpr int kTileKeys = 128;           // keys per tile (UMMA N of S, K of P V)
+constexpr int kSoftmaxThreads = 256;
+constexpr int kAttnThreads = 320;
+constexpr int kColO = 256;  // tensor memory: S / P of the streams at 0 and 128, O at 256 and 384
 constexpr float kRaise = 8.f;
 
 struct AttnArgs {
@@ -58,29 +62,31 @@ struct AttnArgs {
   const void* q;
   int64_t q_b, q_t, q_h;  // element strides
   const int32_t* lens;
-  int64_t prefix;
+  int prefix;
   int batch, lq, heads, group, own;  // heads: of k and v; group: q heads per k/v head; own: rows of the own caches
   int causal;
   float scale_log2;
-  // plan
+  // plan: items 0..items-1 are the row tiles of `groups` groups (packed: k/v heads, fused:
+  // (head, request) pairs), every group's last tile after all others; those from `whole` on
+  // are split in `splits`; then, packed, the own rows of each (request, head)
   int fused;
-  int row_tiles;   // per k/v head over all requests (packed) or per request (fused)
-  int own_tiles;   // packed: row tiles per request
-  int whole;       // fused: items that are not split
-  int items;       // first kind: packed prefix items, or fused items
-  int splits;      // of the items after the first `whole`
-  int own_splits;  // packed: of a request's own rows
-  float* part_o;   // [slots, D]
+  int groups, row_tiles;
+  int items, whole, splits;
+  int own_tiles, own_splits;
+  int blocks;           // work units in all
+  int64_t rows;         // queries per k/v head
+  int64_t slot_tail;    // first slot of the split items' parts
+  int64_t slot_own;     // and of the own rows'; whole items' parts (packed): from 0
+  float* part_o;        // [slots, D]
   float* part_lse;
   unsigned int* fault;
 };
 
-// One CTA's share: rows [row0, row0 + rows) of k/v head h (flat row: (b * Lq + i) * G + g),
-// and tiles [first, last) of the prefix's, then the request's own, keys.
+// One work unit: rows [row0, row0 + rows) of k/v head h (row: (b * Lq + i) * G + g) and tiles
+// [first, last) of the prefix's, then the request's own, keys.
 struct Item {
   int h, b;  // b: the request of the own rows (-1: none)
-  int64_t row0;
-  int rows;
+  int row0, rows;
   int prefix_tiles;  // tiles of the walk that belong to the prefix
   int first, last;
   int len;       // own rows of b
@@ -91,68 +97,71 @@ __device__ __forceinline__ int own_visible(const AttnArgs& a, int len, int i) {
   return a.causal ? min(len, max(0, len - a.lq + i + 1)) : len;
 }
 
+// Group and row tile of an item.
+__device__ __forceinline__ void tile_of(const AttnArgs& a, int item, int& grp, int& t) {
+  const int full = a.groups * (a.row_tiles - 1);
+  if (item < full) {
+    grp = item / (a.row_tiles - 1);
+    t = item - grp * (a.row_tiles - 1);
+  } else {
+    grp = item - full;
+    t = a.row_tiles - 1;
+  }
+}
+
 __device__ Item item_of(const AttnArgs& a, int block) {
   Item it;
   const int per_request = a.lq * a.group;
-  const int ptiles = (int)((a.prefix + kTileKeys - 1) / kTileKeys);
-  int piece = 0, pieces = 1;
+  const int ptiles = (a.prefix + kTileKeys - 1) / kTileKeys;
+  int piece = 0, pieces = 1, t;
   it.slot = -1;
-  int t;
-  bool own;
-  if (a.fused) {
+  const int first_kind = a.whole + (a.items - a.whole) * a.splits;
+  if (block < first_kind) {
     int item = block;
     if (block >= a.whole) {
       const int tail = a.items - a.whole, j = block - a.whole;
-      item = a.whole + j % tail;
       piece = j / tail;
+      item = a.whole + j - piece * tail;
       pieces = a.splits;
-      if (pieces > 1) it.slot = ((int64_t)(item - a.whole) * pieces + piece) * kTileRows;
     }
-    it.h = item / (a.batch * a.row_tiles);
-    const int rest = item - it.h * (a.batch * a.row_tiles);
-    it.b = rest / a.row_tiles;
-    t = rest - it.b * a.row_tiles;
-    it.prefix_tiles = ptiles;
-    own = true;
-  } else {
-    const int64_t rows = (int64_t)a.batch * per_request;
-    const int first_kind = a.items * a.splits;
-    int slot;
-    if (block < first_kind) {
-      const int item = block % a.items;
-      slot = piece = block / a.items;
-      pieces = a.splits;
-      it.h = item / a.row_tiles;
-      it.b = -1;
-      t = item - it.h * a.row_tiles;
-      it.row0 = (int64_t)t * kTileRows;
-      it.rows = (int)min((int64_t)kTileRows, rows - it.row0);
-      it.prefix_tiles = ptiles;
-      own = false;
+    int grp;
+    tile_of(a, item, grp, t);
+    if (a.fused) {
+      it.h = grp / a.batch;
+      it.b = grp - it.h * a.batch;
+      it.row0 = it.b * per_request + t * kItemRows;
+      it.rows = min(kItemRows, per_request - t * kItemRows);
     } else {
-      int j = block - first_kind;
-      piece = j % a.own_splits;
-      pieces = a.own_splits;
-      slot = a.splits + piece;
-      j /= a.own_splits;
-      t = j % a.own_tiles;
-      j /= a.own_tiles;
-      it.h = j % a.heads;
-      it.b = j / a.heads;
-      it.prefix_tiles = 0;
-      own = true;
+      it.h = grp;
+      it.b = -1;
+      it.row0 = t * kItemRows;
+      it.rows = (int)min((int64_t)kItemRows, a.rows - it.row0);
     }
-    if (own) it.row0 = (int64_t)it.b * per_request + t * kTileRows;
-    if (a.splits + a.own_splits > 1) it.slot = ((int64_t)slot * a.heads + it.h) * rows + it.row0;
+    it.prefix_tiles = ptiles;
+    if (item >= a.whole && (pieces > 1 || a.own_splits > 0))
+      it.slot = a.slot_tail + ((int64_t)(item - a.whole) * pieces + piece) * kItemRows;
+    else if (a.own_splits > 0)
+      it.slot = (int64_t)it.h * a.rows + it.row0;
+  } else {
+    int j = block - first_kind;
+    pieces = a.own_splits;
+    const int rest = j / pieces;
+    piece = j - rest * pieces;
+    j = rest / a.own_tiles;
+    t = rest - j * a.own_tiles;
+    it.b = j / a.heads;
+    it.h = j - it.b * a.heads;
+    it.row0 = it.b * per_request + t * kItemRows;
+    it.rows = min(kItemRows, per_request - t * kItemRows);
+    it.prefix_tiles = 0;
+    it.slot = a.slot_own + ((int64_t)piece * a.heads + it.h) * a.rows + it.row0;
   }
   int tiles = it.prefix_tiles;
   it.len = 0;
-  if (own) {
-    it.row0 = (int64_t)it.b * per_request + t * kTileRows;
-    it.rows = min(kTileRows, per_request - t * kTileRows);
-    it.len = min(max(a.lens[it.b], 0), a.own);
+  if (it.b >= 0) {
+    it.len = min(max(__ldg(a.lens + it.b), 0), a.own);
     // the last of the tile's queries sees the most
-    tiles += (own_visible(a, it.len, (t * kTileRows + it.rows - 1) / a.group) + kTileKeys - 1) / kTileKeys;
+    tiles += (own_visible(a, it.len, (it.row0 - it.b * per_request + it.rows - 1) / a.group) + kTileKeys - 1) / kTileKeys;
   }
   it.first = (int)((int64_t)tiles * piece / pieces);
   it.last = (int)((int64_t)tiles * (piece + 1) / pieces);
@@ -170,16 +179,41 @@ __device__ __forceinline__ uint32_t pack16<__half>(float lo, float hi) {
   return pack_f16x2(lo, hi);
 }
 
-template <typename T, int D>
+template <int D>
 struct AttnSmem {
-  static constexpr int kStages = D == 64 ? 2 : 1;  // two CTAs per SM in 227 KB
-  static constexpr int kTile = kTileKeys * D * 2;  // bytes of a K or V tile, and of Q
-  static constexpr int kQ = 0;
-  static constexpr int kK = kQ + kTile;
-  static constexpr int kV = kK + kStages * kTile;
-  static constexpr int kBars = kV + kStages * kTile;
+  static constexpr int kTile = kTileKeys * D * 2;  // bytes of a K, V or Q tile
+  static constexpr int kRing = D == 64 ? 8 : 5;
+  static constexpr int kQ = 0;  // two tiles
+  static constexpr int kKV = 2 * kTile;
+  static constexpr int kJoin = kKV + kRing * kTile;  // (m, l) of stream 1
+  static constexpr int kBars = kJoin + kTileRows * 8;
   static constexpr int kBytes = kBars + 256 + 1024 /*align*/;
 };
+
+// The ring's order of loads for n tiles, which is the order of their first use.
+//   shared by both streams:  K0 V0 K1 V1 ...
+//   alternate tiles:         K0 K1 V0 K2 V1 K3 ... V(n-2) V(n-1)
+__device__ __forceinline__ int k_index(bool alternate, int tile) {
+  return alternate ? (tile < 2 ? tile : 2 * tile - 1) : 2 * tile;
+}
+__device__ __forceinline__ int v_index(bool alternate, int tile, int n) {
+  return alternate ? (tile == n - 1 ? 2 * n - 1 : 2 * tile + 2) : 2 * tile + 1;
+}
+__device__ __forceinline__ void load_at(bool alternate, int idx, int n, int& tile, bool& value) {
+  if (!alternate) {
+    tile = idx >> 1;
+    value = idx & 1;
+  } else if (idx == 2 * n - 1) {
+    tile = n - 1;
+    value = true;
+  } else if (idx < 2) {
+    tile = idx;
+    value = false;
+  } else {
+    value = !(idx & 1);
+    tile = value ? (idx - 2) >> 1 : (idx + 1) >> 1;
+  }
+}
 
 // 16-bit operands, fp32 accumulator, M = 128.
 template <typename T>
@@ -189,287 +223,381 @@ constexpr uint32_t attn_idesc(int n, bool b_mn_major) {
          ((uint32_t)(kTileRows >> 4) << 24);
 }
 
-// Final result or partial of one row: O (this thread's lane) times inv.
+__device__ __forceinline__ void softmax_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+
+// Where a row's result goes, and its log-sum-exp there.
 template <typename T, int D>
-__device__ __forceinline__ void store_row(const AttnArgs& a, const Item& it, int r, uint32_t o_tmem, bool any,
-                                          float m, float l) {
-  const bool live = r < it.rows;
-  const int64_t row = it.row0 + r;
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  const float lse2 = l == 0.f ? -INFINITY : m + __log2f(l);
+struct RowOut {
   T* out = nullptr;
-  float* po = nullptr;
-  if (it.slot >= 0) {
-    po = a.part_o + (it.slot + r) * D;
-    if (live) a.part_lse[it.slot + r] = lse2;
-  } else {
-    const int per_request = a.lq * a.group;
-    const int64_t b = row / per_request;
-    const int in = (int)(row - b * per_request), i = in / a.group, g = in - i * a.group;
-    const int64_t hq = (int64_t)a.heads * a.group, h = (int64_t)it.h * a.group + g;
-    out = reinterpret_cast<T*>(a.out) + ((b * a.lq + i) * hq + h) * D;
-    if (live) a.lse[(b * hq + h) * a.lq + i] = lse2 * 0.6931471805599453f;
-  }
-#pragma unroll 1
-  for (int c = 0; c < D / 32; ++c) {
-    uint32_t o[32];
-    if (any) {
-      tmem_ld32(o_tmem + (uint32_t)(c * 32), o);
+  float* part = nullptr;
+  __device__ __forceinline__ RowOut(const AttnArgs& a, const Item& it, int r, bool live, float m, float l) {
+    if (!live) return;
+    const float lse2 = l == 0.f ? -INFINITY : m + __log2f(l);
+    if (it.slot >= 0) {
+      part = a.part_o + (it.slot + r) * D;
+      a.part_lse[it.slot + r] = lse2;
     } else {
-#pragma unroll
-      for (int e = 0; e < 32; ++e) o[e] = 0;
-    }
-    if (!live) continue;
-    float f[32];
-#pragma unroll
-    for (int e = 0; e < 32; ++e) f[e] = l == 0.f ? 0.f : __uint_as_float(o[e]) * inv;
-    if (po != nullptr) {
-#pragma unroll
-      for (int e = 0; e < 32; e += 4) st_global(po + c * 32 + e, Elt<float>::pack(f + e));
-    } else {
-#pragma unroll
-      for (int e = 0; e < 32; e += 8) st_global(out + c * 32 + e, Elt<T>::pack(f + e));
+      const int per_request = a.lq * a.group, row = it.row0 + r;
+      const int b = row / per_request, in = row - b * per_request, i = in / a.group, g = in - i * a.group;
+      const int64_t hq = (int64_t)a.heads * a.group, h = (int64_t)it.h * a.group + g;
+      out = reinterpret_cast<T*>(a.out) + (((int64_t)b * a.lq + i) * hq + h) * D;
+      a.lse[(b * hq + h) * a.lq + i] = lse2 * 0.6931471805599453f;
     }
   }
-}
+  __device__ __forceinline__ void store32(int c, const float* f) const {
+    if (part != nullptr) {
+#pragma unroll
+      for (int e = 0; e < 32; e += 4) st_global(part + c + e, Elt<float>::pack(f + e));
+    } else if (out != nullptr) {
+#pragma unroll
+      for (int e = 0; e < 32; e += 8) st_global(out + c + e, Elt<T>::pack(f + e));
+    }
+  }
+};
 
 template <typename T, int D>
-__global__ void __launch_bounds__(kAttnThreads, 2)
+__global__ void __launch_bounds__(kAttnThreads, 1)
     prefix_attn_kernel(const __grid_constant__ CUtensorMap map_kp, const __grid_constant__ CUtensorMap map_vp,
                        const __grid_constant__ CUtensorMap map_ko, const __grid_constant__ CUtensorMap map_vo,
                        const AttnArgs a) {
-  using S = AttnSmem<T, D>;
-  constexpr int kStages = S::kStages;
+  using S = AttnSmem<D>;
+  constexpr int kRing = S::kRing;
   constexpr int kBox = kTileKeys * 128;  // bytes of one 64-element-wide box
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;
   uint8_t* gbase = smem_raw + (base - raw);
   const uint32_t bars = base + S::kBars;
-  const uint32_t q_full = bars, s_full = bars + 8, p_full = bars + 16, o_full = bars + 24;
-  auto k_full = [&](int s) { return bars + 32 + 8u * s; };
-  auto k_empty = [&](int s) { return bars + 32 + 8u * (kStages + s); };
-  auto v_full = [&](int s) { return bars + 32 + 8u * (2 * kStages + s); };
-  auto v_empty = [&](int s) { return bars + 32 + 8u * (3 * kStages + s); };
-  const uint32_t tmem_slot = bars + 32 + 8u * (4 * kStages);
+  auto full = [&](int s) { return bars + 8u * s; };
+  auto empty = [&](int s) { return bars + 8u * (kRing + s); };
+  const uint32_t q_full = bars + 8u * (2 * kRing);
+  auto s_full = [&](int s) { return q_full + 8u + 8u * s; };
+  auto p_full = [&](int s, int half) { return q_full + 24u + 16u * half + 8u * s; };
+  auto o_full = [&](int s) { return q_full + 56u + 8u * s; };
+  const uint32_t done = q_full + 72u, tmem_slot = q_full + 80u;
   const int warp = warp_index(), lane = threadIdx.x & 31;
 
-  pdl_wait();  // lens, q, k and v may be the previous kernel's
-  pdl_trigger();
-  const Item it = item_of(a, blockIdx.x);
-  const int n = it.last - it.first;
-  if (n == 0) {  // nothing to see: an empty part
-    if (threadIdx.x < kSoftmaxThreads) store_row<T, D>(a, it, threadIdx.x, 0, false, 0.f, 0.f);
-    return;
-  }
   if (threadIdx.x == 0) {
+    for (int s = 0; s < kRing; ++s) {
+      mbar_init(full(s), 1);
+      mbar_init(empty(s), 1);
+    }
     mbar_init(q_full, kSoftmaxThreads);
-    mbar_init(s_full, 1);
-    mbar_init(p_full, kSoftmaxThreads);
-    mbar_init(o_full, 1);
-    for (int s = 0; s < kStages; ++s) {
-      mbar_init(k_full(s), 1);
-      mbar_init(k_empty(s), 1);
-      mbar_init(v_full(s), 1);
-      mbar_init(v_empty(s), 1);
+    mbar_init(done, 1);
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(s_full(s), 1);
+      mbar_init(p_full(s, 0), kTileRows);
+      mbar_init(p_full(s, 1), kTileRows);
+      mbar_init(o_full(s), 1);
     }
     mbar_init_fence();
   }
-  if (warp == 5) tmem_alloc(tmem_slot, kTmemColsAttn);
+  if (warp == 9) tmem_alloc(tmem_slot, 512);
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *reinterpret_cast<uint32_t*>(gbase + (tmem_slot - base));
-  const uint32_t tmem_o = tmem + kTileKeys;
+  pdl_wait();  // lens, q, k and v may be the previous kernel's
+  pdl_trigger();
 
-  if (warp == 4) {
+  if (warp == 8) {
     if (lane == 0) {
       // ---------------- TMA producer
-      auto load = [&](uint32_t dst, bool value, int tile, uint32_t bar) {
-        const bool own = tile >= it.prefix_tiles;
-        const CUtensorMap* map = value ? (own ? &map_vo : &map_vp) : (own ? &map_ko : &map_kp);
-        const int row = (own ? tile - it.prefix_tiles : tile) * kTileKeys;
-        mbar_expect_tx(bar, S::kTile);
+      int at = 0;  // loads so far
+      bool ok = true;
+      for (int block = blockIdx.x; block < a.blocks && ok; block += gridDim.x) {
+        const Item it = item_of(a, block);
+        const int n = it.last - it.first;
+        const bool alternate = it.rows <= kTileRows;
+        for (int j = 0; j < 2 * n; ++j, ++at) {
+          const int slot = at % kRing;
+          if (!(ok = mbar_wait(empty(slot), ((at / kRing) & 1) ^ 1u, a.fault))) break;
+          int tile;
+          bool value;
+          load_at(alternate, j, n, tile, value);
+          tile += it.first;
+          const bool own = tile >= it.prefix_tiles;
+          const CUtensorMap* map = value ? (own ? &map_vo : &map_vp) : (own ? &map_ko : &map_kp);
+          const int row = (own ? tile - it.prefix_tiles : tile) * kTileKeys;
+          mbar_expect_tx(full(slot), S::kTile);
 #pragma unroll
-        for (int x = 0; x < D; x += 64) tma_load_4d(dst + (x / 64) * kBox, map, x, it.h, row, own ? it.b : 0, bar);
-      };
-      int s = 0;
-      uint32_t phase = 0;
-      int kn = 0, vn = 0;  // tiles issued
-      for (int t = 0; t < n; ++t) {
-        if (!mbar_wait(k_empty(s), phase ^ 1u, a.fault)) break;
-        load(base + S::kK + s * S::kTile, false, it.first + t, k_full(s));
-        ++kn;
-        if (!mbar_wait(v_empty(s), phase ^ 1u, a.fault)) break;
-        load(base + S::kV + s * S::kTile, true, it.first + t, v_full(s));
-        ++vn;
-        if (++s == kStages) s = 0, phase ^= 1u;
+          for (int x = 0; x < D; x += 64)
+            tma_load_4d(base + S::kKV + slot * S::kTile + (x / 64) * kBox, map, x, it.h, row, own ? it.b : 0, full(slot));
+        }
       }
       // every copy issued has landed before the CTA may exit
-      for (int j = max(0, kn - kStages); j < kn; ++j) mbar_wait(k_full(j % kStages), (j / kStages) & 1, a.fault);
-      for (int j = max(0, vn - kStages); j < vn; ++j) mbar_wait(v_full(j % kStages), (j / kStages) & 1, a.fault);
+      for (int j = max(0, at - kRing); j < at; ++j) mbar_wait(full(j % kRing), (j / kRing) & 1, a.fault);
     }
-  } else if (warp == 5) {
-    // ---------------- MMA issuer: the warp stays converged and elects one thread per tile
+  } else if (warp == 9) {
+    // ---------------- MMA issuer: the warp stays converged and elects one thread per step
     constexpr uint32_t idesc_s = attn_idesc<T>(kTileKeys, false), idesc_o = attn_idesc<T>(D, true);
-    const uint64_t qd = sw128_desc(base + S::kQ), kd0 = sw128_desc(base + S::kK);
-    const uint64_t vd0 = sw128_desc_mn(base + S::kV, kBox);
-    bool ok = __all_sync(0xffffffffu, mbar_wait(q_full, 0, a.fault));
-    int s = 0;
-    uint32_t phase = 0;
-    for (int t = 0; t < n && ok; ++t) {
-      if (!(ok = __all_sync(0xffffffffu, mbar_wait(k_full(s), phase, a.fault)))) break;
-      tc_fence_after();
-      if (elect_one()) {
-        const uint64_t kd = kd0 + s * (S::kTile >> 4);
-#pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-          const int off = ((kk / 4) * kBox + (kk % 4) * 32) >> 4;
-          tc_mma_f16_ss(tmem, qd + off, kd + off, idesc_s, kk != 0);
-        }
-        tc_commit(k_empty(s));
-        tc_commit(s_full);
-      }
-      __syncwarp();
-      if (!(ok = __all_sync(0xffffffffu, mbar_wait(v_full(s), phase, a.fault)))) break;
-      if (!(ok = __all_sync(0xffffffffu, mbar_wait(p_full, t & 1, a.fault)))) break;
-      tc_fence_after();
-      if (elect_one()) {
-        const uint64_t vd = vd0 + s * (S::kTile >> 4);
-#pragma unroll
-        for (int kk = 0; kk < kTileKeys / 16; ++kk)
-          tc_mma_f16_ts(tmem_o, tmem + kk * 8, vd + kk * (2048 >> 4), idesc_o, t != 0 || kk != 0);
-        tc_commit(v_empty(s));
-      }
-      __syncwarp();
-      if (++s == kStages) s = 0, phase ^= 1u;
-    }
-    if (elect_one()) tc_commit(o_full);  // also after a failed wait: everything issued has retired
-    __syncwarp();
-    mbar_wait(o_full, 0, a.fault);
-  } else {
-    // ---------------- softmax: thread r owns query row r (tensor-memory lane r)
-    const int r = threadIdx.x;
-    {
-      // Q, 16 bytes per step, 128-byte swizzle; rows past the last are zero
-      constexpr int kVecs = D / 8;
-      const T* q = reinterpret_cast<const T*>(a.q);
-      const int per_request = a.lq * a.group;
-#pragma unroll 4
-      for (int j = r; j < kTileRows * kVecs; j += kSoftmaxThreads) {
-        const int row = j / kVecs, c = j - row * kVecs;
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (row < it.rows) {
-          const int64_t flat = it.row0 + row, b = flat / per_request;
-          const int in = (int)(flat - b * per_request), i = in / a.group, g = in - i * a.group;
-          v = ld_stream(q + b * a.q_b + i * a.q_t + (int64_t)(it.h * a.group + g) * a.q_h + c * 8);
-        }
-        const uint32_t off = (c / 8) * kBox + row * 128 + (((c & 7) ^ (row & 7)) << 4);
-        *reinterpret_cast<uint4*>(gbase + S::kQ + off) = v;
-      }
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      mbar_arrive(q_full);
-    }
-    const bool warp_live = (warp << 5) < it.rows;
-    const uint32_t lanes = (uint32_t)(warp * 32) << 16;
-    // own rows that this query sees
-    int visible = 0;
-    if (it.b >= 0) visible = own_visible(a, it.len, (int)((it.row0 + min(r, it.rows - 1)) % (a.lq * a.group)) / a.group);
-    float m = -INFINITY, l = 0.f;
+    const uint64_t qd = sw128_desc(base + S::kQ), kd0 = sw128_desc(base + S::kKV);
+    const uint64_t vd0 = sw128_desc_mn(base + S::kKV, kBox);
+    int at = 0, count[2] = {0, 0}, items = 0;
     bool ok = true;
-    for (int t = 0; t < n; ++t) {
-      const int tile = it.first + t;
-      const bool own = tile >= it.prefix_tiles;
-      const int key0 = (own ? tile - it.prefix_tiles : tile) * kTileKeys;
-      const int limit = (int)min((int64_t)kTileKeys, (own ? (int64_t)visible : a.prefix) - key0);
-      if (!(ok = mbar_wait(s_full, t & 1, a.fault))) break;
-      tc_fence_after();
-      if (own && key0 + kTileKeys > it.len && it.len < a.own) {
-        // cache rows past the request's length hold anything: their p is 0, but 0 * inf is not
-        const int st = t % kStages;
-        if (!(ok = mbar_wait(v_full(st), (t / kStages) & 1, a.fault))) break;
-        if (key0 + r >= it.len) {
+    auto wait = [&](uint32_t bar, int phase) {
+      if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar, phase & 1, a.fault));
+      return ok;
+    };
+    for (int block = blockIdx.x; block < a.blocks && ok; block += gridDim.x) {
+      const Item it = item_of(a, block);
+      const int n = it.last - it.first;
+      if (n == 0) continue;
+      const bool alternate = it.rows <= kTileRows;
+      const int steps[2] = {alternate ? (n + 1) / 2 : n, alternate ? n / 2 : n};
+      auto products_s = [&](int s, int t) {  // S of stream s, step t
+        const int idx = at + k_index(alternate, alternate ? 2 * t + s : t), slot = idx % kRing;
+        if (!wait(full(slot), idx / kRing)) return;
+        tc_fence_after();
+        if (elect_one()) {
+          const uint64_t kd = kd0 + slot * (S::kTile >> 4), q = qd + (alternate ? 0 : s * (S::kTile >> 4));
 #pragma unroll
-          for (int x = 0; x < D / 64; ++x)
+          for (int kk = 0; kk < D / 16; ++kk) {
+            const int off = ((kk / 4) * kBox + (kk % 4) * 32) >> 4;
+            tc_mma_f16_ss(tmem + s * kTileKeys, q + off, kd + off, idesc_s, kk != 0);
+          }
+          if (alternate || s == 1) tc_commit(empty(slot));
+          tc_commit(s_full(s));
+        }
+        __syncwarp();
+      };
+      auto products_o = [&](int s, int t) {  // O of stream s, step t
+        const int idx = at + v_index(alternate, alternate ? 2 * t + s : t, n), slot = idx % kRing;
+        if (!wait(full(slot), idx / kRing)) return;
+        const uint64_t vd = vd0 + slot * (S::kTile >> 4);
 #pragma unroll
-            for (int c = 0; c < 8; ++c)
-              *reinterpret_cast<uint4*>(gbase + S::kV + st * S::kTile + x * kBox + r * 128 + c * 16) =
-                  make_uint4(0, 0, 0, 0);
+        for (int half = 0; half < 2; ++half) {
+          if (!wait(p_full(s, half), count[s])) return;
+          tc_fence_after();
+          if (elect_one()) {
+#pragma unroll
+            for (int kk = 4 * half; kk < 4 * half + 4; ++kk)
+              tc_mma_f16_ts(tmem + kColO + s * kTileKeys, tmem + s * kTileKeys + kk * 8, vd + kk * (2048 >> 4), idesc_o,
+                            t != 0 || kk != 0);
+            if (half == 1) {
+              if (alternate || s == 1) tc_commit(empty(slot));
+              if (t == steps[s] - 1) tc_commit(o_full(s));
+            }
+          }
+          __syncwarp();
+        }
+        ++count[s];
+      };
+      if (!wait(q_full, items++)) break;
+      products_s(0, 0);
+      if (steps[1] > 0) products_s(1, 0);
+      for (int t = 0; t < steps[0] && ok; ++t) {
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          if (t >= steps[s]) continue;
+          products_o(s, t);
+          if (t + 1 < steps[s]) products_s(s, t + 1);
+        }
+      }
+      at += 2 * n;
+    }
+    // tensor memory is freed below: everything issued has retired, also after a failed wait
+    if (elect_one()) tc_commit(done);
+    __syncwarp();
+    mbar_wait(done, 0, a.fault);
+  } else {
+    // ---------------- softmax: stream s, thread r owns a row (tensor-memory lane r)
+    const int s = warp >> 2, r = threadIdx.x & 127;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t t_s = tmem + lanes + s * kTileKeys, t_o = tmem + lanes + kColO + s * kTileKeys;
+    const int per_request = a.lq * a.group;
+    bool ok = true;
+    auto wait = [&](uint32_t bar, int phase) {
+      if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar, phase & 1, a.fault));
+      return ok;
+    };
+    int count = 0, at = 0, o_count[2] = {0, 0};
+    for (int block = blockIdx.x; block < a.blocks; block += gridDim.x) {
+      const Item it = item_of(a, block);
+      const int n = it.last - it.first;
+      const bool alternate = it.rows <= kTileRows;
+      const int row = alternate ? r : s * kTileRows + r;  // of the item
+      const bool live = row < it.rows;
+      if (n == 0) {  // nothing to see: an empty part
+        if (!alternate || s == 0) {
+          const RowOut<T, D> dst(a, it, row, live, 0.f, 0.f);
+          const float zero[32] = {};
+          for (int c = 0; c < D; c += 32) dst.store32(c, zero);
+        }
+        continue;
+      }
+      softmax_sync();  // both streams are done with the last item's Q and O
+      {
+        // Q, 16 bytes per step, 128-byte swizzle; rows past the last are zero
+        constexpr int kVecs = D / 8, kStep = kSoftmaxThreads / kVecs;
+        const T* q = reinterpret_cast<const T*>(a.q) + (int64_t)it.h * a.group * a.q_h;
+        const int c = threadIdx.x % kVecs, rows = alternate ? kTileRows : kItemRows;
+#pragma unroll 4
+        for (int j = threadIdx.x / kVecs; j < rows; j += kStep) {
+          uint4 v = make_uint4(0, 0, 0, 0);
+          if (j < it.rows) {
+            const int flat = it.row0 + j, b = flat / per_request;
+            const int in = flat - b * per_request, i = in / a.group, g = in - i * a.group;
+            v = ld_stream(q + b * a.q_b + i * a.q_t + g * a.q_h + c * 8);
+          }
+          const uint32_t off = (j / kTileRows) * S::kTile + (c / 8) * kBox + (j % kTileRows) * 128 + (((c & 7) ^ (j & 7)) << 4);
+          *reinterpret_cast<uint4*>(gbase + S::kQ + off) = v;
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        mbar_arrive(q_full);
       }
-      if (warp_live) {
-        const bool masked = __any_sync(0xffffffffu, limit < kTileKeys);
-        float mx = -INFINITY;
+      // own rows that this query sees
+      int visible = 0;
+      if (it.b >= 0) visible = own_visible(a, it.len, (it.row0 - it.b * per_request + min(row, it.rows - 1)) / a.group);
+      const bool warp_live = (alternate ? 0 : s * kTileRows) + ((warp & 3) << 5) < it.rows;
+      const int steps = alternate ? (n + 1 - s) / 2 : n;
+      float m = -INFINITY, l = 0.f;
+      for (int t = 0; t < steps; ++t, ++count) {
+        const int local = alternate ? 2 * t + s : t, tile = it.first + local;
+        const bool own = tile >= it.prefix_tiles;
+        const int key0 = (own ? tile - it.prefix_tiles : tile) * kTileKeys;
+        const int limit = min(kTileKeys, (own ? visible : a.prefix) - key0);
+        if (!wait(s_full(s), count)) break;
+        tc_fence_after();
+        if (own && key0 + kTileKeys > it.len && it.len < a.own && (alternate || s == 0)) {
+          // cache rows past the request's length hold anything: their p is 0, but 0 * inf is
+          // not (a tile that both streams use: stream 0's product comes first)
+          const int idx = at + v_index(alternate, local, n), slot = idx % kRing;
+          if (!wait(full(slot), idx / kRing)) break;
+          if (key0 + r >= it.len) {
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          uint32_t v[64];
-          tmem_ld64(tmem + lanes + c * 64, v);
+            for (int x = 0; x < D / 64; ++x)
+#pragma unroll
+              for (int c = 0; c < 8; ++c)
+                *reinterpret_cast<uint4*>(gbase + S::kKV + slot * S::kTile + x * kBox + r * 128 + c * 16) =
+                    make_uint4(0, 0, 0, 0);
+          }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        }
+        if (warp_live) {
+          const bool masked = __any_sync(0xffffffffu, limit < kTileKeys);
+          uint32_t v[128];
+          tmem_ld128(t_s, v);
           if (masked) {
 #pragma unroll
-            for (int e = 0; e < 64; ++e) mx = fmaxf(mx, c * 64 + e < limit ? __uint_as_float(v[e]) : -INFINITY);
-          } else {
-#pragma unroll
-            for (int e = 0; e < 64; ++e) mx = fmaxf(mx, __uint_as_float(v[e]));
+            for (int e = 0; e < 128; ++e) v[e] = e < limit ? v[e] : 0xff800000u;
           }
-        }
-        mx *= a.scale_log2;
-        const bool raise = mx > m + kRaise;
-        float fac = 1.f;
-        if (raise) {
-          fac = ex2_approx(m - mx);
-          m = mx;
-        }
-        if (t > 0 && __any_sync(0xffffffffu, raise)) {
-          // O so far: its last product finished before this tile's S did
+          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-          for (int c = 0; c < D / 32; ++c) {
-            uint32_t o[32];
-            tmem_ld32(tmem_o + lanes + c * 32, o);
+          for (int e = 0; e < 128; e += 8)
 #pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * fac);
-            tmem_st32(tmem_o + lanes + c * 32, o);
+            for (int j = 0; j < 4; ++j)
+              mx[j] = fmaxf(fmaxf(mx[j], __uint_as_float(v[e + j])), __uint_as_float(v[e + 4 + j]));
+          const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale_log2;
+          const bool raise = top > m + kRaise;
+          float fac = 1.f;
+          if (raise) {
+            fac = ex2_approx(m - top);
+            m = top;
           }
-        }
-        const float shift = m == -INFINITY ? 0.f : m;
-        float sum = 0.f;
+          if (t > 0 && __any_sync(0xffffffffu, raise)) {
+            // O so far: its last product finished before this tile's S did
+#pragma unroll 1
+            for (int c = 0; c < D; c += 16) {
+              uint32_t o[16];
+              tmem_ld16(t_o + c, o);
+              tmem_ld_wait(o);
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          uint32_t v[64];
-          tmem_ld64(tmem + lanes + c * 64, v);
-          uint32_t p[32];
-#pragma unroll
-          for (int e = 0; e < 64; e += 2) {
-            float s0 = __uint_as_float(v[e]), s1 = __uint_as_float(v[e + 1]);
-            if (masked) {
-              s0 = c * 64 + e < limit ? s0 : -INFINITY;
-              s1 = c * 64 + e + 1 < limit ? s1 : -INFINITY;
+              for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * fac);
+              tmem_st16(t_o + c, o);
             }
-            const float p0 = ex2_approx(fmaf(s0, a.scale_log2, -shift));
-            const float p1 = ex2_approx(fmaf(s1, a.scale_log2, -shift));
-            sum += p0 + p1;
-            p[e / 2] = pack16<T>(p0, p1);
           }
-          tmem_st32(tmem + lanes + c * 32, p);  // over columns of S that have been read
+          const float shift = m == -INFINITY ? 0.f : m;
+          const float2 scale2 = make_float2(a.scale_log2, a.scale_log2), shift2 = make_float2(-shift, -shift);
+          float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            uint32_t p[32];
+#pragma unroll
+            for (int e = 0; e < 64; e += 2) {
+              const float2 x = __ffma2_rn(make_float2(__uint_as_float(v[half * 64 + e]), __uint_as_float(v[half * 64 + e + 1])),
+                                          scale2, shift2);
+              const float2 y = make_float2(ex2_approx(x.x), ex2_approx(x.y));
+              sum[(e >> 1) & 1] = __fadd2_rn(sum[(e >> 1) & 1], y);
+              p[e / 2] = pack16<T>(y.x, y.y);
+            }
+            tmem_st32(t_s + half * 32, p);
+            tmem_st_wait();
+            tc_fence_before();
+            mbar_arrive(p_full(s, half));
+          }
+          l = l * fac + ((sum[0].x + sum[0].y) + (sum[1].x + sum[1].y));
+        } else {
+          tc_fence_before();
+          mbar_arrive(p_full(s, 0));
+          mbar_arrive(p_full(s, 1));
         }
-        l = l * fac + sum;
-        tmem_st_wait();
+      }
+      if (steps > 0) wait(o_full(s), o_count[s]);
+      if (!alternate) {
+        tc_fence_after();
+        const RowOut<T, D> dst(a, it, row, live && ok, m, l);
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        if (warp_live && ok) {
+#pragma unroll 1
+          for (int c = 0; c < D; c += 32) {
+            uint32_t o[32];
+            tmem_ld32(t_o + c, o);
+            float f[32];
+#pragma unroll
+            for (int e = 0; e < 32; ++e) f[e] = l == 0.f ? 0.f : __uint_as_float(o[e]) * inv;
+            dst.store32(c, f);
+          }
+        }
+      } else {
+        // join the streams: stream 0's warps read both O
+        float2* const join = reinterpret_cast<float2*>(gbase + S::kJoin);
+        if (s == 1) join[r] = make_float2(m, l);
+        softmax_sync();
+        if (s == 0) {
+          if (n > 1) wait(o_full(1), o_count[1]);
+          tc_fence_after();
+          const float2 other = n > 1 ? join[r] : make_float2(-INFINITY, 0.f);
+          const float top = fmaxf(m, other.x), shift = top == -INFINITY ? 0.f : top;
+          float f0 = ex2_approx(m - shift), f1 = ex2_approx(other.x - shift);
+          const float sum = f0 * l + f1 * other.y;
+          const RowOut<T, D> dst(a, it, row, live && ok, shift, sum);
+          const float inv = sum == 0.f ? 0.f : 1.f / sum;
+          f0 *= inv;
+          f1 *= inv;
+          if (warp_live && ok) {
+#pragma unroll 1
+            for (int c = 0; c < D; c += 32) {
+              uint32_t o[32];
+              tmem_ld32(t_o + c, o);
+              float f[32];
+#pragma unroll
+              for (int e = 0; e < 32; ++e) f[e] = sum == 0.f ? 0.f : __uint_as_float(o[e]) * f0;
+              if (n > 1) {
+                tmem_ld32(t_o + kTileKeys + c, o);
+#pragma unroll
+                for (int e = 0; e < 32; ++e) f[e] = sum == 0.f ? 0.f : fmaf(__uint_as_float(o[e]), f1, f[e]);
+              }
+              dst.store32(c, f);
+            }
+          }
+        }
       }
       tc_fence_before();
-      mbar_arrive(p_full);
+      at += 2 * n;
+      ++o_count[0];
+      if (!alternate || n > 1) ++o_count[1];
     }
-    if (ok) ok = mbar_wait(o_full, 0, a.fault);
-    tc_fence_after();
-    if (ok) store_row<T, D>(a, it, r, tmem_o + lanes, true, m, l);
-    tc_fence_before();
   }
   __syncthreads();
-  if (warp == 5) {
+  if (warp == 9) {
     tc_fence_after();
-    tmem_free(tmem, kTmemColsAttn);
+    tmem_free(tmem, 512);
   }
 }
 
-// Joins the parts of each row by their log2-sum-exps: one warp per row.
+// Joins the parts of each row by their log2-sum-exps: one warp per row.  With own parts,
+// every row has them and one part (whole items) or `splits` over the prefix; without, only
+// the split items' rows are here.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) prefix_attn_join_kernel(const AttnArgs a, int64_t total) {
   constexpr int E = D / 32;
@@ -479,35 +607,47 @@ __global__ void __launch_bounds__(256) prefix_attn_join_kernel(const AttnArgs a,
   pdl_trigger();
   if (w >= total) return;
   const int per_request = a.lq * a.group;
-  int64_t slot0, step, row;
-  int h, parts;
-  if (a.fused) {
-    const int64_t item = a.whole + w / kTileRows;
-    const int r = (int)(w % kTileRows);
-    h = (int)(item / (a.batch * a.row_tiles));
-    const int rest = (int)(item - (int64_t)h * a.batch * a.row_tiles), b = rest / a.row_tiles, t = rest - b * a.row_tiles;
-    if (t * kTileRows + r >= per_request) return;
-    row = (int64_t)b * per_request + t * kTileRows + r;
+  int h, row, parts;
+  int64_t slot0, step;
+  if (a.own_splits == 0) {
+    const int item = a.whole + (int)(w / kItemRows), r = (int)(w % kItemRows);
+    int grp, t;
+    tile_of(a, item, grp, t);
+    h = a.fused ? grp / a.batch : grp;
+    const int b = a.fused ? grp - h * a.batch : 0;
+    if (t * kItemRows + r >= (a.fused ? (int64_t)per_request : a.rows)) return;
+    row = b * per_request + t * kItemRows + r;
     parts = a.splits;
-    slot0 = (w / kTileRows) * parts * kTileRows + r;
-    step = kTileRows;
+    slot0 = a.slot_tail + (w / kItemRows) * parts * kItemRows + r;
+    step = kItemRows;
   } else {
-    const int64_t rows = (int64_t)a.batch * per_request;
-    h = (int)(w / rows);
-    row = w - h * rows;
-    parts = a.splits + a.own_splits;
-    slot0 = w;
-    step = a.heads * rows;
+    h = (int)(w / a.rows);
+    row = (int)(w - h * a.rows);
+    const int t = row / kItemRows, full = a.row_tiles - 1;
+    const int item = t < full ? h * full + t : a.heads * full + h;
+    if (item < a.whole) {
+      parts = 1;
+      slot0 = h * a.rows + row;
+      step = 0;
+    } else {
+      parts = a.splits;
+      slot0 = a.slot_tail + (int64_t)(item - a.whole) * parts * kItemRows + row - t * kItemRows;
+      step = kItemRows;
+    }
   }
+  const int64_t own0 = a.slot_own + (int64_t)h * a.rows + row, own_step = a.heads * a.rows;
+  const int all = parts + a.own_splits;
+  auto slot_of = [&](int s) { return s < parts ? slot0 + s * step : own0 + (s - parts) * own_step; };
   float top = -INFINITY;
-  for (int s = lane; s < parts; s += 32) top = fmaxf(top, a.part_lse[slot0 + s * step]);
+  for (int s = lane; s < all; s += 32) top = fmaxf(top, a.part_lse[slot_of(s)]);
   top = warp_max(top);
   const float shift = top == -INFINITY ? 0.f : top;
   float o[E] = {}, sum = 0.f;
 #pragma unroll 4
-  for (int s = 0; s < parts; ++s) {
-    const float wgt = ex2_approx(a.part_lse[slot0 + s * step] - shift);
-    const float* p = a.part_o + (slot0 + s * step) * D + lane * E;
+  for (int s = 0; s < all; ++s) {
+    const int64_t slot = slot_of(s);
+    const float wgt = ex2_approx(a.part_lse[slot] - shift);
+    const float* p = a.part_o + slot * D + lane * E;
     sum += wgt;
     if constexpr (E == 4) {
       const float4 v = *reinterpret_cast<const float4*>(p);
@@ -517,11 +657,11 @@ __global__ void __launch_bounds__(256) prefix_attn_join_kernel(const AttnArgs a,
       o[0] = fmaf(wgt, v.x, o[0]), o[1] = fmaf(wgt, v.y, o[1]);
     }
   }
-  const int64_t b = row / per_request, hq = (int64_t)a.heads * a.group;
-  const int in = (int)(row - b * per_request), i = in / a.group, g = in - i * a.group;
+  const int64_t hq = (int64_t)a.heads * a.group;
+  const int b = row / per_request, in = row - b * per_request, i = in / a.group, g = in - i * a.group;
   const int64_t hh = (int64_t)h * a.group + g;
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  uint32_t* out = reinterpret_cast<uint32_t*>(reinterpret_cast<T*>(a.out) + ((b * a.lq + i) * hq + hh) * D + lane * E);
+  uint32_t* out = reinterpret_cast<uint32_t*>(reinterpret_cast<T*>(a.out) + (((int64_t)b * a.lq + i) * hq + hh) * D + lane * E);
 #pragma unroll
   for (int e = 0; e < E; e += 2) out[e / 2] = pack16<T>(o[e] * inv, o[e + 1] * inv);
   if (lane == 0)
@@ -531,67 +671,80 @@ __global__ void __launch_bounds__(256) prefix_attn_join_kernel(const AttnArgs a,
 // ------------------------------------------------------------------ host side
 struct Plan {
   bool fused;
-  int64_t row_tiles, own_tiles, whole, items, splits, own_splits, blocks, slots, joined;
+  int64_t groups, row_tiles, items, whole, splits, own_tiles, own_splits, blocks, rows;
+  int64_t slot_tail, slot_own, slots, joined;
+  double cost;  // key tiles that the longest-working SM walks, and what joining costs
 };
 
-// Which tiles there are, how they are split, and what has to be joined.  `hold`: CTAs
-// that the GPU holds at once (two per SM).
+// What a unit costs beside its tiles (Q, the results, the pipeline's ends) and what its rows'
+// parts cost to join, in key tiles; measured on single tokens (about 1 us each).
+constexpr double kUnitTiles = 2.0, kJoinTiles = 1.0;
+
+// How many parts the items that do not fill the last round over `hold` CTAs are split in, and
+// the time of all of them in tiles.
+int64_t best_split(int64_t tail, int64_t tiles, int64_t hold, double per_tile, double* cost) {
+  int64_t best = 1;
+  const int64_t most = tiles / 2 < 1 ? 1 : tiles / 2 < hold ? tiles / 2 : hold;
+  for (int64_t s = 1; s <= most; ++s) {
+    const double c = (double)cdiv(tail * s, hold) * ((double)cdiv(tiles, s) * per_tile + kUnitTiles) +
+                     (s > 1 ? kJoinTiles + 0.05 * (double)s : 0.);
+    if (s == 1 || c < *cost) {
+      *cost = c;
+      best = s;
+    }
+  }
+  return best;
+}
+
+Plan make_plan(bool fused, int64_t batch, int64_t lq, int64_t heads, int64_t group, int64_t prefix, int64_t own,
+               int64_t hold) {
+  Plan p{};
+  const int64_t per_request = lq * group;
+  const int64_t ptiles = cdiv(prefix, kTileKeys), otiles = cdiv(own, kTileKeys);
+  p.fused = fused;
+  p.rows = batch * per_request;
+  const int64_t tile_rows = fused ? per_request : p.rows;
+  p.groups = fused ? heads * batch : heads;
+  p.row_tiles = cdiv(tile_rows, kItemRows);
+  p.items = fused || prefix > 0 ? p.groups * p.row_tiles : 0;
+  p.splits = 1;
+  const int64_t tiles = fused ? ptiles + otiles : ptiles;
+  // up to 128 rows: two tiles per step
+  const double per_tile = tile_rows <= kTileRows ? 0.5 : 1.0;
+  p.whole = p.items / hold * hold;
+  p.cost = (double)(p.whole / hold) * ((double)tiles * per_tile + kUnitTiles);
+  if (p.items > p.whole) {
+    double c;
+    p.splits = best_split(p.items - p.whole, tiles, hold, per_tile, &c);
+    p.cost += c;
+  }
+  if (p.splits == 1) p.whole = p.items;
+  p.blocks = p.whole + (p.items - p.whole) * p.splits;
+  if (!fused && own > 0) {
+    p.own_tiles = cdiv(per_request, kItemRows);
+    const int64_t units = heads * batch * p.own_tiles;
+    const double per = per_request <= kTileRows ? 0.5 : 1.0;
+    double c;
+    p.own_splits = units < hold ? best_split(units, otiles, hold, per, &c) : 1;
+    if (units >= hold) c = (double)units / (double)hold * ((double)otiles * per + kUnitTiles);
+    p.cost += c + kJoinTiles;
+    p.blocks += units * p.own_splits;
+  }
+  const bool keep = p.own_splits > 0;
+  p.slot_tail = keep && p.whole > 0 ? heads * p.rows : 0;
+  p.slot_own = p.slot_tail + (p.items - p.whole) * p.splits * kItemRows;
+  p.slots = p.slot_own + p.own_splits * heads * p.rows;
+  p.joined = keep ? heads * p.rows : (p.items - p.whole) * kItemRows;
+  return p;
+}
+
+// `hold`: CTAs that the GPU holds at once (one per SM).
 Plan plan_attention(int64_t batch, int64_t lq, int64_t heads, int64_t group, int64_t prefix, int64_t own,
                     int64_t hold) {
-  Plan p{};
-  const int64_t per_request = lq * group, rows = batch * per_request;
-  const int64_t ptiles = cdiv(prefix, kTileKeys), otiles = cdiv(own, kTileKeys);
-  const int64_t packed = cdiv(rows, kTileRows), split_rows = cdiv(per_request, kTileRows);
-  // Tiles of work: packed, and with row tiles that stay within a request.  The packed plan
-  // also writes and reads every row's parts, which costs about as much as two tiles.
-  const int64_t cost_packed = packed * (ptiles + 2) + batch * split_rows * (otiles + 2);
-  const int64_t cost_fused = batch * split_rows * (ptiles + otiles);
-  p.fused = cost_fused <= cost_packed;
-  if (prefix == 0) p.fused = true;  // one kind of key: no parts unless split
-  if (prefix > 0 && own == 0) p.fused = batch == 1;
-  if (p.fused) {
-    p.row_tiles = split_rows;
-    p.items = heads * batch * split_rows;
-    p.whole = p.items / hold * hold;
-    const int64_t tail = p.items - p.whole;
-    p.splits = 1;
-    if (tail) {
-      p.splits = hold / tail;
-      const int64_t most = cdiv(ptiles + otiles, 2);  // two tiles per part at least
-      if (p.splits > most) p.splits = most > 0 ? most : 1;
-    }
-    if (p.splits <= 1) {
-      p.splits = 1;
-      p.whole = p.items;
-    }
-    p.blocks = p.whole + (p.items - p.whole) * p.splits;
-    p.slots = p.splits > 1 ? (p.items - p.whole) * p.splits * kTileRows : 0;
-    p.joined = p.splits > 1 ? (p.items - p.whole) * kTileRows : 0;
-  } else {
-    p.row_tiles = packed;
-    p.own_tiles = split_rows;
-    p.items = prefix > 0 ? heads * packed : 0;
-    p.splits = 0;
-    if (p.items) {
-      const int64_t most = cdiv(ptiles, 2);
-      p.splits = hold / p.items;
-      if (p.splits > most) p.splits = most;
-      if (p.splits < 1) p.splits = 1;
-    }
-    const int64_t own_items = own > 0 ? heads * batch * split_rows : 0;
-    p.own_splits = 0;
-    if (own_items) {
-      const int64_t most = cdiv(otiles, 4);
-      p.own_splits = hold / own_items;
-      if (p.own_splits > most) p.own_splits = most;
-      if (p.own_splits < 1) p.own_splits = 1;
-    }
-    p.blocks = p.items * p.splits + own_items * p.own_splits;
-    const bool parts = p.splits + p.own_splits > 1;
-    p.slots = parts ? (p.splits + p.own_splits) * heads * rows : 0;
-    p.joined = parts ? heads * rows : 0;
-  }
-  return p;
+  const Plan fused = make_plan(true, batch, lq, heads, group, prefix, own, hold);
+  if (prefix == 0 || batch == 1) return fused;
+  const Plan packed = make_plan(false, batch, lq, heads, group, prefix, own, hold);
+  return packed.cost < fused.cost ? packed : fused;
 }
 
 int check_sizes(const char* op, int64_t batch, int64_t lq, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
@@ -601,7 +754,8 @@ int check_sizes(const char* op, int64_t batch, int64_t lq, int64_t q_heads, int6
   if (head_dim != 64 && head_dim != 128) return fail(JO_ERR_SHAPE, "%s: head_dim must be 64 or 128", op);
   const int64_t most = INT32_MAX / 2;
   if (batch > most || lq > most || prefix > most || own > most || q_heads > most || lq * (q_heads / kv_heads) > most ||
-      batch * q_heads > most || batch * lq > most || batch * lq * q_heads > (int64_t)1 << 38)
+      batch * q_heads > most || batch * lq > most || batch * lq * (q_heads / kv_heads) > most ||
+      batch * lq * q_heads > (int64_t)1 << 38)
     return fail(JO_ERR_SHAPE, "%s: size too large", op);
   return JO_OK;
 }
@@ -628,10 +782,10 @@ template <typename T, int D>
 int launch_attention(const CUtensorMap* maps, const AttnArgs& a, const Plan& p, cudaStream_t st, const DeviceInfo* di) {
   const char* op = "shared_prefix_attention";
   auto kern = prefix_attn_kernel<T, D>;
-  constexpr int smem = AttnSmem<T, D>::kBytes;
+  constexpr int smem = AttnSmem<D>::kBytes;
   static std::atomic<uint64_t> reserved{0};
   if (int s = reserve_smem((const void*)kern, smem, reserved, di, op)) return s;
-  if (cudaError_t e = launch_pdl(kern, dim3((unsigned)p.blocks), dim3(kAttnThreads), smem, st, maps[0], maps[1],
+  if (cudaError_t e = launch_pdl(kern, dim3((unsigned)(p.blocks < di->sm_count ? p.blocks : di->sm_count)), dim3(kAttnThreads), smem, st, maps[0], maps[1],
                                  maps[2], maps[3], a))
     return launch_failed(e, op);
   if (int s = after_launch("prefix_attn_kernel")) return s;
@@ -657,7 +811,7 @@ int64_t jo_shared_prefix_attention_workspace(int64_t batch, int64_t q_len, int64
   if (device_info(&di)) return -1;
   if (check_sizes("shared_prefix_attention", batch, q_len, q_heads, kv_heads, head_dim, prefix_len, own_len)) return -1;
   if (batch == 0 || q_len == 0) return 0;
-  const Plan p = plan_attention(batch, q_len, kv_heads, q_heads / kv_heads, prefix_len, own_len, 2 * di->sm_count);
+  const Plan p = plan_attention(batch, q_len, kv_heads, q_heads / kv_heads, prefix_len, own_len, di->sm_count);
   return p.slots * (head_dim + 1) * 4;
 }
 
@@ -693,7 +847,7 @@ int jo_shared_prefix_attention(void* out, float* lse, const void* q, int64_t q_s
   for (const auto& u : used)
     if (u.size > 1 && (u.stride % 8 || u.stride < 0))
       return fail(JO_ERR_ALIGN, "%s: strides must be multiples of 16 bytes and not negative", op);
-  const Plan p = plan_attention(batch, q_len, kv_heads, q_heads / kv_heads, prefix_len, own_len, 2 * di->sm_count);
+  const Plan p = plan_attention(batch, q_len, kv_heads, q_heads / kv_heads, prefix_len, own_len, di->sm_count);
   if (p.blocks > INT32_MAX || cdiv(p.joined, 8) > INT32_MAX) return fail(JO_ERR_SHAPE, "%s: size too large", op);
   if (p.slots && (!workspace || !aligned16(workspace) || workspace_bytes < p.slots * (head_dim + 1) * 4))
     return fail(JO_ERR_INVALID, "%s: a 16-byte aligned workspace of %lld bytes is needed", op,
@@ -706,7 +860,7 @@ int jo_shared_prefix_attention(void* out, float* lse, const void* q, int64_t q_s
   a.q_t = q_stride_t;
   a.q_h = q_stride_h;
   a.lens = lens;
-  a.prefix = prefix_len;
+  a.prefix = (int)prefix_len;
   a.batch = (int)batch;
   a.lq = (int)q_len;
   a.heads = (int)kv_heads;
@@ -715,12 +869,17 @@ int jo_shared_prefix_attention(void* out, float* lse, const void* q, int64_t q_s
   a.causal = causal;
   a.scale_log2 = scale * kLog2E;
   a.fused = p.fused;
+  a.groups = (int)p.groups;
   a.row_tiles = (int)p.row_tiles;
-  a.own_tiles = (int)p.own_tiles;
-  a.whole = (int)p.whole;
   a.items = (int)p.items;
+  a.whole = (int)p.whole;
   a.splits = (int)p.splits;
+  a.own_tiles = (int)p.own_tiles;
   a.own_splits = (int)p.own_splits;
+  a.blocks = (int)p.blocks;
+  a.rows = p.rows;
+  a.slot_tail = p.slot_tail;
+  a.slot_own = p.slot_own;
   a.part_o = (float*)workspace;
   a.part_lse = (float*)workspace + p.slots * head_dim;
   a.fault = di->fault;
