@@ -116,6 +116,13 @@ __device__ __forceinline__ void st_global(void* p, const uint4& v) {
   *reinterpret_cast<uint4*>(p) = v;
 }
 
+// 32 bytes in one store (the address a multiple of 32).
+__device__ __forceinline__ void st_global32(void* p, const uint4& lo, const uint4& hi) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(lo.x), "r"(lo.y), "r"(lo.z),
+               "r"(lo.w), "r"(hi.x), "r"(hi.y), "r"(hi.z), "r"(hi.w)
+               : "memory");
+}
+
 // Element traits: 16-byte vectors of T, conversion to/from fp32.
 template <typename T>
 struct Elt;

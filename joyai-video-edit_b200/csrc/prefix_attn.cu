@@ -18,38 +18,40 @@
 // quotient O / l does not depend on m.  Parts over disjoint keys are joined by their
 // log2-sum-exps.
 //
-// Rows.  All queries that read one k/v head can share its keys whatever request they
-// belong to, so over the prefix a row of a tensor-core tile is any (request, query, q head
-// of the k/v head's group): the prefix is read once for up to 256 such rows, not once per
-// request.  Two plans (plan_attention):
-//   packed  row tiles run across requests; the prefix and each request's own rows are
-//           separate work items, joined afterwards;
-//   fused   row tiles stay within a request and walk the prefix, then its own rows.
-// Where the items do not fill the GPU evenly, the last ones' keys are split and joined.
+// Rows and keys.  All queries that read one k/v head can share its keys whatever request
+// they belong to: a row of a tensor-core tile is any (request, query, q head of the k/v
+// head's group), up to 256 of them to a work unit, and the unit's keys are a walk over tiles
+// of 128: first the prefix's, read once for all of the unit's rows, then the own rows of
+// each request that has a row in the unit, which only that request's rows see (for the
+// others their p is 0).  For single tokens the tensor cores have time for that: a tile costs
+// its bytes.  Row tiles run across requests or stay within one, whichever costs fewer tiles
+// (plan_attention).  Where the units do not fill the GPU evenly, the last ones' walks are
+// split and joined.
 //
-// One CTA per SM walks over the items with two streams, each with its own S, P and O in
+// One CTA per SM goes through its units with two streams, each with its own S, P and O in
 // tensor memory, so that one stream's softmax runs while the other's products do:
-//   an item of more than 128 rows: the streams take its two halves, and share every K and
+//   a unit of more than 128 rows: the streams take its two halves, and share every K and
 //   V tile (64 KB per tile of 128 keys would otherwise exceed what an SM can take in);
-//   an item of up to 128 rows (single tokens): the streams take alternate key tiles of the
+//   a unit of up to 128 rows (single tokens): the streams take alternate key tiles of the
 //   same rows and are joined at the end.
 // Warps 0-3 and 4-7: softmax of stream 0 and 1, one row per thread (tensor-memory lane):
 //   S from tensor memory, the running maximum and sum, P back in place of S in two halves
 //   (the product may start on the first), O rescaled in place; Q and the results.
 // Warp 8: TMA producer of K and V tiles of 128 rows (128-byte swizzle) into one ring, in
-//   the order of their first use; it runs ahead across items.
+//   the order of their first use; it runs ahead across units.
 // Warp 9: tcgen05.mma issuer: S = Q K^T (both operands in shared memory), O += P V with P
 //   from tensor memory and V as it lies ([keys, D], the MN-major operand).
 //
 // P is rounded to q's 16-bit type for the tensor cores (its error averages out over the
 // keys: 2^-9 relative for bf16, like the output's own rounding); l sums the unrounded p.
+#include "quant.cuh"
 #include "tcgen05.cuh"
 
 namespace jo {
 namespace {
 
 constexpr int kTileRows = 128;           // rows per stream (UMMA M)
-constexpr int kItemRows = 2 * kTileRows;  // rows per item at most
+constexpr int kUnitRows = 2 * kTileRows;  // rows per unit at most
 constexpr int kTileKeys = 128;           // keys per tile (UMMA N of S, K of P V)
 constexpr int kSoftmaxThreads = 256;
 constexpr int kAttnThreads = 320;
@@ -66,35 +68,37 @@ struct AttnArgs {
   int batch, lq, heads, group, own;  // heads: of k and v; group: q heads per k/v head; own: rows of the own caches
   int causal;
   float scale_log2;
-  // plan: items 0..items-1 are the row tiles of `groups` groups (packed: k/v heads, fused:
-  // (head, request) pairs), every group's last tile after all others; those from `whole` on
-  // are split in `splits`; then, packed, the own rows of each (request, head)
-  int fused;
-  int groups, row_tiles;
+  // plan: items 0..items-1 are the row tiles (of `tile_rows` rows) of `groups` groups (k/v
+  // heads, or within_request: (head, request) pairs), every group's last tile after all
+  // others; the walks of those from `whole` on are split in `splits`
+  int within_request;
+  int tile_rows, groups, row_tiles;
   int items, whole, splits;
-  int own_tiles, own_splits;
-  int blocks;           // work units in all
-  int64_t rows;         // queries per k/v head
-  int64_t slot_tail;    // first slot of the split items' parts
-  int64_t slot_own;     // and of the own rows'; whole items' parts (packed): from 0
+  int units;   // whole + (items - whole) * splits
+  int rows;    // queries per k/v head
   float* part_o;        // [slots, D]
   float* part_lse;
   unsigned int* fault;
 };
 
-// One work unit: rows [row0, row0 + rows) of k/v head h (row: (b * Lq + i) * G + g) and tiles
-// [first, last) of the prefix's, then the request's own, keys.
-struct Item {
-  int h, b;  // b: the request of the own rows (-1: none)
-  int row0, rows;
-  int prefix_tiles;  // tiles of the walk that belong to the prefix
+// One work unit: rows [row0, row0 + rows) of k/v head h (row: (b * Lq + i) * G + g), which
+// belong to requests b0..b1, and tiles [first, last) of its walk.
+struct Unit {
+  int h, row0, rows, b0, b1;
   int first, last;
-  int len;       // own rows of b
   int64_t slot;  // partial slot of row0 (-1: final output)
 };
 
 __device__ __forceinline__ int own_visible(const AttnArgs& a, int len, int i) {
   return a.causal ? min(len, max(0, len - a.lq + i + 1)) : len;
+}
+__device__ __forceinline__ int own_len(const AttnArgs& a, int b) { return min(max(__ldg(a.lens + b), 0), a.own); }
+__device__ __forceinline__ int prefix_tiles(const AttnArgs& a) { return (a.prefix + kTileKeys - 1) / kTileKeys; }
+// Tiles of request b's own rows that the unit's rows see: its last row there sees the most.
+__device__ __forceinline__ int own_tiles(const AttnArgs& a, const Unit& u, int b) {
+  const int per_request = a.lq * a.group;
+  const int last = min(u.row0 + u.rows, (b + 1) * per_request) - 1 - b * per_request;
+  return (own_visible(a, own_len(a, b), last / a.group) + kTileKeys - 1) / kTileKeys;
 }
 
 // Group and row tile of an item.
@@ -109,64 +113,80 @@ __device__ __forceinline__ void tile_of(const AttnArgs& a, int item, int& grp, i
   }
 }
 
-__device__ Item item_of(const AttnArgs& a, int block) {
-  Item it;
-  const int per_request = a.lq * a.group;
-  const int ptiles = (a.prefix + kTileKeys - 1) / kTileKeys;
-  int piece = 0, pieces = 1, t;
-  it.slot = -1;
-  const int first_kind = a.whole + (a.items - a.whole) * a.splits;
-  if (block < first_kind) {
-    int item = block;
-    if (block >= a.whole) {
-      const int tail = a.items - a.whole, j = block - a.whole;
-      piece = j / tail;
-      item = a.whole + j - piece * tail;
-      pieces = a.splits;
-    }
-    int grp;
-    tile_of(a, item, grp, t);
-    if (a.fused) {
-      it.h = grp / a.batch;
-      it.b = grp - it.h * a.batch;
-      it.row0 = it.b * per_request + t * kItemRows;
-      it.rows = min(kItemRows, per_request - t * kItemRows);
-    } else {
-      it.h = grp;
-      it.b = -1;
-      it.row0 = t * kItemRows;
-      it.rows = (int)min((int64_t)kItemRows, a.rows - it.row0);
-    }
-    it.prefix_tiles = ptiles;
-    if (item >= a.whole && (pieces > 1 || a.own_splits > 0))
-      it.slot = a.slot_tail + ((int64_t)(item - a.whole) * pieces + piece) * kItemRows;
-    else if (a.own_splits > 0)
-      it.slot = (int64_t)it.h * a.rows + it.row0;
+// Work unit `index`; by a converged warp.
+__device__ Unit unit_of(const AttnArgs& a, int index) {
+  Unit u;
+  const int per_request = a.lq * a.group, lane = threadIdx.x & 31;
+  int piece = 0, pieces = 1, item = index, grp, t;
+  if (index >= a.whole) {
+    const int tail = a.items - a.whole, j = index - a.whole;
+    piece = j / tail;
+    item = a.whole + j - piece * tail;
+    pieces = a.splits;
+  }
+  tile_of(a, item, grp, t);
+  if (a.within_request) {
+    u.h = grp / a.batch;
+    u.b0 = u.b1 = grp - u.h * a.batch;
+    u.row0 = u.b0 * per_request + t * a.tile_rows;
+    u.rows = min(a.tile_rows, per_request - t * a.tile_rows);
   } else {
-    int j = block - first_kind;
-    pieces = a.own_splits;
-    const int rest = j / pieces;
-    piece = j - rest * pieces;
-    j = rest / a.own_tiles;
-    t = rest - j * a.own_tiles;
-    it.b = j / a.heads;
-    it.h = j - it.b * a.heads;
-    it.row0 = it.b * per_request + t * kItemRows;
-    it.rows = min(kItemRows, per_request - t * kItemRows);
-    it.prefix_tiles = 0;
-    it.slot = a.slot_own + ((int64_t)piece * a.heads + it.h) * a.rows + it.row0;
+    u.h = grp;
+    u.row0 = t * a.tile_rows;
+    u.rows = min(a.tile_rows, a.rows - u.row0);
+    u.b0 = u.row0 / per_request;
+    u.b1 = (u.row0 + u.rows - 1) / per_request;
   }
-  int tiles = it.prefix_tiles;
-  it.len = 0;
-  if (it.b >= 0) {
-    it.len = min(max(__ldg(a.lens + it.b), 0), a.own);
-    // the last of the tile's queries sees the most
-    tiles += (own_visible(a, it.len, (it.row0 - it.b * per_request + it.rows - 1) / a.group) + kTileKeys - 1) / kTileKeys;
-  }
-  it.first = (int)((int64_t)tiles * piece / pieces);
-  it.last = (int)((int64_t)tiles * (piece + 1) / pieces);
-  return it;
+  u.slot = pieces > 1 ? ((int64_t)(item - a.whole) * pieces + piece) * a.tile_rows : -1;
+  int own = 0;
+  if (a.own > 0)
+    for (int b = u.b0 + lane; b <= u.b1; b += 32) own += own_tiles(a, u, b);
+  const uint32_t tiles = prefix_tiles(a) + __reduce_add_sync(0xffffffffu, own);
+  u.first = (int)(tiles * (uint32_t)piece / (uint32_t)pieces);
+  u.last = (int)(tiles * (uint32_t)(piece + 1) / (uint32_t)pieces);
+  return u;
 }
+
+// A place in a unit's walk: tile t of the prefix (b < 0) or of request b's own rows.
+struct Walk {
+  int b, t, count;  // count: tiles of this part of the walk
+  // place `at`; by a converged warp
+  __device__ __forceinline__ Walk(const AttnArgs& a, const Unit& u, int at) {
+    b = -1;
+    t = at;
+    count = prefix_tiles(a);
+    if (at < count) return;
+    at -= count;
+    const int lane = threadIdx.x & 31;
+    for (int first = u.b0; first <= u.b1; first += 32) {
+      const int mine = first + lane <= u.b1 ? own_tiles(a, u, first + lane) : 0;
+      int upto = mine;  // inclusive sum over the lanes
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += v;
+      }
+      const uint32_t past = __ballot_sync(0xffffffffu, upto > at);
+      if (past) {
+        const int l = __ffs(past) - 1;
+        b = first + l;
+        count = __shfl_sync(0xffffffffu, mine, l);
+        t = at - (__shfl_sync(0xffffffffu, upto, l) - count);
+        return;
+      }
+      at -= __shfl_sync(0xffffffffu, upto, 31);
+    }
+    b = u.b1 + 1;  // the end
+    t = count = 0;
+  }
+  __device__ __forceinline__ void next(const AttnArgs& a, const Unit& u) {
+    if (++t < count) return;
+    t = 0;
+    b = b < 0 ? u.b0 : b + 1;
+    for (; b <= u.b1; ++b)
+      if ((count = a.own > 0 ? own_tiles(a, u, b) : 0) > 0) return;
+  }
+};
 
 template <typename T>
 __device__ __forceinline__ uint32_t pack16(float lo, float hi);
@@ -187,7 +207,8 @@ struct AttnSmem {
   static constexpr int kKV = 2 * kTile;
   static constexpr int kJoin = kKV + kRing * kTile;  // (m, l) of stream 1
   static constexpr int kBars = kJoin + kTileRows * 8;
-  static constexpr int kBytes = kBars + 256 + 1024 /*align*/;
+  static constexpr int kGuard = kBars + 256;  // first non-finite value row of a tile, per warp
+  static constexpr int kBytes = kGuard + 64 + 1024 /*align*/;
 };
 
 // The ring's order of loads for n tiles, which is the order of their first use.
@@ -199,20 +220,10 @@ __device__ __forceinline__ int k_index(bool alternate, int tile) {
 __device__ __forceinline__ int v_index(bool alternate, int tile, int n) {
   return alternate ? (tile == n - 1 ? 2 * n - 1 : 2 * tile + 2) : 2 * tile + 1;
 }
-__device__ __forceinline__ void load_at(bool alternate, int idx, int n, int& tile, bool& value) {
-  if (!alternate) {
-    tile = idx >> 1;
-    value = idx & 1;
-  } else if (idx == 2 * n - 1) {
-    tile = n - 1;
-    value = true;
-  } else if (idx < 2) {
-    tile = idx;
-    value = false;
-  } else {
-    value = !(idx & 1);
-    tile = value ? (idx - 2) >> 1 : (idx + 1) >> 1;
-  }
+// Whether load `idx` is a V tile.
+__device__ __forceinline__ bool value_at(bool alternate, int idx, int n) {
+  if (!alternate) return idx & 1;
+  return idx == 2 * n - 1 || (idx >= 2 && !(idx & 1));
 }
 
 // 16-bit operands, fp32 accumulator, M = 128.
@@ -230,16 +241,16 @@ template <typename T, int D>
 struct RowOut {
   T* out = nullptr;
   float* part = nullptr;
-  __device__ __forceinline__ RowOut(const AttnArgs& a, const Item& it, int r, bool live, float m, float l) {
+  __device__ __forceinline__ RowOut(const AttnArgs& a, const Unit& u, int r, bool live, float m, float l) {
     if (!live) return;
     const float lse2 = l == 0.f ? -INFINITY : m + __log2f(l);
-    if (it.slot >= 0) {
-      part = a.part_o + (it.slot + r) * D;
-      a.part_lse[it.slot + r] = lse2;
+    if (u.slot >= 0) {
+      part = a.part_o + (u.slot + r) * D;
+      a.part_lse[u.slot + r] = lse2;
     } else {
-      const int per_request = a.lq * a.group, row = it.row0 + r;
+      const int per_request = a.lq * a.group, row = u.row0 + r;
       const int b = row / per_request, in = row - b * per_request, i = in / a.group, g = in - i * a.group;
-      const int64_t hq = (int64_t)a.heads * a.group, h = (int64_t)it.h * a.group + g;
+      const int64_t hq = (int64_t)a.heads * a.group, h = (int64_t)u.h * a.group + g;
       out = reinterpret_cast<T*>(a.out) + (((int64_t)b * a.lq + i) * hq + h) * D;
       a.lse[(b * hq + h) * a.lq + i] = lse2 * 0.6931471805599453f;
     }
@@ -247,10 +258,10 @@ struct RowOut {
   __device__ __forceinline__ void store32(int c, const float* f) const {
     if (part != nullptr) {
 #pragma unroll
-      for (int e = 0; e < 32; e += 4) st_global(part + c + e, Elt<float>::pack(f + e));
+      for (int e = 0; e < 32; e += 8) st_global32(part + c + e, Elt<float>::pack(f + e), Elt<float>::pack(f + e + 4));
     } else if (out != nullptr) {
 #pragma unroll
-      for (int e = 0; e < 32; e += 8) st_global(out + c + e, Elt<T>::pack(f + e));
+      for (int e = 0; e < 32; e += 16) st_global32(out + c + e, Elt<T>::pack(f + e), Elt<T>::pack(f + e + 8));
     }
   }
 };
@@ -300,49 +311,50 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
   pdl_trigger();
 
   if (warp == 8) {
-    if (lane == 0) {
-      // ---------------- TMA producer
-      int at = 0;  // loads so far
-      bool ok = true;
-      for (int block = blockIdx.x; block < a.blocks && ok; block += gridDim.x) {
-        const Item it = item_of(a, block);
-        const int n = it.last - it.first;
-        const bool alternate = it.rows <= kTileRows;
-        for (int j = 0; j < 2 * n; ++j, ++at) {
-          const int slot = at % kRing;
-          if (!(ok = mbar_wait(empty(slot), ((at / kRing) & 1) ^ 1u, a.fault))) break;
-          int tile;
-          bool value;
-          load_at(alternate, j, n, tile, value);
-          tile += it.first;
-          const bool own = tile >= it.prefix_tiles;
-          const CUtensorMap* map = value ? (own ? &map_vo : &map_vp) : (own ? &map_ko : &map_kp);
-          const int row = (own ? tile - it.prefix_tiles : tile) * kTileKeys;
-          mbar_expect_tx(full(slot), S::kTile);
+    // ---------------- TMA producer (lane 0; the warp finds the units together)
+    int at = 0;  // loads so far
+    bool ok = true;
+    for (int unit = blockIdx.x; unit < a.units; unit += gridDim.x) {
+      const Unit u = unit_of(a, unit);
+      const int n = u.last - u.first;
+      if (n == 0) continue;
+      const bool alternate = u.rows <= kTileRows;
+      Walk walk[2] = {Walk(a, u, u.first), Walk(a, u, u.first)};  // of K, of V
+      for (int j = 0; j < 2 * n && lane == 0 && ok; ++j, ++at) {
+        const int slot = at % kRing;
+        if (!(ok = mbar_wait(empty(slot), ((at / kRing) & 1) ^ 1u, a.fault))) break;
+        const bool value = value_at(alternate, j, n);
+        Walk& w = walk[value];
+        const bool own = w.b >= 0;
+        const CUtensorMap* map = value ? (own ? &map_vo : &map_vp) : (own ? &map_ko : &map_kp);
+        mbar_expect_tx(full(slot), S::kTile);
 #pragma unroll
-          for (int x = 0; x < D; x += 64)
-            tma_load_4d(base + S::kKV + slot * S::kTile + (x / 64) * kBox, map, x, it.h, row, own ? it.b : 0, full(slot));
-        }
+        for (int x = 0; x < D; x += 64)
+          tma_load_4d(base + S::kKV + slot * S::kTile + (x / 64) * kBox, map, x, u.h, w.t * kTileKeys, own ? w.b : 0,
+                      full(slot));
+        w.next(a, u);
       }
-      // every copy issued has landed before the CTA may exit
-      for (int j = max(0, at - kRing); j < at; ++j) mbar_wait(full(j % kRing), (j / kRing) & 1, a.fault);
+      __syncwarp();
     }
+    // every copy issued has landed before the CTA may exit
+    if (lane == 0)
+      for (int j = max(0, at - kRing); j < at; ++j) mbar_wait(full(j % kRing), (j / kRing) & 1, a.fault);
   } else if (warp == 9) {
     // ---------------- MMA issuer: the warp stays converged and elects one thread per step
     constexpr uint32_t idesc_s = attn_idesc<T>(kTileKeys, false), idesc_o = attn_idesc<T>(D, true);
     const uint64_t qd = sw128_desc(base + S::kQ), kd0 = sw128_desc(base + S::kKV);
     const uint64_t vd0 = sw128_desc_mn(base + S::kKV, kBox);
-    int at = 0, count[2] = {0, 0}, items = 0;
+    int at = 0, count[2] = {0, 0}, q_count = 0;
     bool ok = true;
     auto wait = [&](uint32_t bar, int phase) {
       if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar, phase & 1, a.fault));
       return ok;
     };
-    for (int block = blockIdx.x; block < a.blocks && ok; block += gridDim.x) {
-      const Item it = item_of(a, block);
-      const int n = it.last - it.first;
+    for (int unit = blockIdx.x; unit < a.units && ok; unit += gridDim.x) {
+      const Unit u = unit_of(a, unit);
+      const int n = u.last - u.first;
       if (n == 0) continue;
-      const bool alternate = it.rows <= kTileRows;
+      const bool alternate = u.rows <= kTileRows;
       const int steps[2] = {alternate ? (n + 1) / 2 : n, alternate ? n / 2 : n};
       auto products_s = [&](int s, int t) {  // S of stream s, step t
         const int idx = at + k_index(alternate, alternate ? 2 * t + s : t), slot = idx % kRing;
@@ -382,7 +394,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         }
         ++count[s];
       };
-      if (!wait(q_full, items++)) break;
+      if (!wait(q_full, q_count++)) break;
       products_s(0, 0);
       if (steps[1] > 0) products_s(1, 0);
       for (int t = 0; t < steps[0] && ok; ++t) {
@@ -410,32 +422,32 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar, phase & 1, a.fault));
       return ok;
     };
-    int count = 0, at = 0, o_count[2] = {0, 0};
-    for (int block = blockIdx.x; block < a.blocks; block += gridDim.x) {
-      const Item it = item_of(a, block);
-      const int n = it.last - it.first;
-      const bool alternate = it.rows <= kTileRows;
-      const int row = alternate ? r : s * kTileRows + r;  // of the item
-      const bool live = row < it.rows;
+    int count = 0, at = 0, guards = 0, o_count[2] = {0, 0};
+    for (int unit = blockIdx.x; unit < a.units; unit += gridDim.x) {
+      const Unit u = unit_of(a, unit);
+      const int n = u.last - u.first;
+      const bool alternate = u.rows <= kTileRows;
+      const int row = alternate ? r : s * kTileRows + r;  // of the unit
+      const bool live = row < u.rows;
       if (n == 0) {  // nothing to see: an empty part
         if (!alternate || s == 0) {
-          const RowOut<T, D> dst(a, it, row, live, 0.f, 0.f);
+          const RowOut<T, D> dst(a, u, row, live, 0.f, 0.f);
           const float zero[32] = {};
           for (int c = 0; c < D; c += 32) dst.store32(c, zero);
         }
         continue;
       }
-      softmax_sync();  // both streams are done with the last item's Q and O
+      softmax_sync();  // both streams are done with the last unit's Q and O
       {
         // Q, 16 bytes per step, 128-byte swizzle; rows past the last are zero
         constexpr int kVecs = D / 8, kStep = kSoftmaxThreads / kVecs;
-        const T* q = reinterpret_cast<const T*>(a.q) + (int64_t)it.h * a.group * a.q_h;
-        const int c = threadIdx.x % kVecs, rows = alternate ? kTileRows : kItemRows;
+        const T* q = reinterpret_cast<const T*>(a.q) + (int64_t)u.h * a.group * a.q_h;
+        const int c = threadIdx.x % kVecs, rows = alternate ? kTileRows : kUnitRows;
 #pragma unroll 4
         for (int j = threadIdx.x / kVecs; j < rows; j += kStep) {
           uint4 v = make_uint4(0, 0, 0, 0);
-          if (j < it.rows) {
-            const int flat = it.row0 + j, b = flat / per_request;
+          if (j < u.rows) {
+            const int flat = u.row0 + j, b = flat / per_request;
             const int in = flat - b * per_request, i = in / a.group, g = in - i * a.group;
             v = ld_stream(q + b * a.q_b + i * a.q_t + g * a.q_h + c * 8);
           }
@@ -445,35 +457,84 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         mbar_arrive(q_full);
       }
-      // own rows that this query sees
-      int visible = 0;
-      if (it.b >= 0) visible = own_visible(a, it.len, (it.row0 - it.b * per_request + min(row, it.rows - 1)) / a.group);
-      const bool warp_live = (alternate ? 0 : s * kTileRows) + ((warp & 3) << 5) < it.rows;
+      // this row's request and how many of its own rows it sees
+      const int flat = u.row0 + min(row, u.rows - 1), my_b = flat / per_request;
+      const int visible = a.own > 0 ? own_visible(a, own_len(a, my_b), (flat - my_b * per_request) / a.group) : 0;
+      const bool warp_live = (alternate ? 0 : s * kTileRows) + ((warp & 3) << 5) < u.rows;
       const int steps = alternate ? (n + 1 - s) / 2 : n;
+      // of a unit within one request: own rows that all of its rows see
+      const int seen_by_all =
+          a.own > 0 ? own_visible(a, own_len(a, u.b0), (u.row0 - u.b0 * per_request) / a.group) : 0;
+      bool poisoned = false;
+      Walk w(a, u, u.first);
+      if (alternate && s == 1) w.next(a, u);
       float m = -INFINITY, l = 0.f;
       for (int t = 0; t < steps; ++t, ++count) {
-        const int local = alternate ? 2 * t + s : t, tile = it.first + local;
-        const bool own = tile >= it.prefix_tiles;
-        const int key0 = (own ? tile - it.prefix_tiles : tile) * kTileKeys;
-        const int limit = min(kTileKeys, (own ? visible : a.prefix) - key0);
-        if (!wait(s_full(s), count)) break;
+        const bool own = w.b >= 0;
+        const int key0 = w.t * kTileKeys;
+        const int limit = min(kTileKeys, (own ? (my_b == w.b ? visible : 0) : a.prefix) - key0);
+        wait(s_full(s), count);
         tc_fence_after();
-        if (own && key0 + kTileKeys > it.len && it.len < a.own && (alternate || s == 0)) {
-          // cache rows past the request's length hold anything: their p is 0, but 0 * inf is
-          // not (a tile that both streams use: stream 0's product comes first)
-          const int idx = at + v_index(alternate, local, n), slot = idx % kRing;
-          if (!wait(full(slot), idx / kRing)) break;
-          if (key0 + r >= it.len) {
+        if (own) {
+          // Value rows that not every row here sees must not reach the others' products, where
+          // p is 0 but 0 * inf is not: cache rows past the request's length, which hold
+          // anything, and rows with an infinity or a NaN where requests or causal limits
+          // differ.  They are zeroed (a tile that both streams use: by stream 0, whose product
+          // comes first); a row that does see such a value gives NaN.
+          const int len = own_len(a, w.b);
+          const bool guarded = u.b0 != u.b1 || key0 + kTileKeys > seen_by_all;
+          const bool ends = len < a.own && key0 + kTileKeys > len;
+          int* const first_bad = reinterpret_cast<int*>(gbase + S::kGuard) + (guards & 1) * 8 + (alternate ? s * 4 : 0);
+          if ((guarded || ends) && (alternate || s == 0)) {
+            const int idx = at + v_index(alternate, alternate ? 2 * t + s : t, n), slot = idx % kRing;
+            wait(full(slot), idx / kRing);
+            uint8_t* const vrow = gbase + S::kKV + slot * S::kTile + r * 128;
+            bool zero = ok && key0 + r >= len, bad = false;
+            if (ok && guarded && !zero) {
+              uint32_t mag = 0;
 #pragma unroll
-            for (int x = 0; x < D / 64; ++x)
+              for (int c = 0; c < D / 8; ++c) {
+                const uint4 x = *reinterpret_cast<const uint4*>(vrow + (c / 8) * kBox + (((c ^ r) & 7) << 4));
+                mag = absmax16x2<T>(absmax16x2<T>(absmax16x2<T>(absmax16x2<T>(mag, x.x), x.y), x.z), x.w);
+              }
+              zero = bad = !isfinite(bits16_to_f<T>(amax16_bits(mag)));
+            }
+            if (zero) {
 #pragma unroll
-              for (int c = 0; c < 8; ++c)
-                *reinterpret_cast<uint4*>(gbase + S::kKV + slot * S::kTile + x * kBox + r * 128 + c * 16) =
-                    make_uint4(0, 0, 0, 0);
+              for (int c = 0; c < D / 8; ++c)
+                *reinterpret_cast<uint4*>(vrow + (c / 8) * kBox + (((c ^ r) & 7) << 4)) = make_uint4(0, 0, 0, 0);
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            if (guarded) {
+              const int low = __reduce_min_sync(0xffffffffu, bad ? r : kTileKeys);
+              if (lane == 0) first_bad[warp & 3] = low;
+            }
           }
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          if (guarded) {
+            if (!alternate && s == 0) asm volatile("bar.arrive 4, 256;" ::: "memory");
+            if (s == 0)
+              asm volatile("bar.sync 2, 128;" ::: "memory");
+            else if (alternate)
+              asm volatile("bar.sync 3, 128;" ::: "memory");
+            else  // what stream 0 found
+              asm volatile("bar.sync 4, 256;" ::: "memory");
+            const int low = min(min(first_bad[0], first_bad[1]), min(first_bad[2], first_bad[3]));
+            poisoned = poisoned || low < limit;
+            ++guards;
+          }
         }
-        if (warp_live) {
+        if (!ok) {
+          // a wait ran out: the rest of the walk is only gone through, for the barriers in it
+        } else if (warp_live && !__any_sync(0xffffffffu, limit > 0)) {
+          // a request's own rows, none of whose queries is here
+          const uint32_t p[32] = {};
+          tmem_st32(t_s, p);
+          tmem_st32(t_s + 32, p);
+          tmem_st_wait();
+          tc_fence_before();
+          mbar_arrive(p_full(s, 0));
+          mbar_arrive(p_full(s, 1));
+        } else if (warp_live) {
           const bool masked = __any_sync(0xffffffffu, limit < kTileKeys);
           uint32_t v[128];
           tmem_ld128(t_s, v);
@@ -531,12 +592,14 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
           mbar_arrive(p_full(s, 0));
           mbar_arrive(p_full(s, 1));
         }
+        w.next(a, u);
+        if (alternate) w.next(a, u);
       }
       if (steps > 0) wait(o_full(s), o_count[s]);
       if (!alternate) {
         tc_fence_after();
-        const RowOut<T, D> dst(a, it, row, live && ok, m, l);
-        const float inv = l == 0.f ? 0.f : 1.f / l;
+        const RowOut<T, D> dst(a, u, row, live && ok, m, l);
+        const float inv = poisoned ? __int_as_float(0x7fffffff) : l == 0.f ? 0.f : 1.f / l;
         if (warp_live && ok) {
 #pragma unroll 1
           for (int c = 0; c < D; c += 32) {
@@ -551,17 +614,19 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       } else {
         // join the streams: stream 0's warps read both O
         float2* const join = reinterpret_cast<float2*>(gbase + S::kJoin);
-        if (s == 1) join[r] = make_float2(m, l);
+        if (s == 1) join[r] = make_float2(m, poisoned ? -l : l);  // l >= 0: the sign bit is free
         softmax_sync();
         if (s == 0) {
           if (n > 1) wait(o_full(1), o_count[1]);
           tc_fence_after();
-          const float2 other = n > 1 ? join[r] : make_float2(-INFINITY, 0.f);
+          float2 other = n > 1 ? join[r] : make_float2(-INFINITY, 0.f);
+          poisoned = poisoned || signbit(other.y);
+          other.y = fabsf(other.y);
           const float top = fmaxf(m, other.x), shift = top == -INFINITY ? 0.f : top;
           float f0 = ex2_approx(m - shift), f1 = ex2_approx(other.x - shift);
           const float sum = f0 * l + f1 * other.y;
-          const RowOut<T, D> dst(a, it, row, live && ok, shift, sum);
-          const float inv = sum == 0.f ? 0.f : 1.f / sum;
+          const RowOut<T, D> dst(a, u, row, live && ok, shift, sum);
+          const float inv = poisoned ? __int_as_float(0x7fffffff) : sum == 0.f ? 0.f : 1.f / sum;
           f0 *= inv;
           f1 *= inv;
           if (warp_live && ok) {
@@ -595,9 +660,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
   }
 }
 
-// Joins the parts of each row by their log2-sum-exps: one warp per row.  With own parts,
-// every row has them and one part (whole items) or `splits` over the prefix; without, only
-// the split items' rows are here.
+// Joins the parts of each row of the split units by their log2-sum-exps: one warp per row.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) prefix_attn_join_kernel(const AttnArgs a, int64_t total) {
   constexpr int E = D / 32;
@@ -607,37 +670,14 @@ __global__ void __launch_bounds__(256) prefix_attn_join_kernel(const AttnArgs a,
   pdl_trigger();
   if (w >= total) return;
   const int per_request = a.lq * a.group;
-  int h, row, parts;
-  int64_t slot0, step;
-  if (a.own_splits == 0) {
-    const int item = a.whole + (int)(w / kItemRows), r = (int)(w % kItemRows);
-    int grp, t;
-    tile_of(a, item, grp, t);
-    h = a.fused ? grp / a.batch : grp;
-    const int b = a.fused ? grp - h * a.batch : 0;
-    if (t * kItemRows + r >= (a.fused ? (int64_t)per_request : a.rows)) return;
-    row = b * per_request + t * kItemRows + r;
-    parts = a.splits;
-    slot0 = a.slot_tail + (w / kItemRows) * parts * kItemRows + r;
-    step = kItemRows;
-  } else {
-    h = (int)(w / a.rows);
-    row = (int)(w - h * a.rows);
-    const int t = row / kItemRows, full = a.row_tiles - 1;
-    const int item = t < full ? h * full + t : a.heads * full + h;
-    if (item < a.whole) {
-      parts = 1;
-      slot0 = h * a.rows + row;
-      step = 0;
-    } else {
-      parts = a.splits;
-      slot0 = a.slot_tail + (int64_t)(item - a.whole) * parts * kItemRows + row - t * kItemRows;
-      step = kItemRows;
-    }
-  }
-  const int64_t own0 = a.slot_own + (int64_t)h * a.rows + row, own_step = a.heads * a.rows;
-  const int all = parts + a.own_splits;
-  auto slot_of = [&](int s) { return s < parts ? slot0 + s * step : own0 + (s - parts) * own_step; };
+  const int j = (int)(w / a.tile_rows), r = (int)(w - (int64_t)j * a.tile_rows);
+  int grp, t;
+  tile_of(a, a.whole + j, grp, t);
+  const int h = a.within_request ? grp / a.batch : grp, b0 = a.within_request ? grp - h * a.batch : 0;
+  if (t * a.tile_rows + r >= (a.within_request ? per_request : a.rows)) return;
+  const int row = b0 * per_request + t * a.tile_rows + r, all = a.splits;
+  const int64_t slot0 = (int64_t)j * all * a.tile_rows + r;
+  auto slot_of = [&](int s) { return slot0 + (int64_t)s * a.tile_rows; };
   float top = -INFINITY;
   for (int s = lane; s < all; s += 32) top = fmaxf(top, a.part_lse[slot_of(s)]);
   top = warp_max(top);
@@ -670,81 +710,66 @@ __global__ void __launch_bounds__(256) prefix_attn_join_kernel(const AttnArgs a,
 
 // ------------------------------------------------------------------ host side
 struct Plan {
-  bool fused;
-  int64_t groups, row_tiles, items, whole, splits, own_tiles, own_splits, blocks, rows;
-  int64_t slot_tail, slot_own, slots, joined;
+  bool within_request;
+  int64_t tile_rows, groups, row_tiles, items, whole, splits, units, rows, slots;
   double cost;  // key tiles that the longest-working SM walks, and what joining costs
 };
 
-// What a unit costs beside its tiles (Q, the results, the pipeline's ends) and what its rows'
-// parts cost to join, in key tiles; measured on single tokens (about 1 us each).
+// What a unit costs beside its tiles (finding it, Q, the pipeline's ends, the results) and
+// what joining costs, in steps of 128 keys and 256 rows.
 constexpr double kUnitTiles = 2.0, kJoinTiles = 1.0;
+// A step of a unit of up to 128 rows takes two tiles, which is as much to load as two steps.
+constexpr double kHalfStep = 0.6;
 
-// How many parts the items that do not fill the last round over `hold` CTAs are split in, and
-// the time of all of them in tiles.
-int64_t best_split(int64_t tail, int64_t tiles, int64_t hold, double per_tile, double* cost) {
-  int64_t best = 1;
-  const int64_t most = tiles / 2 < 1 ? 1 : tiles / 2 < hold ? tiles / 2 : hold;
-  for (int64_t s = 1; s <= most; ++s) {
-    const double c = (double)cdiv(tail * s, hold) * ((double)cdiv(tiles, s) * per_tile + kUnitTiles) +
-                     (s > 1 ? kJoinTiles + 0.05 * (double)s : 0.);
-    if (s == 1 || c < *cost) {
-      *cost = c;
-      best = s;
-    }
-  }
-  return best;
-}
-
-Plan make_plan(bool fused, int64_t batch, int64_t lq, int64_t heads, int64_t group, int64_t prefix, int64_t own,
-               int64_t hold) {
+Plan make_plan(bool within_request, int64_t tile_rows, int64_t batch, int64_t lq, int64_t heads, int64_t group,
+               int64_t prefix, int64_t own, int64_t hold) {
   Plan p{};
   const int64_t per_request = lq * group;
-  const int64_t ptiles = cdiv(prefix, kTileKeys), otiles = cdiv(own, kTileKeys);
-  p.fused = fused;
+  p.within_request = within_request;
   p.rows = batch * per_request;
-  const int64_t tile_rows = fused ? per_request : p.rows;
-  p.groups = fused ? heads * batch : heads;
-  p.row_tiles = cdiv(tile_rows, kItemRows);
-  p.items = fused || prefix > 0 ? p.groups * p.row_tiles : 0;
-  p.splits = 1;
-  const int64_t tiles = fused ? ptiles + otiles : ptiles;
-  // up to 128 rows: two tiles per step
-  const double per_tile = tile_rows <= kTileRows ? 0.5 : 1.0;
+  p.tile_rows = tile_rows;
+  p.groups = within_request ? heads * batch : heads;
+  p.row_tiles = cdiv(within_request ? per_request : p.rows, tile_rows);
+  p.items = p.groups * p.row_tiles;
+  // requests that a row tile meets
+  int64_t met = within_request ? 1 : tile_rows / per_request + (tile_rows % per_request ? 2 : 0);
+  if (met > batch) met = batch;
+  const int64_t tiles = cdiv(prefix, kTileKeys) + met * cdiv(own, kTileKeys);
+  const double step = tile_rows <= kTileRows ? kHalfStep : 1.0;
   p.whole = p.items / hold * hold;
-  p.cost = (double)(p.whole / hold) * ((double)tiles * per_tile + kUnitTiles);
-  if (p.items > p.whole) {
-    double c;
-    p.splits = best_split(p.items - p.whole, tiles, hold, per_tile, &c);
-    p.cost += c;
+  p.cost = (double)(p.whole / hold) * ((double)tiles * step + kUnitTiles);
+  p.splits = 1;
+  if (const int64_t tail = p.items - p.whole) {
+    // the items that do not fill a last round over the SMs: the number of parts that ends first
+    const int64_t most = tiles / 2 < 1 ? 1 : tiles / 2 < hold ? tiles / 2 : hold;
+    double best = 0.;
+    for (int64_t s = 1; s <= most; ++s) {
+      const double c = (double)cdiv(tail * s, hold) * ((double)cdiv(tiles, s) * step + kUnitTiles) +
+                       (s > 1 ? kJoinTiles + 0.05 * (double)s : 0.);
+      if (s == 1 || c < best) {
+        best = c;
+        p.splits = s;
+      }
+    }
+    p.cost += best;
   }
   if (p.splits == 1) p.whole = p.items;
-  p.blocks = p.whole + (p.items - p.whole) * p.splits;
-  if (!fused && own > 0) {
-    p.own_tiles = cdiv(per_request, kItemRows);
-    const int64_t units = heads * batch * p.own_tiles;
-    const double per = per_request <= kTileRows ? 0.5 : 1.0;
-    double c;
-    p.own_splits = units < hold ? best_split(units, otiles, hold, per, &c) : 1;
-    if (units >= hold) c = (double)units / (double)hold * ((double)otiles * per + kUnitTiles);
-    p.cost += c + kJoinTiles;
-    p.blocks += units * p.own_splits;
-  }
-  const bool keep = p.own_splits > 0;
-  p.slot_tail = keep && p.whole > 0 ? heads * p.rows : 0;
-  p.slot_own = p.slot_tail + (p.items - p.whole) * p.splits * kItemRows;
-  p.slots = p.slot_own + p.own_splits * heads * p.rows;
-  p.joined = keep ? heads * p.rows : (p.items - p.whole) * kItemRows;
+  p.units = p.whole + (p.items - p.whole) * p.splits;
+  p.slots = (p.items - p.whole) * p.splits * tile_rows;
   return p;
 }
 
 // `hold`: CTAs that the GPU holds at once (one per SM).
 Plan plan_attention(int64_t batch, int64_t lq, int64_t heads, int64_t group, int64_t prefix, int64_t own,
                     int64_t hold) {
-  const Plan fused = make_plan(true, batch, lq, heads, group, prefix, own, hold);
-  if (prefix == 0 || batch == 1) return fused;
-  const Plan packed = make_plan(false, batch, lq, heads, group, prefix, own, hold);
-  return packed.cost < fused.cost ? packed : fused;
+  Plan best{};
+  for (int64_t tile_rows : {(int64_t)kUnitRows, (int64_t)kTileRows})
+    for (bool within : {true, false}) {
+      if (!within && batch == 1) continue;
+      const Plan p = make_plan(within, tile_rows, batch, lq, heads, group, prefix, own, hold);
+      if (best.units == 0 || p.cost < best.cost) best = p;
+    }
+  return best;
 }
 
 int check_sizes(const char* op, int64_t batch, int64_t lq, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
@@ -785,13 +810,13 @@ int launch_attention(const CUtensorMap* maps, const AttnArgs& a, const Plan& p, 
   constexpr int smem = AttnSmem<D>::kBytes;
   static std::atomic<uint64_t> reserved{0};
   if (int s = reserve_smem((const void*)kern, smem, reserved, di, op)) return s;
-  if (cudaError_t e = launch_pdl(kern, dim3((unsigned)(p.blocks < di->sm_count ? p.blocks : di->sm_count)), dim3(kAttnThreads), smem, st, maps[0], maps[1],
+  if (cudaError_t e = launch_pdl(kern, dim3((unsigned)(p.units < di->sm_count ? p.units : di->sm_count)), dim3(kAttnThreads), smem, st, maps[0], maps[1],
                                  maps[2], maps[3], a))
     return launch_failed(e, op);
   if (int s = after_launch("prefix_attn_kernel")) return s;
-  if (p.joined) {
-    if (cudaError_t e = launch_pdl(prefix_attn_join_kernel<T, D>, dim3((unsigned)cdiv(p.joined, 8)), dim3(256), 0, st,
-                                   a, p.joined))
+  if (const int64_t joined = (p.items - p.whole) * p.tile_rows) {
+    if (cudaError_t e = launch_pdl(prefix_attn_join_kernel<T, D>, dim3((unsigned)cdiv(joined, 8)), dim3(256), 0, st, a,
+                                   joined))
       return launch_failed(e, op);
     return after_launch("prefix_attn_join_kernel");
   }
@@ -832,9 +857,9 @@ int jo_shared_prefix_attention(void* out, float* lse, const void* q, int64_t q_s
   if (batch == 0 || q_len == 0) return JO_OK;
   if (!out || !lse || !q || !lens || (prefix_len && (!k_prefix || !v_prefix)) || (own_len && (!k_own || !v_own)))
     return fail(JO_ERR_INVALID, "%s: null operand", op);
-  if (!aligned16(out) || !aligned16(q) || !aligned16(k_prefix) || !aligned16(v_prefix) || !aligned16(k_own) ||
+  if ((reinterpret_cast<uintptr_t>(out) & 31) || !aligned16(q) || !aligned16(k_prefix) || !aligned16(v_prefix) || !aligned16(k_own) ||
       !aligned16(v_own))
-    return fail(JO_ERR_ALIGN, "%s: operands must be 16-byte aligned", op);
+    return fail(JO_ERR_ALIGN, "%s: operands must be 16-byte aligned (out: 32)", op);
   // a stride of a dimension of size 1 is never used
   const struct {
     int64_t size, stride;
@@ -848,9 +873,9 @@ int jo_shared_prefix_attention(void* out, float* lse, const void* q, int64_t q_s
     if (u.size > 1 && (u.stride % 8 || u.stride < 0))
       return fail(JO_ERR_ALIGN, "%s: strides must be multiples of 16 bytes and not negative", op);
   const Plan p = plan_attention(batch, q_len, kv_heads, q_heads / kv_heads, prefix_len, own_len, di->sm_count);
-  if (p.blocks > INT32_MAX || cdiv(p.joined, 8) > INT32_MAX) return fail(JO_ERR_SHAPE, "%s: size too large", op);
-  if (p.slots && (!workspace || !aligned16(workspace) || workspace_bytes < p.slots * (head_dim + 1) * 4))
-    return fail(JO_ERR_INVALID, "%s: a 16-byte aligned workspace of %lld bytes is needed", op,
+  if (p.units > INT32_MAX / 2) return fail(JO_ERR_SHAPE, "%s: size too large", op);
+  if (p.slots && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 31) || workspace_bytes < p.slots * (head_dim + 1) * 4))
+    return fail(JO_ERR_INVALID, "%s: a 32-byte aligned workspace of %lld bytes is needed", op,
                 (long long)(p.slots * (head_dim + 1) * 4));
   AttnArgs a{};
   a.out = out;
@@ -868,18 +893,15 @@ int jo_shared_prefix_attention(void* out, float* lse, const void* q, int64_t q_s
   a.own = (int)own_len;
   a.causal = causal;
   a.scale_log2 = scale * kLog2E;
-  a.fused = p.fused;
+  a.within_request = p.within_request;
+  a.tile_rows = (int)p.tile_rows;
   a.groups = (int)p.groups;
   a.row_tiles = (int)p.row_tiles;
   a.items = (int)p.items;
   a.whole = (int)p.whole;
   a.splits = (int)p.splits;
-  a.own_tiles = (int)p.own_tiles;
-  a.own_splits = (int)p.own_splits;
-  a.blocks = (int)p.blocks;
-  a.rows = p.rows;
-  a.slot_tail = p.slot_tail;
-  a.slot_own = p.slot_own;
+  a.units = (int)p.units;
+  a.rows = (int)p.rows;
   a.part_o = (float*)workspace;
   a.part_lse = (float*)workspace + p.slots * head_dim;
   a.fault = di->fault;
