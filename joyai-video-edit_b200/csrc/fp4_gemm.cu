@@ -221,7 +221,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       mbar_init(empty_bar(s), 1);
     }
     mbar_init(tfull, 1);
-    mbar_init(drained, 2 * kEpiWarps * 32);  // the epilogue threads of both CTAs
+    mbar_init(drained, 2 * kEpiWarps);  // the epilogue warps of both CTAs
     mbar_init(done, 1);
     mbar_init_fence();
   }
@@ -327,10 +327,13 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     };
     auto drained_by_us = [&]() {
       tc_fence_before();
-      if (leader)
-        mbar_arrive(drained);
-      else
-        mbar_arrive_cluster(cluster_addr(drained, 0));
+      __syncwarp();
+      if (lane == 0) {
+        if (leader)
+          mbar_arrive(drained);
+        else
+          mbar_arrive_cluster(cluster_addr(drained, 0));
+      }
     };
     int i = 0;
     for (int tile = cluster; tile < num_tiles; tile += nclusters, ++i) {

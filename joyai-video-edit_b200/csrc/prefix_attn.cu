@@ -54,9 +54,18 @@ constexpr int kTileRows = 128;           // rows per stream (UMMA M)
 constexpr int kUnitRows = 2 * kTileRows;  // rows per unit at most
 constexpr int kTileKeys = 128;           // keys per tile (UMMA N of S, K of P V)
 constexpr int kSoftmaxThreads = 256;
-constexpr int kAttnThreads = 320;
+constexpr int kAttnThreads = 384;  // two softmax warpgroups; producer, issuer and two idle warps
+// The launch gives each of the 384 threads 168 registers, 64,512 in all; the softmax threads
+// hold a row of S (128 values) and take 224 each, the others keep 56: 64,512.
+constexpr int kSoftmaxRegs = 224, kOtherRegs = 56;
 constexpr int kColO = 256;  // tensor memory: S / P of the streams at 0 and 128, O at 256 and 384
 constexpr float kRaise = 8.f;
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
 
 struct AttnArgs {
   void* out;
@@ -114,14 +123,21 @@ __device__ __forceinline__ void tile_of(const AttnArgs& a, int item, int& grp, i
 }
 
 // Work unit `index`; by a converged warp.
-__device__ Unit unit_of(const AttnArgs& a, int index) {
+__device__ __forceinline__ Unit unit_of(const AttnArgs& a, int index) {
   Unit u;
   const int per_request = a.lq * a.group, lane = threadIdx.x & 31;
   int piece = 0, pieces = 1, item = index, grp, t;
   if (index >= a.whole) {
-    const int tail = a.items - a.whole, j = index - a.whole;
+    // the parts of full row tiles first, then those of the groups' last tiles
+    const int full = a.groups * (a.row_tiles - 1), cut = max(a.whole, full);
+    int j = index - a.whole, first = a.whole, tail = cut - a.whole;
+    if (j >= tail * a.splits) {
+      j -= tail * a.splits;
+      first = cut;
+      tail = a.items - cut;
+    }
     piece = j / tail;
-    item = a.whole + j - piece * tail;
+    item = first + j - piece * tail;
     pieces = a.splits;
   }
   tile_of(a, item, grp, t);
@@ -214,12 +230,22 @@ struct AttnSmem {
 // The ring's order of loads for n tiles, which is the order of their first use.
 //   shared by both streams:  K0 V0 K1 V1 ...
 //   alternate tiles:         K0 K1 V0 K2 V1 K3 ... V(n-2) V(n-1)
-__device__ __forceinline__ int k_index(bool alternate, int tile) {
-  return alternate ? (tile < 2 ? tile : 2 * tile - 1) : 2 * tile;
-}
 __device__ __forceinline__ int v_index(bool alternate, int tile, int n) {
   return alternate ? (tile == n - 1 ? 2 * n - 1 : 2 * tile + 2) : 2 * tile + 1;
 }
+// A place in the ring: slot, and the parity of its full barrier.
+template <int kRing>
+struct Ring {
+  int slot = 0;
+  uint32_t phase = 0;
+  __device__ __forceinline__ void advance(int by) {  // by <= kRing
+    slot += by;
+    if (slot >= kRing) {
+      slot -= kRing;
+      phase ^= 1u;
+    }
+  }
+};
 // Whether load `idx` is a V tile.
 __device__ __forceinline__ bool value_at(bool alternate, int idx, int n) {
   if (!alternate) return idx & 1;
@@ -293,12 +319,12 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       mbar_init(full(s), 1);
       mbar_init(empty(s), 1);
     }
-    mbar_init(q_full, kSoftmaxThreads);
+    mbar_init(q_full, kSoftmaxThreads / 32);
     mbar_init(done, 1);
     for (int s = 0; s < 2; ++s) {
       mbar_init(s_full(s), 1);
-      mbar_init(p_full(s, 0), kTileRows);
-      mbar_init(p_full(s, 1), kTileRows);
+      mbar_init(p_full(s, 0), kTileRows / 32);  // one arrival per warp
+      mbar_init(p_full(s, 1), kTileRows / 32);
       mbar_init(o_full(s), 1);
     }
     mbar_init_fence();
@@ -310,108 +336,144 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
   pdl_wait();  // lens, q, k and v may be the previous kernel's
   pdl_trigger();
 
-  if (warp == 8) {
-    // ---------------- TMA producer (lane 0; the warp finds the units together)
-    int at = 0;  // loads so far
-    bool ok = true;
-    for (int unit = blockIdx.x; unit < a.units; unit += gridDim.x) {
-      const Unit u = unit_of(a, unit);
-      const int n = u.last - u.first;
-      if (n == 0) continue;
-      const bool alternate = u.rows <= kTileRows;
-      Walk walk[2] = {Walk(a, u, u.first), Walk(a, u, u.first)};  // of K, of V
-      for (int j = 0; j < 2 * n && lane == 0 && ok; ++j, ++at) {
-        const int slot = at % kRing;
-        if (!(ok = mbar_wait(empty(slot), ((at / kRing) & 1) ^ 1u, a.fault))) break;
-        const bool value = value_at(alternate, j, n);
-        Walk& w = walk[value];
-        const bool own = w.b >= 0;
-        const CUtensorMap* map = value ? (own ? &map_vo : &map_vp) : (own ? &map_ko : &map_kp);
-        mbar_expect_tx(full(slot), S::kTile);
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+    if (warp == 8) {
+      // ---------------- TMA producer (lane 0; the warp finds the units together)
+      int at = 0;  // loads so far
+      bool ok = true;
+      for (int unit = blockIdx.x; unit < a.units; unit += gridDim.x) {
+        const Unit u = unit_of(a, unit);
+        const int n = u.last - u.first;
+        if (n == 0) continue;
+        const bool alternate = u.rows <= kTileRows;
+        Walk wk(a, u, u.first), wv(wk);  // of K, of V
+        for (int j = 0; j < 2 * n && lane == 0 && ok; ++j, ++at) {
+          const int slot = at % kRing;
+          if (!(ok = mbar_wait(empty(slot), ((at / kRing) & 1) ^ 1u, a.fault))) break;
+          auto load = [&](const CUtensorMap* prefix, const CUtensorMap* own, Walk& w) {
+            mbar_expect_tx(full(slot), S::kTile);
 #pragma unroll
-        for (int x = 0; x < D; x += 64)
-          tma_load_4d(base + S::kKV + slot * S::kTile + (x / 64) * kBox, map, x, u.h, w.t * kTileKeys, own ? w.b : 0,
-                      full(slot));
-        w.next(a, u);
+            for (int x = 0; x < D; x += 64)
+              tma_load_4d(base + S::kKV + slot * S::kTile + (x / 64) * kBox, w.b < 0 ? prefix : own, x, u.h,
+                          w.t * kTileKeys, max(w.b, 0), full(slot));
+            w.next(a, u);
+          };
+          if (value_at(alternate, j, n))
+            load(&map_vp, &map_vo, wv);
+          else
+            load(&map_kp, &map_ko, wk);
+        }
+        __syncwarp();
       }
-      __syncwarp();
-    }
-    // every copy issued has landed before the CTA may exit
-    if (lane == 0)
-      for (int j = max(0, at - kRing); j < at; ++j) mbar_wait(full(j % kRing), (j / kRing) & 1, a.fault);
-  } else if (warp == 9) {
-    // ---------------- MMA issuer: the warp stays converged and elects one thread per step
-    constexpr uint32_t idesc_s = attn_idesc<T>(kTileKeys, false), idesc_o = attn_idesc<T>(D, true);
-    const uint64_t qd = sw128_desc(base + S::kQ), kd0 = sw128_desc(base + S::kKV);
-    const uint64_t vd0 = sw128_desc_mn(base + S::kKV, kBox);
-    int at = 0, count[2] = {0, 0}, q_count = 0;
-    bool ok = true;
-    auto wait = [&](uint32_t bar, int phase) {
-      if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar, phase & 1, a.fault));
-      return ok;
-    };
-    for (int unit = blockIdx.x; unit < a.units && ok; unit += gridDim.x) {
-      const Unit u = unit_of(a, unit);
-      const int n = u.last - u.first;
-      if (n == 0) continue;
-      const bool alternate = u.rows <= kTileRows;
-      const int steps[2] = {alternate ? (n + 1) / 2 : n, alternate ? n / 2 : n};
-      auto products_s = [&](int s, int t) {  // S of stream s, step t
-        const int idx = at + k_index(alternate, alternate ? 2 * t + s : t), slot = idx % kRing;
-        if (!wait(full(slot), idx / kRing)) return;
+      // every copy issued has landed before the CTA may exit
+      if (lane == 0)
+        for (int j = max(0, at - kRing); j < at; ++j) mbar_wait(full(j % kRing), (j / kRing) & 1, a.fault);
+    } else if (warp == 9) {
+      // ---------------- MMA issuer: the warp stays converged and elects one thread per step
+      constexpr uint32_t idesc_s = attn_idesc<T>(kTileKeys, false), idesc_o = attn_idesc<T>(D, true);
+      const uint64_t qd0 = sw128_desc(base + S::kQ), kd0 = sw128_desc(base + S::kKV);
+      const uint64_t vd0 = sw128_desc_mn(base + S::kKV, kBox);
+      bool ok = true;
+      auto wait = [&](uint32_t bar, uint32_t phase) {
+        if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar, phase, a.fault));
         tc_fence_after();
-        if (elect_one()) {
-          const uint64_t kd = kd0 + slot * (S::kTile >> 4), q = qd + (alternate ? 0 : s * (S::kTile >> 4));
+      };
+      Ring<kRing> k, v;  // the next K and V tiles
+      uint32_t p_phase[2] = {0, 0}, q_phase = 0;
+      // S of stream s; `last`: no other stream uses the K tile
+      auto products_s = [&](int s, const Ring<kRing>& at, bool alternate, bool last) {
+        if (ok && elect_one()) {
+          const uint64_t kd = kd0 + at.slot * (S::kTile >> 4), qd = qd0 + (alternate ? 0 : s * (S::kTile >> 4));
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk) {
             const int off = ((kk / 4) * kBox + (kk % 4) * 32) >> 4;
-            tc_mma_f16_ss(tmem + s * kTileKeys, q + off, kd + off, idesc_s, kk != 0);
+            tc_mma_f16_ss(tmem + s * kTileKeys, qd + off, kd + off, idesc_s, kk != 0);
           }
-          if (alternate || s == 1) tc_commit(empty(slot));
           tc_commit(s_full(s));
+          if (last) tc_commit(empty(at.slot));
         }
         __syncwarp();
       };
-      auto products_o = [&](int s, int t) {  // O of stream s, step t
-        const int idx = at + v_index(alternate, alternate ? 2 * t + s : t, n), slot = idx % kRing;
-        if (!wait(full(slot), idx / kRing)) return;
-        const uint64_t vd = vd0 + slot * (S::kTile >> 4);
+      // O of stream s
+      auto products_o = [&](int s, const Ring<kRing>& at, bool first, bool last, bool end) {
+        const uint64_t vd = vd0 + at.slot * (S::kTile >> 4);
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-          if (!wait(p_full(s, half), count[s])) return;
-          tc_fence_after();
-          if (elect_one()) {
+          wait(p_full(s, half), p_phase[s]);
+          if (ok && elect_one()) {
 #pragma unroll
             for (int kk = 4 * half; kk < 4 * half + 4; ++kk)
               tc_mma_f16_ts(tmem + kColO + s * kTileKeys, tmem + s * kTileKeys + kk * 8, vd + kk * (2048 >> 4), idesc_o,
-                            t != 0 || kk != 0);
+                            !first || kk != 0);
             if (half == 1) {
-              if (alternate || s == 1) tc_commit(empty(slot));
-              if (t == steps[s] - 1) tc_commit(o_full(s));
+              if (last) tc_commit(empty(at.slot));
+              if (end) tc_commit(o_full(s));
             }
           }
           __syncwarp();
         }
-        ++count[s];
+        p_phase[s] ^= 1u;
       };
-      if (!wait(q_full, q_count++)) break;
-      products_s(0, 0);
-      if (steps[1] > 0) products_s(1, 0);
-      for (int t = 0; t < steps[0] && ok; ++t) {
+      for (int unit = blockIdx.x; unit < a.units && ok; unit += gridDim.x) {
+        const Unit u = unit_of(a, unit);
+        const int n = u.last - u.first;
+        if (n == 0) continue;
+        wait(q_full, q_phase);
+        q_phase ^= 1u;
+        if (u.rows > kTileRows) {
+          // both streams use every tile: K0 V0 K1 V1 ...
+          v = k;
+          v.advance(1);
+          wait(full(k.slot), k.phase);
+          products_s(0, k, false, false);
+          products_s(1, k, false, true);
+          for (int t = 0; t < n && ok; ++t) {
+            const bool end = t == n - 1;
+            k.advance(2);
+            wait(full(v.slot), v.phase);
+            products_o(0, v, t == 0, false, end);
+            if (!end) {
+              wait(full(k.slot), k.phase);
+              products_s(0, k, false, false);
+            }
+            products_o(1, v, t == 0, true, end);
+            if (!end) products_s(1, k, false, true);
+            v.advance(2);
+          }
+        } else {
+          // alternate tiles: every load is used once, in the order of the loads
+          for (int s = 0; s < 2 && s < n; ++s) {
+            wait(full(k.slot), k.phase);
+            if (s == 0)
+              products_s(0, k, true, true);
+            else
+              products_s(1, k, true, true);
+            k.advance(1);
+          }
+          for (int t = 0; t < n && ok; t += 2) {
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
-          if (t >= steps[s]) continue;
-          products_o(s, t);
-          if (t + 1 < steps[s]) products_s(s, t + 1);
+            for (int s = 0; s < 2; ++s) {
+              if (t + s >= n) continue;
+              wait(full(k.slot), k.phase);
+              products_o(s, k, t == 0, true, t + s + 2 >= n);
+              k.advance(1);
+              if (t + s + 2 < n) {
+                wait(full(k.slot), k.phase);
+                products_s(s, k, true, true);
+                k.advance(1);
+              }
+            }
+          }
         }
       }
-      at += 2 * n;
+      // tensor memory is freed below: everything issued has retired, also after a failed wait
+      if (elect_one()) tc_commit(done);
+      __syncwarp();
+      mbar_wait(done, 0, a.fault);
     }
-    // tensor memory is freed below: everything issued has retired, also after a failed wait
-    if (elect_one()) tc_commit(done);
-    __syncwarp();
-    mbar_wait(done, 0, a.fault);
   } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
     // ---------------- softmax: stream s, thread r owns a row (tensor-memory lane r)
     const int s = warp >> 2, r = threadIdx.x & 127;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
@@ -421,6 +483,10 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     auto wait = [&](uint32_t bar, int phase) {
       if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar, phase & 1, a.fault));
       return ok;
+    };
+    auto arrive_warp = [&](uint32_t bar) {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar);
     };
     int count = 0, at = 0, guards = 0, o_count[2] = {0, 0};
     for (int unit = blockIdx.x; unit < a.units; unit += gridDim.x) {
@@ -455,7 +521,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
           *reinterpret_cast<uint4*>(gbase + S::kQ + off) = v;
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        mbar_arrive(q_full);
+        arrive_warp(q_full);
       }
       // this row's request and how many of its own rows it sees
       const int flat = u.row0 + min(row, u.rows - 1), my_b = flat / per_request;
@@ -532,23 +598,29 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
           tmem_st32(t_s + 32, p);
           tmem_st_wait();
           tc_fence_before();
-          mbar_arrive(p_full(s, 0));
-          mbar_arrive(p_full(s, 1));
+          arrive_warp(p_full(s, 0));
+          arrive_warp(p_full(s, 1));
         } else if (warp_live) {
           const bool masked = __any_sync(0xffffffffu, limit < kTileKeys);
+          // S in two halves, the second under way while the first's maximum is found
           uint32_t v[128];
-          tmem_ld128(t_s, v);
-          if (masked) {
-#pragma unroll
-            for (int e = 0; e < 128; ++e) v[e] = e < limit ? v[e] : 0xff800000u;
-          }
+          tmem_ld64_async(t_s, v);
+          tmem_ld_wait64(v);
+          tmem_ld64_async(t_s + 64, v + 64);
           float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-          for (int e = 0; e < 128; e += 8)
+          for (int half = 0; half < 2; ++half) {
+            if (half == 1) tmem_ld_wait64(v + 64);
+            if (masked) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-              mx[j] = fmaxf(fmaxf(mx[j], __uint_as_float(v[e + j])), __uint_as_float(v[e + 4 + j]));
-          const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale_log2;
+              for (int e = half * 64; e < half * 64 + 64; ++e) v[e] = e < limit ? v[e] : 0xff800000u;
+            }
+#pragma unroll
+            for (int e = half * 64; e < half * 64 + 64; e += 8)
+#pragma unroll
+              for (int j = 0; j < 4; ++j) mx[j] = max3(mx[j], __uint_as_float(v[e + j]), __uint_as_float(v[e + 4 + j]));
+          }
+          const float top = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) * a.scale_log2;
           const bool raise = top > m + kRaise;
           float fac = 1.f;
           if (raise) {
@@ -572,25 +644,28 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
           float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
-            uint32_t p[32];
 #pragma unroll
-            for (int e = 0; e < 64; e += 2) {
-              const float2 x = __ffma2_rn(make_float2(__uint_as_float(v[half * 64 + e]), __uint_as_float(v[half * 64 + e + 1])),
-                                          scale2, shift2);
-              const float2 y = make_float2(ex2_approx(x.x), ex2_approx(x.y));
-              sum[(e >> 1) & 1] = __fadd2_rn(sum[(e >> 1) & 1], y);
-              p[e / 2] = pack16<T>(y.x, y.y);
+            for (int c = half * 64; c < half * 64 + 64; c += 32) {
+              uint32_t p[16];
+#pragma unroll
+              for (int e = 0; e < 32; e += 2) {
+                const float2 x = __ffma2_rn(make_float2(__uint_as_float(v[c + e]), __uint_as_float(v[c + e + 1])),
+                                            scale2, shift2);
+                const float2 y = make_float2(ex2_approx(x.x), ex2_approx(x.y));
+                sum[(e >> 1) & 1] = __fadd2_rn(sum[(e >> 1) & 1], y);
+                p[e / 2] = pack16<T>(y.x, y.y);
+              }
+              tmem_st16(t_s + c / 2, p);
             }
-            tmem_st32(t_s + half * 32, p);
             tmem_st_wait();
             tc_fence_before();
-            mbar_arrive(p_full(s, half));
+            arrive_warp(p_full(s, half));
           }
           l = l * fac + ((sum[0].x + sum[0].y) + (sum[1].x + sum[1].y));
         } else {
           tc_fence_before();
-          mbar_arrive(p_full(s, 0));
-          mbar_arrive(p_full(s, 1));
+          arrive_warp(p_full(s, 0));
+          arrive_warp(p_full(s, 1));
         }
         w.next(a, u);
         if (alternate) w.next(a, u);
@@ -599,7 +674,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       if (!alternate) {
         tc_fence_after();
         const RowOut<T, D> dst(a, u, row, live && ok, m, l);
-        const float inv = poisoned ? __int_as_float(0x7fffffff) : l == 0.f ? 0.f : 1.f / l;
+        const float inv = poisoned ? __int_as_float(0x7fffffff) : l == 0.f ? 0.f : rcp_approx(l);
         if (warp_live && ok) {
 #pragma unroll 1
           for (int c = 0; c < D; c += 32) {
@@ -626,7 +701,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
           float f0 = ex2_approx(m - shift), f1 = ex2_approx(other.x - shift);
           const float sum = f0 * l + f1 * other.y;
           const RowOut<T, D> dst(a, u, row, live && ok, shift, sum);
-          const float inv = poisoned ? __int_as_float(0x7fffffff) : sum == 0.f ? 0.f : 1.f / sum;
+          const float inv = poisoned ? __int_as_float(0x7fffffff) : sum == 0.f ? 0.f : rcp_approx(sum);
           f0 *= inv;
           f1 *= inv;
           if (warp_live && ok) {
@@ -735,24 +810,36 @@ Plan make_plan(bool within_request, int64_t tile_rows, int64_t batch, int64_t lq
   int64_t met = within_request ? 1 : tile_rows / per_request + (tile_rows % per_request ? 2 : 0);
   if (met > batch) met = batch;
   const int64_t tiles = cdiv(prefix, kTileKeys) + met * cdiv(own, kTileKeys);
-  const double step = tile_rows <= kTileRows ? kHalfStep : 1.0;
-  p.whole = p.items / hold * hold;
-  p.cost = (double)(p.whole / hold) * ((double)tiles * step + kUnitTiles);
-  p.splits = 1;
-  if (const int64_t tail = p.items - p.whole) {
-    // the items that do not fill a last round over the SMs: the number of parts that ends first
-    const int64_t most = tiles / 2 < 1 ? 1 : tiles / 2 < hold ? tiles / 2 : hold;
-    double best = 0.;
-    for (int64_t s = 1; s <= most; ++s) {
-      const double c = (double)cdiv(tail * s, hold) * ((double)cdiv(tiles, s) * step + kUnitTiles) +
-                       (s > 1 ? kJoinTiles + 0.05 * (double)s : 0.);
-      if (s == 1 || c < best) {
-        best = c;
+  const int64_t full = p.groups * (p.row_tiles - 1);  // items before the groups' last row tiles
+  const int64_t last_rows = (within_request ? per_request : p.rows) - (p.row_tiles - 1) * tile_rows;
+  auto step = [](int64_t rows) { return rows <= kTileRows ? kHalfStep : 1.0; };
+  // The units go round the SMs in order, the longest first: the first SM's are the most work.
+  // Every whole round of items is left whole, or all but the last; the rest is split in the
+  // number of parts that ends first.
+  const int64_t most = tiles / 2 < 1 ? 1 : tiles / 2 < hold ? tiles / 2 : hold;
+  const int64_t rounds = p.items / hold;
+  bool any = false;
+  for (int64_t whole = rounds * hold; whole >= 0 && whole >= (rounds - 1) * hold; whole -= hold)
+    for (int64_t s = 1; s <= (whole < p.items ? most : 1); ++s) {
+      const int64_t cut = whole > full ? whole : full;
+      double cost = s > 1 ? kJoinTiles + 0.05 * (double)s : 0.;
+      int64_t at = 0;
+      auto add = [&](int64_t units, double tiles_each, double per_tile) {
+        cost += (double)(cdiv(at + units, hold) - cdiv(at, hold)) * (tiles_each * per_tile + kUnitTiles);
+        at += units;
+      };
+      const int64_t whole_full = whole < full ? whole : full;
+      add(whole_full, (double)tiles, step(tile_rows));
+      add(whole - whole_full, (double)tiles, step(last_rows));
+      add((cut - whole) * s, (double)cdiv(tiles, s), step(tile_rows));
+      add((p.items - cut) * s, (double)cdiv(tiles, s), step(last_rows));
+      if (!any || cost < p.cost) {
+        p.cost = cost;
+        p.whole = whole;
         p.splits = s;
+        any = true;
       }
     }
-    p.cost += best;
-  }
   if (p.splits == 1) p.whole = p.items;
   p.units = p.whole + (p.items - p.whole) * p.splits;
   p.slots = (p.items - p.whole) * p.splits * tile_rows;
@@ -763,7 +850,7 @@ Plan make_plan(bool within_request, int64_t tile_rows, int64_t batch, int64_t lq
 Plan plan_attention(int64_t batch, int64_t lq, int64_t heads, int64_t group, int64_t prefix, int64_t own,
                     int64_t hold) {
   Plan best{};
-  for (int64_t tile_rows : {(int64_t)kUnitRows, (int64_t)kTileRows})
+  for (int64_t tile_rows : {(int64_t)kTileRows, (int64_t)kUnitRows})
     for (bool within : {true, false}) {
       if (!within && batch == 1) continue;
       const Plan p = make_plan(within, tile_rows, batch, lq, heads, group, prefix, own, hold);
