@@ -503,29 +503,39 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         }
         continue;
       }
-      softmax_sync();  // both streams are done with the last unit's Q and O
+      // this row's request, query and head, and how many of the request's own rows it sees
+      const int flat = u.row0 + min(row, u.rows - 1), my_b = flat / per_request;
+      const int in = flat - my_b * per_request, my_i = in / a.group, my_g = in - my_i * a.group;
+      const int visible = a.own > 0 ? own_visible(a, own_len(a, my_b), my_i) : 0;
       {
-        // Q, 16 bytes per step, 128-byte swizzle; rows past the last are zero
-        constexpr int kVecs = D / 8, kStep = kSoftmaxThreads / kVecs;
-        const T* q = reinterpret_cast<const T*>(a.q) + (int64_t)u.h * a.group * a.q_h;
-        const int c = threadIdx.x % kVecs, rows = alternate ? kTileRows : kUnitRows;
-#pragma unroll 4
-        for (int j = threadIdx.x / kVecs; j < rows; j += kStep) {
-          uint4 v = make_uint4(0, 0, 0, 0);
-          if (j < u.rows) {
-            const int flat = u.row0 + j, b = flat / per_request;
-            const int in = flat - b * per_request, i = in / a.group, g = in - i * a.group;
-            v = ld_stream(q + b * a.q_b + i * a.q_t + g * a.q_h + c * 8);
+        // Q: a thread loads its row (of a row that both streams use, one half), 32 bytes at a
+        // time, all of it before the streams meet; 128-byte swizzle; rows past the last are zero
+        constexpr int kVecs = D / 16;
+        const T* q = reinterpret_cast<const T*>(a.q) + my_b * a.q_b + my_i * a.q_t + (int64_t)(u.h * a.group + my_g) * a.q_h;
+        const int first = alternate ? s * (kVecs / 2) : 0, last = alternate ? first + kVecs / 2 : kVecs;
+        uint4 v[kVecs][2];
+#pragma unroll
+        for (int c = 0; c < kVecs; ++c) {
+          v[c][0] = v[c][1] = make_uint4(0, 0, 0, 0);
+          if (live && c >= first && c < last) {
+            v[c][0] = ld_stream(q + c * 16);
+            v[c][1] = ld_stream(q + c * 16 + 8);
           }
-          const uint32_t off = (j / kTileRows) * S::kTile + (c / 8) * kBox + (j % kTileRows) * 128 + (((c & 7) ^ (j & 7)) << 4);
-          *reinterpret_cast<uint4*>(gbase + S::kQ + off) = v;
         }
+        softmax_sync();  // both streams are done with the last unit's Q and O
+        uint8_t* const dst = gbase + S::kQ + (alternate ? 0 : s * S::kTile) + r * 128;
+#pragma unroll
+        for (int c = 0; c < kVecs; ++c)
+          if (c >= first && c < last) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const int g = 2 * c + e;  // 16-byte vector of the row
+              *reinterpret_cast<uint4*>(dst + (g / 8) * kBox + (((g ^ r) & 7) << 4)) = v[c][e];
+            }
+          }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         arrive_warp(q_full);
       }
-      // this row's request and how many of its own rows it sees
-      const int flat = u.row0 + min(row, u.rows - 1), my_b = flat / per_request;
-      const int visible = a.own > 0 ? own_visible(a, own_len(a, my_b), (flat - my_b * per_request) / a.group) : 0;
       const bool warp_live = (alternate ? 0 : s * kTileRows) + ((warp & 3) << 5) < u.rows;
       const int steps = alternate ? (n + 1 - s) / 2 : n;
       // of a unit within one request: own rows that all of its rows see
@@ -735,20 +745,23 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
   }
 }
 
-// Joins the parts of each row of the split units by their log2-sum-exps: one warp per row.
+// Joins the parts of each row of the split units by their log2-sum-exps.  One CTA per row,
+// its warps taking every fourth part, so that a row of many parts (single tokens: as many as
+// fill the GPU) costs a few loads in a row and not one per part; the warps' sums are added in
+// their order.
+constexpr int kJoinWarps = 4;
 template <typename T, int D>
-__global__ void __launch_bounds__(256) prefix_attn_join_kernel(const AttnArgs a, int64_t total) {
+__global__ void __launch_bounds__(32 * kJoinWarps) prefix_attn_join_kernel(const AttnArgs a) {
   constexpr int E = D / 32;
-  const int lane = threadIdx.x & 31;
-  const int64_t w = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  pdl_wait();
-  pdl_trigger();
-  if (w >= total) return;
+  __shared__ float sums[kJoinWarps][D + 1];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int per_request = a.lq * a.group;
-  const int j = (int)(w / a.tile_rows), r = (int)(w - (int64_t)j * a.tile_rows);
+  const int j = (int)(blockIdx.x / (unsigned)a.tile_rows), r = (int)(blockIdx.x - (unsigned)j * a.tile_rows);
   int grp, t;
   tile_of(a, a.whole + j, grp, t);
   const int h = a.within_request ? grp / a.batch : grp, b0 = a.within_request ? grp - h * a.batch : 0;
+  pdl_wait();
+  pdl_trigger();
   if (t * a.tile_rows + r >= (a.within_request ? per_request : a.rows)) return;
   const int row = b0 * per_request + t * a.tile_rows + r, all = a.splits;
   const int64_t slot0 = (int64_t)j * all * a.tile_rows + r;
@@ -759,7 +772,7 @@ __global__ void __launch_bounds__(256) prefix_attn_join_kernel(const AttnArgs a,
   const float shift = top == -INFINITY ? 0.f : top;
   float o[E] = {}, sum = 0.f;
 #pragma unroll 4
-  for (int s = 0; s < all; ++s) {
+  for (int s = warp; s < all; s += kJoinWarps) {
     const int64_t slot = slot_of(s);
     const float wgt = ex2_approx(a.part_lse[slot] - shift);
     const float* p = a.part_o + slot * D + lane * E;
@@ -771,6 +784,17 @@ __global__ void __launch_bounds__(256) prefix_attn_join_kernel(const AttnArgs a,
       const float2 v = *reinterpret_cast<const float2*>(p);
       o[0] = fmaf(wgt, v.x, o[0]), o[1] = fmaf(wgt, v.y, o[1]);
     }
+  }
+#pragma unroll
+  for (int e = 0; e < E; ++e) sums[warp][lane * E + e] = o[e];
+  if (lane == 0) sums[warp][D] = sum;
+  __syncthreads();
+  if (warp != 0) return;
+#pragma unroll
+  for (int w = 1; w < kJoinWarps; ++w) {
+    sum += sums[w][D];
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] += sums[w][lane * E + e];
   }
   const int64_t hq = (int64_t)a.heads * a.group;
   const int b = row / per_request, in = row - b * per_request, i = in / a.group, g = in - i * a.group;
@@ -902,8 +926,7 @@ int launch_attention(const CUtensorMap* maps, const AttnArgs& a, const Plan& p, 
     return launch_failed(e, op);
   if (int s = after_launch("prefix_attn_kernel")) return s;
   if (const int64_t joined = (p.items - p.whole) * p.tile_rows) {
-    if (cudaError_t e = launch_pdl(prefix_attn_join_kernel<T, D>, dim3((unsigned)cdiv(joined, 8)), dim3(256), 0, st, a,
-                                   joined))
+    if (cudaError_t e = launch_pdl(prefix_attn_join_kernel<T, D>, dim3((unsigned)joined), dim3(32 * kJoinWarps), 0, st, a))
       return launch_failed(e, op);
     return after_launch("prefix_attn_join_kernel");
   }
@@ -960,7 +983,7 @@ int jo_shared_prefix_attention(void* out, float* lse, const void* q, int64_t q_s
     if (u.size > 1 && (u.stride % 8 || u.stride < 0))
       return fail(JO_ERR_ALIGN, "%s: strides must be multiples of 16 bytes and not negative", op);
   const Plan p = plan_attention(batch, q_len, kv_heads, q_heads / kv_heads, prefix_len, own_len, di->sm_count);
-  if (p.units > INT32_MAX / 2) return fail(JO_ERR_SHAPE, "%s: size too large", op);
+  if (p.units > INT32_MAX / 2 || (p.items - p.whole) * p.tile_rows > INT32_MAX) return fail(JO_ERR_SHAPE, "%s: size too large", op);
   if (p.slots && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 31) || workspace_bytes < p.slots * (head_dim + 1) * 4))
     return fail(JO_ERR_INVALID, "%s: a 32-byte aligned workspace of %lld bytes is needed", op,
                 (long long)(p.slots * (head_dim + 1) * 4));
