@@ -95,8 +95,18 @@ struct Run {
   }
 };
 
-__device__ __forceinline__ uint32_t e2m1x2(float2 v) {  // v.x in the low half of the byte
-  return (uint32_t)__nv_cvt_float2_to_fp4x2(v, __NV_E2M1, cudaRoundNearest);
+// Eight codes, p[0].x lowest.
+__device__ __forceinline__ uint32_t e2m1x8(const float2 (&p)[4]) {
+  uint32_t r;
+  asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b1, %4, %3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b2, %6, %5;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b3, %8, %7;\n\t"
+      "mov.b32 %0, {b0, b1, b2, b3};\n\t}"
+      : "=r"(r)
+      : "f"(p[0].x), "f"(p[0].y), "f"(p[1].x), "f"(p[1].y), "f"(p[2].x), "f"(p[2].y), "f"(p[3].x), "f"(p[3].y));
+  return r;
 }
 
 // 16 codes of a run of a block with scale step d: e2m1 of the correctly rounded
@@ -104,18 +114,26 @@ __device__ __forceinline__ uint32_t e2m1x2(float2 v) {  // v.x in the low half o
 template <typename T>
 __device__ __forceinline__ uint2 codes_of(const Run<T>& r, float d) {
   const float2 nd = f2(-d), rc = f2(__frcp_rn(d));
-  uint32_t c[2] = {0, 0};
+  float2 q[2][4];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) c[i / 4] |= e2m1x2(div2_ms(r.pair(i), nd, rc)) << (8 * (i % 4));
-  return make_uint2(c[0], c[1]);
+  for (int i = 0; i < 8; ++i) q[i / 4][i % 4] = div2_ms(r.pair(i), nd, rc);
+  return make_uint2(e2m1x8(q[0]), e2m1x8(q[1]));
 }
 // The same for a power-of-two step, whose reciprocal is exact.
 template <typename T>
 __device__ __forceinline__ uint2 codes_of_pow2(const Run<T>& r, float inv) {
-  uint32_t c[2] = {0, 0};
+  float2 q[2][4];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) c[i / 4] |= e2m1x2(__fmul2_rn(r.pair(i), f2(inv))) << (8 * (i % 4));
-  return make_uint2(c[0], c[1]);
+  for (int i = 0; i < 8; ++i) q[i / 4][i % 4] = __fmul2_rn(r.pair(i), f2(inv));
+  return make_uint2(e2m1x8(q[0]), e2m1x8(q[1]));
+}
+
+// Correctly rounded x / s from RN(1/s), as div2_ms (quant.cuh): where x / s is too small for
+// the steps to be exact, e4m3 rounds it to zero anyway.
+constexpr float kSixth = 0.16666667f;  // RN(1/6)
+__device__ __forceinline__ float quotient(float x, float s, float rc) {
+  const float q = __fmul_rn(x, rc);
+  return __fmaf_rn(__fmaf_rn(-s, q, x), rc, q);
 }
 
 struct QuantArgs {
@@ -165,7 +183,7 @@ __global__ void __launch_bounds__(kMaxThreads) quant_fp4_kernel(const QuantArgs 
     else
       all = max(all, top[j]);
   }
-  float rs = 0.f;
+  float rs = 0.f, rc_rs = 0.f;
   bool bad_row = false;
   if constexpr (!kMx) {
     all = __reduce_max_sync(0xffffffffu, all);
@@ -176,6 +194,7 @@ __global__ void __launch_bounds__(kMaxThreads) quant_fp4_kernel(const QuantArgs 
     }
     bad_row = all >= 0x7f800000u;
     rs = __fdiv_rn(fmaxf(__uint_as_float(all), 1e-8f), 6.f * kFp8Max);
+    rc_rs = __frcp_rn(rs);
     if (live && w == 0 && lane == 0) a.rs[m] = bad_row ? __int_as_float(0x7fffffff) : rs;
   }
   if (m >= a.rows_padded) return;
@@ -195,7 +214,7 @@ __global__ void __launch_bounds__(kMaxThreads) quant_fp4_kernel(const QuantArgs 
           c = codes_of_pow2(run[j], __uint_as_float((254u - code) << 23));  // 2^-(code - 127)
         }
       } else if (!bad_row) {
-        const float t = __fdiv_rn(__fdiv_rn(__uint_as_float(top[j]), rs), 6.f);
+        const float t = quotient(quotient(__uint_as_float(top[j]), rs, rc_rs), 6.f, kSixth);
         code = (uint32_t)__nv_cvt_float_to_fp8(t, __NV_SATFINITE, __NV_E4M3);
         if (code) c = codes_of(run[j], __fmul_rn(fp4_scale_value<false>((uint8_t)code), rs));
       }
@@ -220,42 +239,65 @@ struct DequantArgs {
   const float* rs;
   int64_t total;  // runs
   int runs, tiles_k;
-  int vec;  // elements per store
+  int align;  // of every run's address in the output
 };
 
-// Store 16 floats as T, `vec` elements at a time.
+// Store 16 floats as T.
 template <typename T>
-__device__ __forceinline__ void store16(T* p, const float* f, int vec) {
-  if (vec == Elt<T>::kVec) {
+__device__ __forceinline__ void store16(T* p, const float* f, int align) {
+  constexpr int V = Elt<T>::kVec;
+  if (align == 32) {
 #pragma unroll
-    for (int i = 0; i < 16; i += Elt<T>::kVec) st_global(p + i, Elt<T>::pack(f + i));
+    for (int i = 0; i < 16; i += 2 * V) st_global32(p + i, Elt<T>::pack(f + i), Elt<T>::pack(f + i + V));
+  } else if (align == 16) {
+#pragma unroll
+    for (int i = 0; i < 16; i += V) st_global(p + i, Elt<T>::pack(f + i));
   } else {
 #pragma unroll
     for (int i = 0; i < 16; ++i) p[i] = Elt<T>::from_f(f[i]);
   }
 }
 
+// kDeqRuns runs per thread, their loads before the first conversion; a CTA's runs are
+// consecutive, so the row of each follows from the CTA's first by a 32-bit division.
+constexpr int kDeqRuns = 4;
+
 template <typename T, bool kMx>
 __global__ void __launch_bounds__(kQuantThreads) dequant_fp4_kernel(const DequantArgs a) {
+  const int64_t base = (int64_t)blockIdx.x * (kQuantThreads * kDeqRuns);
+  const int64_t m0 = base / a.runs;
+  const uint32_t u0 = (uint32_t)(base - m0 * a.runs) + threadIdx.x;
   pdl_wait();
   pdl_trigger();
-  for (int64_t i = (int64_t)blockIdx.x * kQuantThreads + threadIdx.x; i < a.total;
-       i += (int64_t)gridDim.x * kQuantThreads) {
-    const int64_t m = i / a.runs;
-    const int u = (int)(i - m * a.runs);
-    const uint2 c = __ldg(reinterpret_cast<const uint2*>(a.q + m * a.ldq + (int64_t)u * 8));
-    const float s = fp4_scale_value<kMx>(__ldg(a.bs + fp4_scale_offset(m, kMx ? u >> 1 : u, a.tiles_k)));
-    const float r = kMx ? 1.f : __ldg(a.rs + m);
-    const uint32_t w[2] = {c.x, c.y};
+  uint2 code[kDeqRuns];
+  uint8_t scale[kDeqRuns];
+  float row[kDeqRuns];
+#pragma unroll
+  for (int i = 0; i < kDeqRuns; ++i) {
+    const uint32_t at = u0 + i * kQuantThreads, over = at / (uint32_t)a.runs, u = at - over * a.runs;
+    const int64_t m = m0 + over;
+    if (base + threadIdx.x + i * kQuantThreads >= a.total) break;
+    code[i] = __ldg(reinterpret_cast<const uint2*>(a.q + m * a.ldq + (int64_t)u * 8));
+    scale[i] = __ldg(a.bs + fp4_scale_offset(m, kMx ? u >> 1 : u, a.tiles_k));
+    row[i] = kMx ? 1.f : __ldg(a.rs + m);
+  }
+#pragma unroll
+  for (int i = 0; i < kDeqRuns; ++i) {
+    const uint32_t at = u0 + i * kQuantThreads, over = at / (uint32_t)a.runs, u = at - over * a.runs;
+    const int64_t m = m0 + over;
+    if (base + threadIdx.x + i * kQuantThreads >= a.total) break;
+    const float s = fp4_scale_value<kMx>(scale[i]);
+    const uint32_t w[2] = {code[i].x, code[i].y};
     float f[16];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const __half2_raw h = __nv_cvt_fp4x2_to_halfraw2((__nv_fp4x2_storage_t)((w[j / 4] >> (8 * (j % 4))) & 0xffu), __NV_E2M1);
+      const __half2_raw h =
+          __nv_cvt_fp4x2_to_halfraw2((__nv_fp4x2_storage_t)((w[j / 4] >> (8 * (j % 4))) & 0xffu), __NV_E2M1);
       const float2 v = __half22float2(__half2(h));
-      f[2 * j] = kMx ? v.x * s : __fmul_rn(v.x * s, r);  // code * s is exact
-      f[2 * j + 1] = kMx ? v.y * s : __fmul_rn(v.y * s, r);
+      f[2 * j] = kMx ? v.x * s : __fmul_rn(v.x * s, row[i]);  // code * s is exact
+      f[2 * j + 1] = kMx ? v.y * s : __fmul_rn(v.y * s, row[i]);
     }
-    store16(reinterpret_cast<T*>(a.out) + m * a.ldo + (int64_t)u * 16, f, a.vec);
+    store16(reinterpret_cast<T*>(a.out) + m * a.ldo + (int64_t)u * 16, f, a.align);
   }
 }
 
@@ -272,14 +314,20 @@ int launch_quant(const QuantArgs& a, cudaStream_t st) {
 
 template <typename T, bool kMx>
 int dispatch_quant(QuantArgs a, const DeviceInfo* di, cudaStream_t st) {
-  // A row's runs in warps-full: as few warps per row as still give every SM 32
-  // warps, each lane with up to 6 runs in flight (fp32: 4).
+  // One run per lane while that does not give every SM 32 warps (latency counts), else the
+  // fewest runs per lane with at most 8 warps per row: small CTAs overlap one's loads with
+  // another's arithmetic.  Measured, bf16: 10800 x 3072 with 1 / 2 / 4 / 6 runs 21.4 / 18.8 /
+  // 18.8 / 20.1 us, 10800 x 12288 101 / 77 / 65 / 65, 1350 x 3072 3.8 / 4.1 / 4.7 / 4.8.
   const int full = (int)cdiv(a.runs, 32);
   constexpr int kMost = sizeof(T) == 4 ? 4 : 6;
   int runs = 1;
-  for (int r : {2, 4, 6})
-    if (r <= kMost && (a.rows * cdiv(full, r) >= (int64_t)32 * di->sm_count || cdiv(full, runs) > 32)) runs = r;
-  if (runs > full) runs = full <= 1 ? 1 : full <= 2 ? 2 : full <= 4 ? 4 : 6;
+  if (a.rows * full >= (int64_t)64 * di->sm_count || full > 32)
+    for (int r : {2, 4, 6}) {
+      if (r > kMost) break;
+      runs = r;
+      if (cdiv(full, r) <= 8) break;
+    }
+  if (runs > full) runs = full;
   a.warps = (int)cdiv(full, runs);
   if (a.warps > 32) return fail(JO_ERR_SHAPE, "quant_fp4: rows of at most %d elements", 32 * 32 * 16 * kMost);
   switch (runs) {
@@ -376,11 +424,11 @@ int jo_dequant_fp4(void* out, int64_t out_row_stride, const void* q, int64_t q_r
   a.total = rows * a.runs;
   const uint64_t at = reinterpret_cast<uintptr_t>(out) | (uint64_t)(rows > 1 ? out_row_stride * esize : 0);
   if (at % esize) return fail(JO_ERR_ALIGN, "%s: out must be aligned to its elements", op);
-  a.vec = at % 16 == 0 ? (int)(16 / esize) : 1;
+  a.align = at % 32 == 0 ? 32 : at % 16 == 0 ? 16 : (int)esize;
   auto launch = [&](auto kern) -> int {
-    const int64_t cap = (int64_t)di->sm_count * occupancy((const void*)kern, kQuantThreads, 0);
-    const int64_t need = cdiv(a.total, kQuantThreads);
-    if (cudaError_t e = launch_pdl(kern, dim3((unsigned)(need < cap ? need : cap)), dim3(kQuantThreads), 0,
+    const int64_t need = cdiv(a.total, kQuantThreads * kDeqRuns);
+    if (need > INT32_MAX) return fail(JO_ERR_SHAPE, "%s: size too large", op);
+    if (cudaError_t e = launch_pdl(kern, dim3((unsigned)need), dim3(kQuantThreads), 0,
                                    (cudaStream_t)stream, a))
       return launch_failed(e, op);
     return after_launch("dequant_fp4_kernel");

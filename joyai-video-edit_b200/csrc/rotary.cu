@@ -61,29 +61,31 @@ __device__ __forceinline__ uint4 ld_once(const void* p) {
 }
 
 // V = 1: one element (or pair) per place, for strides, addresses or R that no
-// 16-byte vector fits; otherwise V = the 16-byte vector's elements.
+// 16-byte vector fits; otherwise V = the 16-byte vector's elements, kept as they lie in
+// memory until they are rotated.
 template <typename T, int V>
 struct Chunk {
-  float f[V];
-  __device__ __forceinline__ void load(const T* p) {
-    if constexpr (V == 1)
-      f[0] = Elt<T>::to_f(*p);
-    else
-      Elt<T>::unpack(ld_once(p), f);
-  }
-  __device__ __forceinline__ void store(T* p) const {
-    if constexpr (V == 1)
-      *p = Elt<T>::from_f(f[0]);
-    else
-      st_global(p, Elt<T>::pack(f));
-  }
+  uint4 w;
+  __device__ __forceinline__ void load(const T* p) { w = ld_once(p); }
+  __device__ __forceinline__ void store(T* p) const { st_global(p, w); }
+  __device__ __forceinline__ void unpack(float* f) const { Elt<T>::unpack(w, f); }
+  __device__ __forceinline__ void pack(const float* f) { w = Elt<T>::pack(f); }
+};
+template <typename T>
+struct Chunk<T, 1> {
+  T w;
+  __device__ __forceinline__ void load(const T* p) { w = *p; }
+  __device__ __forceinline__ void store(T* p) const { *p = w; }
+  __device__ __forceinline__ void unpack(float* f) const { f[0] = Elt<T>::to_f(w); }
+  __device__ __forceinline__ void pack(const float* f) { w = Elt<T>::from_f(f[0]); }
 };
 
 template <typename T, int V, bool kInterleaved>
-__global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryArgs a) {
+__global__ void __launch_bounds__(kThreads, 4) rotary_kernel(const RotaryArgs a) {
   // the interleaved scalar form moves a pair of elements per place
   constexpr bool kPair = V == 1 && kInterleaved;
   constexpr int kTab = kInterleaved ? (V == 1 ? 1 : V / 2) : V;  // table entries per place
+  constexpr int kBatch = kInterleaved ? 4 : 2;  // heads under way (half layout: two loads each)
   const int groups = kThreads / a.items;
   const int place = threadIdx.x % a.items, group = threadIdx.x / a.items;
   const int half = a.rot_dim / 2;
@@ -106,89 +108,87 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryArgs a) {
   pdl_trigger();
   if (group >= groups) return;
   for (int64_t t = blockIdx.x; t < a.tokens; t += gridDim.x) {
+    const int64_t pos = tab >= 0 ? index_at(a.positions, t, a.wide) : 0;
+    const int64_t row = a.slots != nullptr ? index_at(a.slots, t, a.wide) : t;
+    const bool keep = a.slots == nullptr || (row >= 0 && row < a.cache_rows);
     float c[kTab], s[kTab];
-    if (tab >= 0) {
-      const int64_t pos = index_at(a.positions, t, a.wide);
-      const bool ok = pos >= 0 && pos < a.table_rows;  // a position outside the tables: not read, NaN
-      const float* cr = a.cos + (ok ? pos : 0) * half + tab;
-      const float* sr = a.sin + (ok ? pos : 0) * half + tab;
-      if constexpr (kTab >= 4) {
+    // kBatch heads' loads before the first store (the output may be the input, so the compiler
+    // would keep each load behind the stores before it) and before the table row, whose
+    // address waits for the position
+    for (int h0 = group; h0 < heads; h0 += kBatch * groups) {
+      Chunk<T, V> x[kBatch], y[kBatch];
 #pragma unroll
-        for (int j = 0; j < kTab; j += 4) {
-          const float4 cv = ok ? __ldg(reinterpret_cast<const float4*>(cr + j)) : make_float4(0, 0, 0, 0);
-          const float4 sv = ok ? __ldg(reinterpret_cast<const float4*>(sr + j)) : make_float4(0, 0, 0, 0);
-          c[j] = cv.x, c[j + 1] = cv.y, c[j + 2] = cv.z, c[j + 3] = cv.w;
-          s[j] = sv.x, s[j + 1] = sv.y, s[j + 2] = sv.z, s[j + 3] = sv.w;
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < kTab; ++j) c[j] = ok ? __ldg(cr + j) : 0.f, s[j] = ok ? __ldg(sr + j) : 0.f;
+      for (int i = 0; i < kBatch; ++i) {
+        const int h = h0 + i * groups;
+        if (h >= heads) break;
+        const T* in = h < a.q_heads ? reinterpret_cast<const T*>(a.q.p) + t * a.q.st + h * a.q.sh
+                      : h < a.q_heads + a.k_heads
+                          ? reinterpret_cast<const T*>(a.k.p) + t * a.k.st + (h - a.q_heads) * a.k.sh
+                          : reinterpret_cast<const T*>(a.v.p) + t * a.v.st + (h - a.q_heads - a.k_heads) * a.v.sh;
+        x[i].load(in + e0);
+        if constexpr (kPair)
+          y[i].load(in + e0 + 1);
+        else if (!kInterleaved && e1 >= 0)
+          y[i].load(in + e1);
       }
+      if (tab >= 0 && h0 == group) {
+        const bool ok = pos >= 0 && pos < a.table_rows;  // a position outside the tables: not read, NaN
+        const float* cr = a.cos + (ok ? pos : 0) * half + tab;
+        const float* sr = a.sin + (ok ? pos : 0) * half + tab;
+        if constexpr (kTab >= 4) {
 #pragma unroll
-      for (int j = 0; j < kTab; ++j) {
-        c[j] = ok ? c[j] : __int_as_float(0x7fffffff);
-        s[j] *= a.sign;
-      }
-    }
-    int64_t row = t;
-    bool keep = true;
-    if (a.slots != nullptr) {
-      row = index_at(a.slots, t, a.wide);
-      keep = row >= 0 && row < a.cache_rows;
-    }
-#pragma unroll 3
-    for (int h = group; h < heads; h += groups) {
-      const T* in;
-      T* out;
-      bool rotate = tab >= 0, write = true;
-      if (h < a.q_heads) {
-        in = reinterpret_cast<const T*>(a.q.p) + t * a.q.st + h * a.q.sh;
-        out = reinterpret_cast<T*>(a.q_out.p) + t * a.q_out.st + h * a.q_out.sh;
-      } else if (h < a.q_heads + a.k_heads) {
-        const int hk = h - a.q_heads;
-        in = reinterpret_cast<const T*>(a.k.p) + t * a.k.st + hk * a.k.sh;
-        out = reinterpret_cast<T*>(a.k_out.p) + row * a.k_out.st + hk * a.k_out.sh;
-        write = keep;
-      } else {
-        const int hv = h - a.q_heads - a.k_heads;
-        in = reinterpret_cast<const T*>(a.v.p) + t * a.v.st + hv * a.v.sh;
-        out = reinterpret_cast<T*>(a.v_out.p) + row * a.v_out.st + hv * a.v_out.sh;
-        rotate = false;
-        write = keep;
-      }
-      if (!write) continue;
-      Chunk<T, V> x, y;
-      x.load(in + e0);
-      if constexpr (kPair) {
-        y.load(in + e0 + 1);
-        if (rotate) {
-          const float u = x.f[0], w = y.f[0];
-          x.f[0] = u * c[0] - w * s[0];
-          y.f[0] = u * s[0] + w * c[0];
-        }
-        y.store(out + e0 + 1);
-      } else if constexpr (kInterleaved) {
-        if (rotate) {
-#pragma unroll
-          for (int j = 0; j < V / 2; ++j) {
-            const float u = x.f[2 * j], w = x.f[2 * j + 1];
-            x.f[2 * j] = u * c[j] - w * s[j];
-            x.f[2 * j + 1] = u * s[j] + w * c[j];
+          for (int j = 0; j < kTab; j += 4) {
+            const float4 cv = __ldg(reinterpret_cast<const float4*>(cr + j));
+            const float4 sv = __ldg(reinterpret_cast<const float4*>(sr + j));
+            c[j] = cv.x, c[j + 1] = cv.y, c[j + 2] = cv.z, c[j + 3] = cv.w;
+            s[j] = sv.x, s[j + 1] = sv.y, s[j + 2] = sv.z, s[j + 3] = sv.w;
           }
-        }
-      } else if (e1 >= 0) {
-        y.load(in + e1);
-        if (rotate) {
+        } else {
 #pragma unroll
-          for (int j = 0; j < V; ++j) {
-            const float u = x.f[j], w = y.f[j];
-            x.f[j] = u * c[j] - w * s[j];
-            y.f[j] = u * s[j] + w * c[j];
-          }
+          for (int j = 0; j < kTab; ++j) c[j] = __ldg(cr + j), s[j] = __ldg(sr + j);
         }
-        y.store(out + e1);
+#pragma unroll
+        for (int j = 0; j < kTab; ++j) {
+          c[j] = ok ? c[j] : __int_as_float(0x7fffffff);
+          s[j] *= a.sign;
+        }
       }
-      x.store(out + e0);
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        const int h = h0 + i * groups;
+        if (h >= heads || (h >= a.q_heads && !keep)) break;
+        if (tab >= 0 && h < a.q_heads + a.k_heads) {
+          float u[V], w[V];
+          x[i].unpack(u);
+          if constexpr (kInterleaved && !kPair) {
+#pragma unroll
+            for (int j = 0; j < V / 2; ++j) {
+              const float p = u[2 * j], q = u[2 * j + 1];
+              u[2 * j] = p * c[j] - q * s[j];
+              u[2 * j + 1] = p * s[j] + q * c[j];
+            }
+          } else {
+            y[i].unpack(w);
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+              const float p = u[j], q = w[j];
+              u[j] = p * c[j] - q * s[j];
+              w[j] = p * s[j] + q * c[j];
+            }
+            y[i].pack(w);
+          }
+          x[i].pack(u);
+        }
+        T* out = h < a.q_heads ? reinterpret_cast<T*>(a.q_out.p) + t * a.q_out.st + h * a.q_out.sh
+                 : h < a.q_heads + a.k_heads
+                     ? reinterpret_cast<T*>(a.k_out.p) + row * a.k_out.st + (h - a.q_heads) * a.k_out.sh
+                     : reinterpret_cast<T*>(a.v_out.p) + row * a.v_out.st + (h - a.q_heads - a.k_heads) * a.v_out.sh;
+        x[i].store(out + e0);
+        if constexpr (kPair)
+          y[i].store(out + e0 + 1);
+        else if (!kInterleaved && e1 >= 0)
+          y[i].store(out + e1);
+      }
     }
   }
 }
