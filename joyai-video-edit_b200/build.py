@@ -104,7 +104,7 @@ def build_shim(jobs: int = 8) -> Path:
     with cf.ThreadPoolExecutor(max_workers=jobs) as ex:
         list(ex.map(_run, todo))
     _run(["g++", "-shared", *map(str, objs), "-o", str(SHIM), *[f"-L{p}" for p in libdirs], f"-L{OUT}",
-          "-ljoyomni_b200", "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-Wl,-rpath,$ORIGIN"])
+          "-ljoyomni_b200", "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-Wl,-rpath,$ORIGIN"])
     return SHIM
 
 

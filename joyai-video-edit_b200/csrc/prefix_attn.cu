@@ -844,7 +844,10 @@ Plan make_plan(bool within_request, int64_t tile_rows, int64_t batch, int64_t lq
   const int64_t rounds = p.items / hold;
   bool any = false;
   for (int64_t whole = rounds * hold; whole >= 0 && whole >= (rounds - 1) * hold; whole -= hold)
-    for (int64_t s = 1; s <= (whole < p.items ? most : 1); ++s) {
+    for (int trial = 1; trial <= 19; ++trial) {
+      // up to 16 parts, and the numbers that fill one, two and three rounds
+      const int64_t s = trial <= 16 ? trial : whole < p.items ? (trial - 16) * hold / (p.items - whole) : 1;
+      if (s > most || s < 1 || (s > 1 && whole == p.items)) continue;
       const int64_t cut = whole > full ? whole : full;
       double cost = s > 1 ? kJoinTiles + 0.05 * (double)s : 0.;
       int64_t at = 0;

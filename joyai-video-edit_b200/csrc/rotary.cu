@@ -22,6 +22,7 @@ namespace jo {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kResident = 4;  // CTAs per SM
 
 // One tensor of heads: element (t, h, d) at p[t*st + h*sh + d].
 template <typename P>
@@ -81,7 +82,7 @@ struct Chunk<T, 1> {
 };
 
 template <typename T, int V, bool kInterleaved>
-__global__ void __launch_bounds__(kThreads, 4) rotary_kernel(const RotaryArgs a) {
+__global__ void __launch_bounds__(kThreads, kResident) rotary_kernel(const RotaryArgs a) {
   // the interleaved scalar form moves a pair of elements per place
   constexpr bool kPair = V == 1 && kInterleaved;
   constexpr int kTab = kInterleaved ? (V == 1 ? 1 : V / 2) : V;  // table entries per place
@@ -196,7 +197,7 @@ __global__ void __launch_bounds__(kThreads, 4) rotary_kernel(const RotaryArgs a)
 template <typename T, int V>
 int launch(const RotaryArgs& a, bool interleaved, const DeviceInfo* di, cudaStream_t st, const char* op) {
   auto kern = interleaved ? rotary_kernel<T, V, true> : rotary_kernel<T, V, false>;
-  const int64_t cap = (int64_t)di->sm_count * occupancy((const void*)kern, kThreads, 0);
+  const int64_t cap = (int64_t)di->sm_count * kResident;
   const int64_t grid = a.tokens < cap ? a.tokens : cap;
   if (cudaError_t e = launch_pdl(kern, dim3((unsigned)grid), dim3(kThreads), 0, st, a)) return launch_failed(e, op);
   return after_launch("rotary_kernel");

@@ -1,9 +1,17 @@
 // torch.ops.joyomni_ops.* of the attention layer of a batch that shares a long prefix:
 // matrices in 4 bits and their product, the rotary embedding, and attention over the
 // shared prefix and each request's own rows.
+#include <ATen/cuda/EmptyTensor.h>
+
 #include "torch_shim.h"
 
 namespace {
+
+// An uninitialised tensor on `like`'s device, without a trip through the dispatcher (the
+// smallest calls are bound by the host).
+torch::Tensor new_empty(at::IntArrayRef sizes, at::ScalarType dtype, const torch::Tensor& like) {
+  return at::detail::empty_cuda(sizes, dtype, like.device(), c10::nullopt);
+}
 
 // ------------------------------------------------------------------ 4 bits
 int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
@@ -44,9 +52,9 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> quant_fp4(const torch::T
   const int64_t M = x.size(0), K = x.size(1);
   TORCH_CHECK(K > 0 && K % 32 == 0, "K must be a positive multiple of 32");
   const c10::cuda::CUDAGuard guard(x.device());
-  auto q = torch::empty({M, K / 2}, x.options().dtype(at::kByte));
-  auto block = torch::empty(scale_shape(M, K, (int)format), x.options().dtype(scale_type((int)format)));
-  auto row = torch::empty({format == JO_FP4_NV ? M : 0, 1}, x.options().dtype(at::kFloat));
+  auto q = new_empty({M, K / 2}, at::kByte, x);
+  auto block = new_empty(scale_shape(M, K, (int)format), scale_type((int)format), x);
+  auto row = new_empty({format == JO_FP4_NV ? M : 0, 1}, at::kFloat, x);
   jo_check(jo_quant_fp4(q.data_ptr(), K / 2, block.data_ptr(), row.numel() ? row.data_ptr<float>() : nullptr,
                         x.data_ptr(), x.stride(0), M, K, (int)format, dt_code(x.scalar_type()), stream_of(x)),
            "quant_fp4");
@@ -59,31 +67,21 @@ torch::Tensor dequant_fp4(const torch::Tensor& q, const torch::Tensor& block, co
   const int format = check_fp4(q, block, row, q, "q");
   const int64_t M = q.size(0), K = 2 * q.size(1);
   const c10::cuda::CUDAGuard guard(q.device());
-  auto out = torch::empty({M, K}, q.options().dtype(dtype));
+  auto out = new_empty({M, K}, dtype, q);
   jo_check(jo_dequant_fp4(out.data_ptr(), K, q.data_ptr(), q.stride(0), block.data_ptr(),
                           (const float*)opt_ptr(row), M, K, format, dt_code(dtype), stream_of(q)),
            "dequant_fp4");
   return out;
 }
 
-torch::Tensor fp4_mm(const torch::Tensor& a, const torch::Tensor& b, const torch::Tensor& block_a,
-                     const torch::Tensor& block_b, const c10::optional<torch::Tensor>& scales_a,
-                     const c10::optional<torch::Tensor>& scales_b, at::ScalarType out_dtype,
-                     const c10::optional<torch::Tensor>& bias, int format) {
-  const int64_t M = a.size(0), N = b.size(0), K = 2 * a.size(1);
+void check_product(const torch::Tensor& a, int64_t n, at::ScalarType out_dtype,
+                   const c10::optional<torch::Tensor>& bias) {
   TORCH_CHECK(out_dtype == at::kHalf || out_dtype == at::kBFloat16, "out_dtype must be Half or BFloat16");
-  TORCH_CHECK(N % 8 == 0, "the number of mat_b's rows must be a multiple of 8");
+  TORCH_CHECK(n % 8 == 0, "the number of mat_b's rows must be a multiple of 8");
   check_dev(bias, a, "bias");
   if (bias.has_value() && bias->defined())
-    TORCH_CHECK(bias->numel() == N && bias->is_contiguous() && bias->scalar_type() == out_dtype,
+    TORCH_CHECK(bias->numel() == n && bias->is_contiguous() && bias->scalar_type() == out_dtype,
                 "bias must be contiguous [N] of the output dtype");
-  auto out = torch::empty({M, N}, a.options().dtype(out_dtype));
-  jo_check(jo_fp4_scaled_mm(out.data_ptr(), N, a.data_ptr(), a.stride(0), b.data_ptr(), b.stride(0),
-                            block_a.data_ptr(), block_b.data_ptr(), (const float*)opt_ptr(scales_a),
-                            (const float*)opt_ptr(scales_b), opt_ptr(bias), M, N, K, format, dt_code(out_dtype),
-                            stream_of(a)),
-           "fp4_scaled_mm");
-  return out;
 }
 
 torch::Tensor fp4_scaled_mm(const torch::Tensor& mat_a, const torch::Tensor& mat_b, const torch::Tensor& block_a,
@@ -95,22 +93,43 @@ torch::Tensor fp4_scaled_mm(const torch::Tensor& mat_a, const torch::Tensor& mat
   TORCH_CHECK(check_fp4(mat_b, block_b, scales_b, mat_a, "mat_b") == format,
               "mat_a and mat_b must have one 4-bit format");
   TORCH_CHECK(mat_a.size(1) == mat_b.size(1), "mat_a and mat_b shapes cannot be multiplied");
+  const int64_t M = mat_a.size(0), N = mat_b.size(0);
+  check_product(mat_a, N, out_dtype, bias);
   const c10::cuda::CUDAGuard guard(mat_a.device());
-  return fp4_mm(mat_a, mat_b, block_a, block_b, scales_a, scales_b, out_dtype, bias, format);
+  auto out = new_empty({M, N}, out_dtype, mat_a);
+  jo_check(jo_fp4_scaled_mm(out.data_ptr(), N, mat_a.data_ptr(), mat_a.stride(0), mat_b.data_ptr(), mat_b.stride(0),
+                            block_a.data_ptr(), block_b.data_ptr(), (const float*)opt_ptr(scales_a),
+                            (const float*)opt_ptr(scales_b), opt_ptr(bias), M, N, 2 * mat_a.size(1), format,
+                            dt_code(out_dtype), stream_of(mat_a)),
+           "fp4_scaled_mm");
+  return out;
 }
 
-// quant_fp4 of x in mat_b's format, then the product: a Linear layer in 4 bits.
+// quant_fp4 of x in mat_b's format, then the product: a Linear layer in 4 bits.  The codes
+// and scales of x share one workspace.
 torch::Tensor fp4_linear(const torch::Tensor& x, const torch::Tensor& mat_b, const torch::Tensor& block_b,
                          const c10::optional<torch::Tensor>& scales_b, const c10::optional<torch::Tensor>& bias) {
   JO_CHECK_CUDA(x);
   TORCH_CHECK(x.dim() == 2 && x.stride(1) == 1, "x must be [M, K] with contiguous rows");
   const int format = check_fp4(mat_b, block_b, scales_b, x, "mat_b");
   TORCH_CHECK(x.size(1) == 2 * mat_b.size(1), "x and mat_b shapes cannot be multiplied");
+  const int64_t M = x.size(0), N = mat_b.size(0), K = x.size(1);
+  check_product(x, N, x.scalar_type(), bias);
   const c10::cuda::CUDAGuard guard(x.device());
-  auto [a, block_a, scales_a] = quant_fp4(x, format);
-  return fp4_mm(a, mat_b, block_a, block_b,
-                format == JO_FP4_NV ? c10::optional<torch::Tensor>(scales_a) : c10::nullopt, scales_b,
-                x.scalar_type(), bias, format);
+  auto out = new_empty({M, N}, x.scalar_type(), x);
+  const int64_t codes = cdiv(M * (K / 2), 512) * 512, scales = jo_fp4_scale_bytes(M, K, format);
+  auto work = new_empty({codes + scales + 4 * M}, at::kByte, x);
+  uint8_t* const q = work.data_ptr<uint8_t>();
+  float* const row = format == JO_FP4_NV ? reinterpret_cast<float*>(q + codes + scales) : nullptr;
+  void* const stream = stream_of(x);
+  jo_check(jo_quant_fp4(q, K / 2, q + codes, row, x.data_ptr(), x.stride(0), M, K, format, dt_code(x.scalar_type()),
+                        stream),
+           "fp4_linear");
+  jo_check(jo_fp4_scaled_mm(out.data_ptr(), N, q, K / 2, mat_b.data_ptr(), mat_b.stride(0), q + codes,
+                            block_b.data_ptr(), row, (const float*)opt_ptr(scales_b), opt_ptr(bias), M, N, K, format,
+                            dt_code(x.scalar_type()), stream),
+           "fp4_linear");
+  return out;
 }
 
 // ------------------------------------------------------------------ rotary
@@ -145,8 +164,8 @@ std::tuple<torch::Tensor, torch::Tensor> rotary_embed(const torch::Tensor& q, co
   if (has_k) check_heads(*k, q, "k");
   check_tables(q, cos, sin, positions);
   const c10::cuda::CUDAGuard guard(q.device());
-  auto qo = torch::empty(q.sizes(), q.options());
-  auto ko = has_k ? torch::empty(k->sizes(), q.options()) : torch::empty({0}, q.options());
+  auto qo = new_empty(q.sizes(), q.scalar_type(), q);
+  auto ko = has_k ? new_empty(k->sizes(), q.scalar_type(), q) : new_empty({0}, q.scalar_type(), q);
   jo_check(jo_rotary_embed(qo.data_ptr(), qo.stride(0), qo.stride(1), q.data_ptr(), q.stride(0), q.stride(1),
                            has_k ? ko.data_ptr() : nullptr, has_k ? ko.stride(0) : 0, has_k ? ko.stride(1) : 0,
                            has_k ? k->data_ptr() : nullptr, has_k ? k->stride(0) : 0, has_k ? k->stride(1) : 0,
@@ -180,7 +199,7 @@ torch::Tensor rotary_embed_append(const torch::Tensor& q, const torch::Tensor& k
   }
   TORCH_CHECK(k_cache.size(0) == v_cache.size(0), "k_cache and v_cache must have the same rows");
   const c10::cuda::CUDAGuard guard(q.device());
-  auto qo = torch::empty(q.sizes(), q.options());
+  auto qo = new_empty(q.sizes(), q.scalar_type(), q);
   jo_check(jo_rotary_embed_append(qo.data_ptr(), qo.stride(0), qo.stride(1), q.data_ptr(), q.stride(0), q.stride(1),
                                   k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
                                   k_cache.data_ptr(), k_cache.stride(0), k_cache.stride(1), v_cache.data_ptr(),
@@ -222,12 +241,12 @@ std::tuple<torch::Tensor, torch::Tensor> shared_prefix_attention(const torch::Te
               "lens must be contiguous Int32 [batch]");
   TORCH_CHECK(HK > 0 && H % HK == 0, "q heads must be a multiple of kv heads");
   const c10::cuda::CUDAGuard guard(q.device());
-  auto out = torch::empty({B, L, H, D}, q.options());
-  auto lse = torch::empty({B, H, L}, q.options().dtype(at::kFloat));
+  auto out = new_empty({B, L, H, D}, q.scalar_type(), q);
+  auto lse = new_empty({B, H, L}, at::kFloat, q);
   const int64_t bytes = jo_shared_prefix_attention_workspace(B, L, H, HK, D, k_prefix.size(0), k_own.size(1));
   TORCH_CHECK(bytes >= 0, "joyomni_ops::shared_prefix_attention: ", jo_last_error());
   torch::Tensor work;
-  if (bytes) work = torch::empty({bytes}, q.options().dtype(at::kByte));
+  if (bytes) work = new_empty({bytes}, at::kByte, q);
   jo_check(jo_shared_prefix_attention(
                out.data_ptr(), lse.data_ptr<float>(), q.data_ptr(), q.stride(0), q.stride(1), q.stride(2),
                k_prefix.data_ptr(), k_prefix.stride(0), k_prefix.stride(1), v_prefix.data_ptr(), v_prefix.stride(0),

@@ -457,7 +457,7 @@ def quant_fp4(x, format="nvfp4"):
     row_scale None.  block_scale: tiles [ceil(M/128), ceil(blocks/4), 32, 4, 4], where row m and block b of
     a tile sit at [m % 32, m // 32, b].  The rounding rules stand in ``include/joyomni_b200.h``."""
     q, block, row = _ops.quant_fp4(x, _fp4_code(format))
-    return q, block, row if row.shape[0] == x.shape[0] and block.dtype == torch.float8_e4m3fn else None
+    return q, block, row if format == "nvfp4" else None
 
 
 def dequant_fp4(q, block_scale, row_scale=None, dtype=torch.bfloat16):
