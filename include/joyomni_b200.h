@@ -487,9 +487,11 @@ JO_API int jo_rotary_embed_append(void* q_out, int64_t qo_stride_t, int64_t qo_s
  * rows query i sees all or, causal != 0, those up to lens[b] - q_len + i (the queries
  * are the last q_len rows).  out [batch, q_len, q_heads, head_dim] contiguous, lse
  * (natural log-sum-exp of the scaled scores) fp32 [batch, q_heads, q_len]; a query
- * that sees nothing gives 0 and -inf.  dtype F16/BF16, head_dim 64 or 128.  Pointers
- * and strides of q, k and v: multiples of 16 bytes.  workspace: 16-byte aligned,
- * jo_shared_prefix_attention_workspace(...) bytes (-1: bad arguments). */
+ * that sees nothing gives 0 and -inf.  An infinity or a NaN in a key or a value reaches
+ * the queries that see its row and no others; one in an own row's value may make all of
+ * those queries' out NaN.  dtype F16/BF16, head_dim 64 or 128; scale > 0.  Pointers and
+ * strides of q, k and v: multiples of 16 bytes; out and workspace: 32-byte aligned;
+ * workspace: jo_shared_prefix_attention_workspace(...) bytes (-1: bad arguments). */
 JO_API int64_t jo_shared_prefix_attention_workspace(int64_t batch, int64_t q_len, int64_t q_heads, int64_t kv_heads,
                                                     int64_t head_dim, int64_t prefix_len, int64_t own_len);
 JO_API int jo_shared_prefix_attention(void* out, float* lse, const void* q, int64_t q_stride_b, int64_t q_stride_t,

@@ -9,13 +9,16 @@ the reference does (deploy/xvideo/models/dit/dit.py:896-934 and :1159-1163):
 * ``rope_3d``: the (t, h, w) tables concatenated along the head dimension;
 * ``paired_tables``: the half-width bf16 ``[L, D/2]`` tables the paired kernels
   read, taken as every other column of the full-width tables
-  (deploy/xvideo/models/dit/sgl_fused_ops.py:94-119).
+  (deploy/xvideo/models/dit/sgl_fused_ops.py:94-119);
+* ``rotary_tables``: the half-width fp32 tables of ``rotary_embed``, with the frequencies
+  stretched for long contexts (``scaled_freqs``; no reference counterpart).
 
 These are small torch tensor computations, not kernels; the hot path only
 consumes their output.
 """
 from __future__ import annotations
 
+import math
 from typing import Sequence, Tuple
 
 import torch
@@ -64,3 +67,45 @@ def video_chunk_tables(frames: int = 3, height: int = 45, width: int = 80, t0: i
     pos = grid_positions(frames, height, width, t0)
     cos, sin = rope_3d(pos, dims, theta)
     return paired_tables(cos, sin, device=device)
+
+
+def scaled_freqs(dim: int, theta: float = 10000.0, scaling: str = "none", factor: float = 1.0,
+                 original: int = 8192, beta: Tuple[float, float] = (32.0, 1.0)) -> Tuple[torch.Tensor, float]:
+    """Inverse frequencies (fp64 [dim/2]) and the tables' scale for contexts ``factor`` times longer.
+
+    ``"none"``: theta^(-2i/dim).  ``"linear"``: positions divided by factor.  ``"ntk"``: theta times
+    factor^(dim / (dim - 2)), so the lowest frequency is divided by factor and the highest stays.
+    ``"yarn"`` (Peng et al., "YaRN", 2023): frequencies that turn more than beta[0] times within the
+    ``original`` context stay, those below beta[1] turns are divided by factor, a ramp in between; the
+    tables are scaled by 0.1 ln(factor) + 1.
+    """
+    if dim % 2 or dim <= 0:
+        raise ValueError(f"RoPE dimension must be even and positive, got {dim}")
+    if not factor >= 1.0:
+        raise ValueError(f"factor must be at least 1, got {factor}")
+    i = torch.arange(0, dim, 2, dtype=torch.float64)
+    if scaling == "ntk":
+        if dim == 2:
+            raise ValueError("ntk scaling needs more than one frequency")
+        theta = theta * factor ** (dim / (dim - 2))
+    freq = theta ** (-i / dim)
+    if scaling in ("none", "ntk"):
+        return freq, 1.0
+    if scaling == "linear":
+        return freq / factor, 1.0
+    if scaling == "yarn":
+        fast, slow = beta
+        turns = original * freq / (2 * math.pi)
+        keep = ((turns - slow) / (fast - slow)).clamp(0.0, 1.0)
+        return freq / factor * (1 - keep) + freq * keep, 0.1 * math.log(factor) + 1.0
+    raise ValueError(f"unknown scaling {scaling!r}")
+
+
+def rotary_tables(length: int, dim: int, theta: float = 10000.0, scaling: str = "none", factor: float = 1.0,
+                  original: int = 8192, beta: Tuple[float, float] = (32.0, 1.0), device=None):
+    """fp32 cos/sin [length, dim/2] of positions 0..length-1 for ``joyomni_ops.rotary_embed`` (angles in fp64,
+    so that a position of any size keeps its phase); arguments as ``scaled_freqs``."""
+    freq, scale = scaled_freqs(dim, theta, scaling, factor, original, beta)
+    angle = torch.outer(torch.arange(length, dtype=torch.float64), freq)
+    return ((angle.cos() * scale).to(device=device, dtype=torch.float32),
+            (angle.sin() * scale).to(device=device, dtype=torch.float32))
