@@ -444,6 +444,18 @@ JO_API int jo_fp4_scaled_mm(void* d, int64_t ldd, const void* a, int64_t lda, co
                             const void* bias, int64_t m, int64_t n, int64_t k, int format, int out_dtype,
                             void* stream);
 
+/* A Linear layer in 4 bits: jo_quant_fp4 of x [M, K] (F16/BF16) in the weight's format
+ * into the workspace, then jo_fp4_scaled_mm with the weight b [N, K] (packed codes, its
+ * block scales and row scales); D and bias of x's dtype.  Two kernels: the product's
+ * starts loading the weight while the quantisation runs, so nothing else may be writing
+ * the weight by then but work that was queued on `stream` before this call.
+ * workspace: 16-byte aligned, jo_fp4_linear_workspace(m, k, format) bytes (-1: bad
+ * arguments). */
+JO_API int64_t jo_fp4_linear_workspace(int64_t m, int64_t k, int format);
+JO_API int jo_fp4_linear(void* d, int64_t ldd, const void* x, int64_t x_row_stride, const void* b, int64_t ldb,
+                         const void* block_b, const float* scale_b, const void* bias, int64_t m, int64_t n, int64_t k,
+                         int format, int dtype, void* workspace, int64_t workspace_bytes, void* stream);
+
 /* Rotary position embedding by gathered table rows.  q: [tokens, q_heads,
  * head_dim], k: [tokens, k_heads, head_dim] (k_heads == 0: q alone), element
  * (t, h, d) at p[t*stride_t + h*stride_h + d]; an output may be its input.

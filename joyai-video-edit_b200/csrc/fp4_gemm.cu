@@ -110,6 +110,7 @@ struct Fp4GemmArgs {
   const void* bias;
   int m, n, k;
   int tiles_m, tiles_n;
+  bool b_ready;  // B was complete before the previous kernel of the stream began
   unsigned int* fault;
 };
 
@@ -463,6 +464,15 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
   if (split > 1) cluster_sync();  // every CTA of the cluster runs before any part is sent
   tc_fence_after();
   const uint32_t tmem = *reinterpret_cast<uint32_t*>(gbase + (tmem_slot - base));
+  auto load_b = [&](int stage, int kb) {
+    mbar_expect_tx(full_bar(stage), S::kStage);
+    tma_load_2d(base + S::kOffB + stage * S::kB, &map_b, kb * kKBytes, tn * 128, full_bar(stage));
+    tma_load_3d(base + S::kOffSB + stage * F::kScale, &map_sb, 0, kb * F::kTiles, tn, full_bar(stage));
+  };
+  // a layer's weight streams in while the kernel before still quantises its input
+  const int early = args.b_ready ? min(kStages, kb1 - kb0) : 0;
+  if (warp == 0 && lane == 0)
+    for (int s = 0; s < early; ++s) load_b(s, kb0 + s);
   pdl_wait();
   pdl_trigger();
 
@@ -471,10 +481,10 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
       int stage = 0, issued = 0;
       uint32_t phase = 0;
       for (int kb = kb0; kb < kb1; ++kb) {
-        if (!mbar_wait(empty_bar(stage), phase ^ 1u, fault)) break;
-        mbar_expect_tx(full_bar(stage), S::kStage);
-        tma_load_2d(base + S::kOffB + stage * S::kB, &map_b, kb * kKBytes, tn * 128, full_bar(stage));
-        tma_load_3d(base + S::kOffSB + stage * F::kScale, &map_sb, 0, kb * F::kTiles, tn, full_bar(stage));
+        if (issued >= early) {
+          if (!mbar_wait(empty_bar(stage), phase ^ 1u, fault)) break;
+          load_b(stage, kb);
+        }
         tma_load_2d(base + S::kOffA + stage * S::kA, &map_a, kb * kKBytes, tm * kCols, full_bar(stage));
         tma_load_3d(base + S::kOffSA + stage * F::kScale, &map_sa, 0, kb * F::kTiles, tm, full_bar(stage));
         ++issued;
@@ -717,14 +727,12 @@ int dispatch(const Operands& o, const Fp4GemmArgs& g, cudaStream_t st, const Dev
 }  // namespace
 }  // namespace jo
 
-using namespace jo;
+namespace jo {
+namespace {
 
-extern "C" {
-
-int jo_fp4_scaled_mm(void* d, int64_t ldd, const void* a, int64_t lda, const void* b, int64_t ldb,
-                     const void* block_a, const void* block_b, const float* scale_a, const float* scale_b,
-                     const void* bias, int64_t m, int64_t n, int64_t k, int format, int out_dtype, void* stream) {
-  const char* op = "fp4_scaled_mm";
+int fp4_mm(const char* op, void* d, int64_t ldd, const Operands& o, const float* scale_a, const float* scale_b,
+           const void* bias, int64_t m, int64_t n, int64_t k, int format, int out_dtype, bool b_ready,
+           cudaStream_t st) {
   const DeviceInfo* di;
   if (int s = device_info(&di)) return s;
   if (format != JO_FP4_NV && format != JO_FP4_MX) return fail(JO_ERR_INVALID, "%s: unknown 4-bit format %d", op, format);
@@ -734,11 +742,12 @@ int jo_fp4_scaled_mm(void* d, int64_t ldd, const void* a, int64_t lda, const voi
   if (k == 0 || k % 32) return fail(JO_ERR_SHAPE, "%s: K must be a positive multiple of 32", op);
   const int64_t most = INT32_MAX - 512;
   if (m > most || n > most || k > most) return fail(JO_ERR_SHAPE, "%s: size too large", op);
-  if (!d || !a || !b || !block_a || !block_b) return fail(JO_ERR_INVALID, "%s: null operand", op);
-  if (lda < k / 2 || ldb < k / 2 || ldd < n) return fail(JO_ERR_SHAPE, "%s: leading dimension smaller than the row", op);
-  if (lda % 16 || ldb % 16 || n % 8 || ldd % 8)
+  if (!d || !o.a || !o.b || !o.block_a || !o.block_b) return fail(JO_ERR_INVALID, "%s: null operand", op);
+  if (o.lda < k / 2 || o.ldb < k / 2 || ldd < n)
+    return fail(JO_ERR_SHAPE, "%s: leading dimension smaller than the row", op);
+  if (o.lda % 16 || o.ldb % 16 || n % 8 || ldd % 8)
     return fail(JO_ERR_ALIGN, "%s: lda and ldb must be multiples of 16 bytes, N and ldd of 8", op);
-  if (!aligned16(d) || !aligned16(a) || !aligned16(b) || !aligned16(block_a) || !aligned16(block_b) ||
+  if (!aligned16(d) || !aligned16(o.a) || !aligned16(o.b) || !aligned16(o.block_a) || !aligned16(o.block_b) ||
       (scale_b && !aligned16(scale_b)) || (bias && !aligned16(bias)))
     return fail(JO_ERR_ALIGN, "%s: operands must be 16-byte aligned", op);
   Fp4GemmArgs g{};
@@ -750,13 +759,63 @@ int jo_fp4_scaled_mm(void* d, int64_t ldd, const void* a, int64_t lda, const voi
   g.m = (int)m;
   g.n = (int)n;
   g.k = (int)k;
+  g.b_ready = b_ready;
   g.fault = di->fault;
-  const Operands o{a, b, block_a, block_b, lda, ldb};
-  cudaStream_t st = (cudaStream_t)stream;
   const bool mx = format == JO_FP4_MX;
   if (out_dtype == JO_BF16)
     return mx ? dispatch<__nv_bfloat16, true>(o, g, st, di) : dispatch<__nv_bfloat16, false>(o, g, st, di);
   return mx ? dispatch<__half, true>(o, g, st, di) : dispatch<__half, false>(o, g, st, di);
+}
+
+// fp4_linear's workspace: codes, block scales and row scales of x, each from 512 bytes on.
+struct LinearWork {
+  int64_t scales, rows, bytes;
+};
+LinearWork linear_work(int64_t m, int64_t k, int format) {
+  LinearWork w;
+  w.scales = cdiv(m * (k / 2), 512) * 512;
+  w.rows = w.scales + jo_fp4_scale_bytes(m, k, format);
+  w.bytes = w.rows + cdiv(4 * m, 512) * 512;
+  return w;
+}
+
+}  // namespace
+}  // namespace jo
+
+using namespace jo;
+
+extern "C" {
+
+int jo_fp4_scaled_mm(void* d, int64_t ldd, const void* a, int64_t lda, const void* b, int64_t ldb,
+                     const void* block_a, const void* block_b, const float* scale_a, const float* scale_b,
+                     const void* bias, int64_t m, int64_t n, int64_t k, int format, int out_dtype, void* stream) {
+  return fp4_mm("fp4_scaled_mm", d, ldd, Operands{a, b, block_a, block_b, lda, ldb}, scale_a, scale_b, bias, m, n, k,
+                format, out_dtype, false, (cudaStream_t)stream);
+}
+
+int64_t jo_fp4_linear_workspace(int64_t m, int64_t k, int format) {
+  if (m < 0 || k <= 0 || k % 32 || (format != JO_FP4_NV && format != JO_FP4_MX)) return -1;
+  return linear_work(m, k, format).bytes;
+}
+
+int jo_fp4_linear(void* d, int64_t ldd, const void* x, int64_t x_row_stride, const void* b, int64_t ldb,
+                  const void* block_b, const float* scale_b, const void* bias, int64_t m, int64_t n, int64_t k,
+                  int format, int dtype, void* workspace, int64_t workspace_bytes, void* stream) {
+  const char* op = "fp4_linear";
+  if (dtype != JO_BF16 && dtype != JO_F16) return fail(JO_ERR_DTYPE, "%s: x must be bf16 or fp16", op);
+  if (m < 0 || n < 0) return fail(JO_ERR_SHAPE, "%s: negative size", op);
+  const int64_t bytes = jo_fp4_linear_workspace(m, k, format);
+  if (bytes < 0) return fail(JO_ERR_SHAPE, "%s: K must be a positive multiple of 32, in a 4-bit format", op);
+  if (m == 0 || n == 0) return JO_OK;
+  if (!workspace || !aligned16(workspace) || workspace_bytes < bytes)
+    return fail(JO_ERR_INVALID, "%s: a 16-byte aligned workspace of %lld bytes is needed", op, (long long)bytes);
+  const LinearWork w = linear_work(m, k, format);
+  uint8_t* const q = (uint8_t*)workspace;
+  float* const rows = format == JO_FP4_NV ? reinterpret_cast<float*>(q + w.rows) : nullptr;
+  if (int s = jo_quant_fp4(q, k / 2, q + w.scales, rows, x, x_row_stride, m, k, format, dtype, stream)) return s;
+  // the quantisation releases the product's launch only once everything before it is complete
+  return fp4_mm(op, d, ldd, Operands{q, b, q + w.scales, block_b, k / 2, ldb}, rows, scale_b, bias, m, n, k, format,
+                dtype, true, (cudaStream_t)stream);
 }
 
 }  // extern "C"

@@ -67,6 +67,21 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return r;
 }
 
+// n / d for 0 <= n < 2^31 by a multiplication: with s = ceil(log2 d) and m =
+// ceil(2^(31+s) / d) < 2^32, the error m d - 2^(31+s) < d <= 2^s keeps floor(n m / 2^(31+s))
+// exact.  A unit's place takes half a dozen divisions in a row, each some 200 cycles otherwise.
+struct FastDiv {
+  uint32_t mul = 1u << 31, shift = 31;
+  FastDiv() = default;
+  explicit FastDiv(int64_t d) {
+    int s = 0;
+    while (((int64_t)1 << s) < d) ++s;
+    shift = 31 + s;
+    mul = (uint32_t)((((uint64_t)1 << shift) + (uint64_t)d - 1) / (uint64_t)d);
+  }
+  __device__ __forceinline__ int operator()(int n) const { return (int)(((uint64_t)(uint32_t)n * mul) >> shift); }
+};
+
 struct AttnArgs {
   void* out;
   float* lse;
@@ -85,6 +100,9 @@ struct AttnArgs {
   int items, whole, splits;
   int units;   // whole + (items - whole) * splits
   int rows;    // queries per k/v head
+  // by lq * group, group, batch, row_tiles - 1, the number of full and of last row tiles that are
+  // split, and splits
+  FastDiv by_request, by_group, by_batch, by_full, by_tail, by_last, by_splits;
   float* part_o;        // [slots, D]
   float* part_lse;
   unsigned int* fault;
@@ -107,14 +125,14 @@ __device__ __forceinline__ int prefix_tiles(const AttnArgs& a) { return (a.prefi
 __device__ __forceinline__ int own_tiles(const AttnArgs& a, const Unit& u, int b) {
   const int per_request = a.lq * a.group;
   const int last = min(u.row0 + u.rows, (b + 1) * per_request) - 1 - b * per_request;
-  return (own_visible(a, own_len(a, b), last / a.group) + kTileKeys - 1) / kTileKeys;
+  return (own_visible(a, own_len(a, b), a.by_group(last)) + kTileKeys - 1) / kTileKeys;
 }
 
 // Group and row tile of an item.
 __device__ __forceinline__ void tile_of(const AttnArgs& a, int item, int& grp, int& t) {
   const int full = a.groups * (a.row_tiles - 1);
   if (item < full) {
-    grp = item / (a.row_tiles - 1);
+    grp = a.by_full(item);
     t = item - grp * (a.row_tiles - 1);
   } else {
     grp = item - full;
@@ -130,19 +148,19 @@ __device__ __forceinline__ Unit unit_of(const AttnArgs& a, int index) {
   if (index >= a.whole) {
     // the parts of full row tiles first, then those of the groups' last tiles
     const int full = a.groups * (a.row_tiles - 1), cut = max(a.whole, full);
-    int j = index - a.whole, first = a.whole, tail = cut - a.whole;
-    if (j >= tail * a.splits) {
-      j -= tail * a.splits;
-      first = cut;
-      tail = a.items - cut;
+    const int j = index - a.whole, tail = cut - a.whole, last = j - tail * a.splits;
+    if (last < 0) {
+      piece = a.by_tail(j);
+      item = a.whole + j - piece * tail;
+    } else {
+      piece = a.by_last(last);
+      item = cut + last - piece * (a.items - cut);
     }
-    piece = j / tail;
-    item = first + j - piece * tail;
     pieces = a.splits;
   }
   tile_of(a, item, grp, t);
   if (a.within_request) {
-    u.h = grp / a.batch;
+    u.h = a.by_batch(grp);
     u.b0 = u.b1 = grp - u.h * a.batch;
     u.row0 = u.b0 * per_request + t * a.tile_rows;
     u.rows = min(a.tile_rows, per_request - t * a.tile_rows);
@@ -150,16 +168,16 @@ __device__ __forceinline__ Unit unit_of(const AttnArgs& a, int index) {
     u.h = grp;
     u.row0 = t * a.tile_rows;
     u.rows = min(a.tile_rows, a.rows - u.row0);
-    u.b0 = u.row0 / per_request;
-    u.b1 = (u.row0 + u.rows - 1) / per_request;
+    u.b0 = a.by_request(u.row0);
+    u.b1 = a.by_request(u.row0 + u.rows - 1);
   }
   u.slot = pieces > 1 ? ((int64_t)(item - a.whole) * pieces + piece) * a.tile_rows : -1;
   int own = 0;
   if (a.own > 0)
     for (int b = u.b0 + lane; b <= u.b1; b += 32) own += own_tiles(a, u, b);
-  const uint32_t tiles = prefix_tiles(a) + __reduce_add_sync(0xffffffffu, own);
-  u.first = (int)(tiles * (uint32_t)piece / (uint32_t)pieces);
-  u.last = (int)(tiles * (uint32_t)(piece + 1) / (uint32_t)pieces);
+  const int tiles = prefix_tiles(a) + __reduce_add_sync(0xffffffffu, own);
+  u.first = pieces > 1 ? a.by_splits(tiles * piece) : 0;
+  u.last = pieces > 1 ? a.by_splits(tiles * (piece + 1)) : tiles;
   return u;
 }
 
@@ -275,7 +293,7 @@ struct RowOut {
       a.part_lse[u.slot + r] = lse2;
     } else {
       const int per_request = a.lq * a.group, row = u.row0 + r;
-      const int b = row / per_request, in = row - b * per_request, i = in / a.group, g = in - i * a.group;
+      const int b = a.by_request(row), in = row - b * per_request, i = a.by_group(in), g = in - i * a.group;
       const int64_t hq = (int64_t)a.heads * a.group, h = (int64_t)u.h * a.group + g;
       out = reinterpret_cast<T*>(a.out) + (((int64_t)b * a.lq + i) * hq + h) * D;
       a.lse[(b * hq + h) * a.lq + i] = lse2 * 0.6931471805599453f;
@@ -504,8 +522,8 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         continue;
       }
       // this row's request, query and head, and how many of the request's own rows it sees
-      const int flat = u.row0 + min(row, u.rows - 1), my_b = flat / per_request;
-      const int in = flat - my_b * per_request, my_i = in / a.group, my_g = in - my_i * a.group;
+      const int flat = u.row0 + min(row, u.rows - 1), my_b = a.by_request(flat);
+      const int in = flat - my_b * per_request, my_i = a.by_group(in), my_g = in - my_i * a.group;
       const int visible = a.own > 0 ? own_visible(a, own_len(a, my_b), my_i) : 0;
       {
         // Q: a thread loads its row (of a row that both streams use, one half), 32 bytes at a
@@ -540,7 +558,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       const int steps = alternate ? (n + 1 - s) / 2 : n;
       // of a unit within one request: own rows that all of its rows see
       const int seen_by_all =
-          a.own > 0 ? own_visible(a, own_len(a, u.b0), (u.row0 - u.b0 * per_request) / a.group) : 0;
+          a.own > 0 ? own_visible(a, own_len(a, u.b0), a.by_group(u.row0 - u.b0 * per_request)) : 0;
       bool poisoned = false;
       Walk w(a, u, u.first);
       if (alternate && s == 1) w.next(a, u);
@@ -759,7 +777,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) prefix_attn_join_kernel(const
   const int j = (int)(blockIdx.x / (unsigned)a.tile_rows), r = (int)(blockIdx.x - (unsigned)j * a.tile_rows);
   int grp, t;
   tile_of(a, a.whole + j, grp, t);
-  const int h = a.within_request ? grp / a.batch : grp, b0 = a.within_request ? grp - h * a.batch : 0;
+  const int h = a.within_request ? a.by_batch(grp) : grp, b0 = a.within_request ? grp - h * a.batch : 0;
   pdl_wait();
   pdl_trigger();
   if (t * a.tile_rows + r >= (a.within_request ? per_request : a.rows)) return;
@@ -797,7 +815,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) prefix_attn_join_kernel(const
     for (int e = 0; e < E; ++e) o[e] += sums[w][lane * E + e];
   }
   const int64_t hq = (int64_t)a.heads * a.group;
-  const int b = row / per_request, in = row - b * per_request, i = in / a.group, g = in - i * a.group;
+  const int b = a.by_request(row), in = row - b * per_request, i = a.by_group(in), g = in - i * a.group;
   const int64_t hh = (int64_t)h * a.group + g;
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   uint32_t* out = reinterpret_cast<uint32_t*>(reinterpret_cast<T*>(a.out) + (((int64_t)b * a.lq + i) * hq + hh) * D + lane * E);
@@ -842,12 +860,13 @@ Plan make_plan(bool within_request, int64_t tile_rows, int64_t batch, int64_t lq
   // number of parts that ends first.
   const int64_t most = tiles / 2 < 1 ? 1 : tiles / 2 < hold ? tiles / 2 : hold;
   const int64_t rounds = p.items / hold;
+  const int64_t limit = INT32_MAX / (tiles + 1);  // tiles * splits stays within 31 bits
   bool any = false;
   for (int64_t whole = rounds * hold; whole >= 0 && whole >= (rounds - 1) * hold; whole -= hold)
     for (int trial = 1; trial <= 19; ++trial) {
       // up to 16 parts, and the numbers that fill one, two and three rounds
       const int64_t s = trial <= 16 ? trial : whole < p.items ? (trial - 16) * hold / (p.items - whole) : 1;
-      if (s > most || s < 1 || (s > 1 && whole == p.items)) continue;
+      if (s > most || s < 1 || (s > 1 && s > limit) || (s > 1 && whole == p.items)) continue;
       const int64_t cut = whole > full ? whole : full;
       double cost = s > 1 ? kJoinTiles + 0.05 * (double)s : 0.;
       int64_t at = 0;
@@ -1015,6 +1034,15 @@ int jo_shared_prefix_attention(void* out, float* lse, const void* q, int64_t q_s
   a.splits = (int)p.splits;
   a.units = (int)p.units;
   a.rows = (int)p.rows;
+  const int64_t full = p.groups * (p.row_tiles - 1), cut = p.whole > full ? p.whole : full;
+  auto at_least_1 = [](int64_t d) { return FastDiv(d > 1 ? d : 1); };
+  a.by_request = FastDiv(q_len * a.group);
+  a.by_group = FastDiv(a.group);
+  a.by_batch = FastDiv(batch);
+  a.by_full = at_least_1(p.row_tiles - 1);
+  a.by_tail = at_least_1(cut - p.whole);
+  a.by_last = at_least_1(p.items - cut);
+  a.by_splits = FastDiv(p.splits);
   a.part_o = (float*)workspace;
   a.part_lse = (float*)workspace + p.slots * head_dim;
   a.fault = di->fault;

@@ -105,8 +105,7 @@ torch::Tensor fp4_scaled_mm(const torch::Tensor& mat_a, const torch::Tensor& mat
   return out;
 }
 
-// quant_fp4 of x in mat_b's format, then the product: a Linear layer in 4 bits.  The codes
-// and scales of x share one workspace.
+// quant_fp4 of x in mat_b's format, then the product: a Linear layer in 4 bits.
 torch::Tensor fp4_linear(const torch::Tensor& x, const torch::Tensor& mat_b, const torch::Tensor& block_b,
                          const c10::optional<torch::Tensor>& scales_b, const c10::optional<torch::Tensor>& bias) {
   JO_CHECK_CUDA(x);
@@ -117,17 +116,11 @@ torch::Tensor fp4_linear(const torch::Tensor& x, const torch::Tensor& mat_b, con
   check_product(x, N, x.scalar_type(), bias);
   const c10::cuda::CUDAGuard guard(x.device());
   auto out = new_empty({M, N}, x.scalar_type(), x);
-  const int64_t codes = cdiv(M * (K / 2), 512) * 512, scales = jo_fp4_scale_bytes(M, K, format);
-  auto work = new_empty({codes + scales + 4 * M}, at::kByte, x);
-  uint8_t* const q = work.data_ptr<uint8_t>();
-  float* const row = format == JO_FP4_NV ? reinterpret_cast<float*>(q + codes + scales) : nullptr;
-  void* const stream = stream_of(x);
-  jo_check(jo_quant_fp4(q, K / 2, q + codes, row, x.data_ptr(), x.stride(0), M, K, format, dt_code(x.scalar_type()),
-                        stream),
-           "fp4_linear");
-  jo_check(jo_fp4_scaled_mm(out.data_ptr(), N, q, K / 2, mat_b.data_ptr(), mat_b.stride(0), q + codes,
-                            block_b.data_ptr(), row, (const float*)opt_ptr(scales_b), opt_ptr(bias), M, N, K, format,
-                            dt_code(x.scalar_type()), stream),
+  const int64_t bytes = jo_fp4_linear_workspace(M, K, format);
+  auto work = new_empty({bytes}, at::kByte, x);
+  jo_check(jo_fp4_linear(out.data_ptr(), N, x.data_ptr(), x.stride(0), mat_b.data_ptr(), mat_b.stride(0),
+                         block_b.data_ptr(), (const float*)opt_ptr(scales_b), opt_ptr(bias), M, N, K, format,
+                         dt_code(x.scalar_type()), work.data_ptr(), bytes, stream_of(x)),
            "fp4_linear");
   return out;
 }

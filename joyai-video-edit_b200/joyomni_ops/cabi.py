@@ -76,6 +76,8 @@ SIGNATURES = {
     "jo_quant_fp4": [P, I64, P, P, P, I64, I64, I64, I32, I32, P],
     "jo_dequant_fp4": [P, I64, P, I64, P, P, I64, I64, I32, I32, P],
     "jo_fp4_scaled_mm": [P, I64, P, I64, P, I64, P, P, P, P, P, I64, I64, I64, I32, I32, P],
+    "jo_fp4_linear_workspace": [I64, I64, I32],
+    "jo_fp4_linear": [P, I64, P, I64, P, I64, P, P, P, I64, I64, I64, I32, I32, P, I64, P],
     "jo_rotary_embed": [P, I64, I64] * 4 + [P, P, I64, P, I32, I64, I64, I64, I64, I64, I32, I32, I32, P],
     "jo_rotary_embed_append": [P, I64, I64] * 6 + [I64, P, P, P, I64, P, I32, I64, I64, I64, I64, I64, I32, I32, P],
     "jo_shared_prefix_attention_workspace": [I64] * 7,
@@ -92,7 +94,7 @@ SIGNATURES = {
 }
 JO_IPC_HANDLE_BYTES = 64
 _RESTYPES = {"jo_status_name": C.c_char_p, "jo_last_error": C.c_char_p, "jo_launch_count": C.c_uint64,
-             "jo_fp4_scale_bytes": C.c_int64, "jo_shared_prefix_attention_workspace": C.c_int64}
+             "jo_fp4_scale_bytes": C.c_int64, "jo_fp4_linear_workspace": C.c_int64, "jo_shared_prefix_attention_workspace": C.c_int64}
 
 _lib = None
 
