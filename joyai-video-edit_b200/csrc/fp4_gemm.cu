@@ -415,14 +415,20 @@ struct RowsSmem {
   static constexpr int kOffPart = kOffSA + kStages * F::kScale;
   static constexpr int kBars = kOffPart + kPart;
   static constexpr int kBytes = kBars + 256 + 1024;
+  static_assert(kCols / kMaxSplit >= 2, "every CTA of a cluster has columns to add up");
   static constexpr int kTmem = kCols + 64 <= 128 ? 128 : 256;  // accumulator, two stages of scales
 };
 
-template <typename OutT>
-__device__ __forceinline__ void store_one(const Fp4GemmArgs& g, float v, int m, int n, float s_b, float bias) {
-  v *= s_b;
-  if (g.sa) v *= __ldg(g.sa + m);
-  reinterpret_cast<OutT*>(g.d)[(int64_t)m * g.ldd + n] = Elt<OutT>::from_f(v + bias);
+// `count` consecutive rows of A at column n of D: a warp writes 64 contiguous bytes per row.
+template <typename OutT, int kCount>
+__device__ __forceinline__ void store_column(const Fp4GemmArgs& g, const float* v, int m0, int n, float s_b, float bias) {
+  float s_a[kCount];
+#pragma unroll
+  for (int e = 0; e < kCount; ++e) s_a[e] = g.sa && m0 + e < g.m ? __ldg(g.sa + m0 + e) : 1.f;
+  OutT* d = reinterpret_cast<OutT*>(g.d) + (int64_t)m0 * g.ldd + n;
+#pragma unroll
+  for (int e = 0; e < kCount; ++e)
+    if (m0 + e < g.m) d[e * g.ldd] = Elt<OutT>::from_f(v[e] * s_b * s_a[e] + bias);
 }
 
 template <typename OutT, bool kMx, int kCols>
@@ -523,7 +529,9 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
     const float bias = live && args.bias ? Elt<OutT>::to_f(reinterpret_cast<const OutT*>(args.bias)[n]) : 0.f;
     const bool ok = mbar_wait(tfull, 0, fault);
     tc_fence_after();
-    const int share = kCols / split;  // columns that each CTA of the cluster adds up
+    // each CTA of the cluster adds up kCols / split of the columns (both powers of two)
+    const int shift = 31 - __clz(kCols / split), share = 1 << shift;
+    const uint32_t part = base + S::kOffPart + (uint32_t)(rank * share * 128 + nl) * 4;
 #pragma unroll 1
     for (int c = 0; c < kCols && ok; c += 16) {
       uint32_t r[16];
@@ -535,40 +543,43 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
         for (int e = 0; e < 16; ++e) r[e] = 0;
       }
       if (split == 1) {
+        float v[16];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int m = tm * kCols + c + e;
-          if (live && m < args.m) store_one<OutT>(args, __uint_as_float(r[e]), m, n, s_b, bias);
-        }
+        for (int e = 0; e < 16; ++e) v[e] = __uint_as_float(r[e]);
+        if (live) store_column<OutT, 16>(args, v, tm * kCols + c, n, s_b, bias);
       } else {
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          const int to = (c + e) / share;
-          const uint32_t at = base + S::kOffPart + (uint32_t)((rank * share + (c + e) - to * share) * 128 + nl) * 4;
-          asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr(at, to)), "r"(r[e]) : "memory");
+          const int to = (c + e) >> shift, at = (c + e) & (share - 1);
+          asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr(part + at * 512, to)), "r"(r[e])
+                       : "memory");
         }
       }
     }
     tc_fence_before();
+    if (split > 1) {
+      cluster_sync();  // every part has arrived, and nothing reaches another CTA any more
+      const float* from = reinterpret_cast<const float*>(gbase + S::kOffPart) + nl;
+      auto sums = [&](auto count, int c) {
+        constexpr int kCount = decltype(count)::value;
+        float v[kCount] = {};
+        for (int r = 0; r < split; ++r)
+#pragma unroll
+          for (int e = 0; e < kCount; ++e) v[e] += from[((r << shift) + c + e) * 128];
+        if (live) store_column<OutT, kCount>(args, v, tm * kCols + rank * share + c, n, s_b, bias);
+      };
+      if (share >= 8)
+        for (int c = 0; c < share; c += 8) sums(std::integral_constant<int, 8>{}, c);
+      else
+        for (int c = 0; c < share; c += 2) sums(std::integral_constant<int, 2>{}, c);
+    }
   }
+  __syncwarp();
+  if (split > 1 && warp < 2) cluster_sync();
   __syncthreads();
   if (warp == 1) {
     tc_fence_after();
     tmem_free(tmem, S::kTmem);
-  }
-  if (split > 1) {
-    cluster_sync();  // every part has arrived, and nothing reaches another CTA any more
-    const int share = kCols / split;
-    const float* part = reinterpret_cast<const float*>(gbase + S::kOffPart);
-    for (int j = threadIdx.x; j < share * 128; j += kRowsThreads) {
-      const int nl = j & 127, c = j >> 7, n = tn * 128 + nl, m = tm * kCols + rank * share + c;
-      if (n >= args.n || m >= args.m) continue;
-      float v = 0.f;
-      for (int r = 0; r < split; ++r) v += part[(r * share + c) * 128 + nl];
-      const float s_b = args.sb ? __ldg(args.sb + n) : 1.f;
-      const float bias = args.bias ? Elt<OutT>::to_f(reinterpret_cast<const OutT*>(args.bias)[n]) : 0.f;
-      store_one<OutT>(args, v, m, n, s_b, bias);
-    }
   }
 }
 
