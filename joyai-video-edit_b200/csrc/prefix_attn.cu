@@ -239,8 +239,7 @@ struct AttnSmem {
   static constexpr int kRing = D == 64 ? 8 : 5;
   static constexpr int kQ = 0;  // two tiles
   static constexpr int kKV = 2 * kTile;
-  static constexpr int kJoin = kKV + kRing * kTile;  // (m, l) of stream 1
-  static constexpr int kBars = kJoin + kTileRows * 8;
+  static constexpr int kBars = kKV + kRing * kTile;
   static constexpr int kGuard = kBars + 256;  // first non-finite value row of a tile, per warp
   static constexpr int kBytes = kGuard + 64 + 1024 /*align*/;
 };
@@ -285,18 +284,18 @@ template <typename T, int D>
 struct RowOut {
   T* out = nullptr;
   float* part = nullptr;
-  __device__ __forceinline__ RowOut(const AttnArgs& a, const Unit& u, int r, bool live, float m, float l) {
+  __device__ __forceinline__ RowOut(const AttnArgs& a, const Unit& u, int r, bool live, bool lse, float m, float l) {
     if (!live) return;
     const float lse2 = l == 0.f ? -INFINITY : m + __log2f(l);
     if (u.slot >= 0) {
       part = a.part_o + (u.slot + r) * D;
-      a.part_lse[u.slot + r] = lse2;
+      if (lse) a.part_lse[u.slot + r] = lse2;
     } else {
       const int per_request = a.lq * a.group, row = u.row0 + r;
       const int b = a.by_request(row), in = row - b * per_request, i = a.by_group(in), g = in - i * a.group;
       const int64_t hq = (int64_t)a.heads * a.group, h = (int64_t)u.h * a.group + g;
       out = reinterpret_cast<T*>(a.out) + (((int64_t)b * a.lq + i) * hq + h) * D;
-      a.lse[(b * hq + h) * a.lq + i] = lse2 * 0.6931471805599453f;
+      if (lse) a.lse[(b * hq + h) * a.lq + i] = lse2 * 0.6931471805599453f;
     }
   }
   __device__ __forceinline__ void store32(int c, const float* f) const {
@@ -515,7 +514,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       const bool live = row < u.rows;
       if (n == 0) {  // nothing to see: an empty part
         if (!alternate || s == 0) {
-          const RowOut<T, D> dst(a, u, row, live, 0.f, 0.f);
+          const RowOut<T, D> dst(a, u, row, live, true, 0.f, 0.f);
           const float zero[32] = {};
           for (int c = 0; c < D; c += 32) dst.store32(c, zero);
         }
@@ -701,7 +700,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       if (steps > 0) wait(o_full(s), o_count[s]);
       if (!alternate) {
         tc_fence_after();
-        const RowOut<T, D> dst(a, u, row, live && ok, m, l);
+        const RowOut<T, D> dst(a, u, row, live && ok, true, m, l);
         const float inv = poisoned ? __int_as_float(0x7fffffff) : l == 0.f ? 0.f : rcp_approx(l);
         if (warp_live && ok) {
 #pragma unroll 1
@@ -715,38 +714,37 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
           }
         }
       } else {
-        // join the streams: stream 0's warps read both O
-        float2* const join = reinterpret_cast<float2*>(gbase + S::kJoin);
-        if (s == 1) join[r] = make_float2(m, poisoned ? -l : l);  // l >= 0: the sign bit is free
+        // join the streams: each one's warps read both O and store half of the columns.  (m, l)
+        // go through the second Q tile, which such a unit does not use.
+        float2* const join = reinterpret_cast<float2*>(gbase + S::kQ + S::kTile);
+        join[s * kTileRows + r] = make_float2(m, poisoned ? -l : l);  // l >= 0: the sign bit is free
         softmax_sync();
-        if (s == 0) {
-          if (n > 1) wait(o_full(1), o_count[1]);
-          tc_fence_after();
-          float2 other = n > 1 ? join[r] : make_float2(-INFINITY, 0.f);
-          poisoned = poisoned || signbit(other.y);
-          other.y = fabsf(other.y);
-          const float top = fmaxf(m, other.x), shift = top == -INFINITY ? 0.f : top;
-          float f0 = ex2_approx(m - shift), f1 = ex2_approx(other.x - shift);
-          const float sum = f0 * l + f1 * other.y;
-          const RowOut<T, D> dst(a, u, row, live && ok, shift, sum);
-          const float inv = poisoned ? __int_as_float(0x7fffffff) : sum == 0.f ? 0.f : rcp_approx(sum);
-          f0 *= inv;
-          f1 *= inv;
-          if (warp_live && ok) {
+        float2 other = join[(s ^ 1) * kTileRows + r];
+        if (n > 1) wait(o_full(s ^ 1), o_count[s ^ 1]);
+        tc_fence_after();
+        poisoned = poisoned || signbit(other.y);
+        other.y = fabsf(other.y);
+        const float top = fmaxf(m, other.x), shift = top == -INFINITY ? 0.f : top;
+        float mine = ex2_approx(m - shift), theirs = ex2_approx(other.x - shift);
+        const float sum = mine * l + theirs * other.y;
+        const RowOut<T, D> dst(a, u, row, live && ok, s == 0, shift, sum);
+        const float inv = poisoned ? __int_as_float(0x7fffffff) : sum == 0.f ? 0.f : rcp_approx(sum);
+        const float f0 = (s == 0 ? mine : theirs) * inv, f1 = (s == 0 ? theirs : mine) * inv;
+        if (warp_live && ok) {
+          const uint32_t t_0 = tmem + lanes + kColO;
 #pragma unroll 1
-            for (int c = 0; c < D; c += 32) {
-              uint32_t o[32];
-              tmem_ld32(t_o + c, o);
-              float f[32];
+          for (int c = s * (D / 2); c < (s + 1) * (D / 2); c += 32) {
+            uint32_t o[32];
+            tmem_ld32(t_0 + c, o);
+            float f[32];
 #pragma unroll
-              for (int e = 0; e < 32; ++e) f[e] = sum == 0.f ? 0.f : __uint_as_float(o[e]) * f0;
-              if (n > 1) {
-                tmem_ld32(t_o + kTileKeys + c, o);
+            for (int e = 0; e < 32; ++e) f[e] = sum == 0.f ? 0.f : __uint_as_float(o[e]) * f0;
+            if (n > 1) {
+              tmem_ld32(t_0 + kTileKeys + c, o);
 #pragma unroll
-                for (int e = 0; e < 32; ++e) f[e] = sum == 0.f ? 0.f : fmaf(__uint_as_float(o[e]), f1, f[e]);
-              }
-              dst.store32(c, f);
+              for (int e = 0; e < 32; ++e) f[e] = sum == 0.f ? 0.f : fmaf(__uint_as_float(o[e]), f1, f[e]);
             }
+            dst.store32(c, f);
           }
         }
       }
