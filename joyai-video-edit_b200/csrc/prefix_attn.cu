@@ -233,14 +233,17 @@ __device__ __forceinline__ uint32_t pack16<__half>(float lo, float hi) {
   return pack_f16x2(lo, hi);
 }
 
-template <int D>
+// kAlone: every unit has at most 128 rows, so one Q tile does, and the other's place is one
+// more of the ring's: such units hold four tiles at work (two streams' K and V) and are bound
+// by the bytes that are under way beside them.
+template <int D, bool kAlone>
 struct AttnSmem {
   static constexpr int kTile = kTileKeys * D * 2;  // bytes of a K, V or Q tile
-  static constexpr int kRing = D == 64 ? 8 : 5;
-  static constexpr int kQ = 0;  // two tiles
-  static constexpr int kKV = 2 * kTile;
+  static constexpr int kRing = (D == 64 ? 11 : 5) + kAlone;
+  static constexpr int kQ = 0;
+  static constexpr int kKV = (kAlone ? 1 : 2) * kTile;
   static constexpr int kBars = kKV + kRing * kTile;
-  static constexpr int kGuard = kBars + 256;  // first non-finite value row of a tile, per warp
+  static constexpr int kGuard = kBars + 320;  // first non-finite value row of a tile, per warp
   static constexpr int kBytes = kGuard + 64 + 1024 /*align*/;
 };
 
@@ -309,12 +312,12 @@ struct RowOut {
   }
 };
 
-template <typename T, int D>
+template <typename T, int D, bool kAlone>
 __global__ void __launch_bounds__(kAttnThreads, 1)
     prefix_attn_kernel(const __grid_constant__ CUtensorMap map_kp, const __grid_constant__ CUtensorMap map_vp,
                        const __grid_constant__ CUtensorMap map_ko, const __grid_constant__ CUtensorMap map_vo,
                        const AttnArgs a) {
-  using S = AttnSmem<D>;
+  using S = AttnSmem<D, kAlone>;
   constexpr int kRing = S::kRing;
   constexpr int kBox = kTileKeys * 128;  // bytes of one 64-element-wide box
   extern __shared__ uint8_t smem_raw[];
@@ -363,7 +366,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         const Unit u = unit_of(a, unit);
         const int n = u.last - u.first;
         if (n == 0) continue;
-        const bool alternate = u.rows <= kTileRows;
+        const bool alternate = kAlone || u.rows <= kTileRows;
         Walk wk(a, u, u.first), wv(wk);  // of K, of V
         for (int j = 0; j < 2 * n && lane == 0 && ok; ++j, ++at) {
           const int slot = at % kRing;
@@ -438,7 +441,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         if (n == 0) continue;
         wait(q_full, q_phase);
         q_phase ^= 1u;
-        if (u.rows > kTileRows) {
+        if (!kAlone && u.rows > kTileRows) {
           // both streams use every tile: K0 V0 K1 V1 ...
           v = k;
           v.advance(1);
@@ -509,7 +512,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     for (int unit = blockIdx.x; unit < a.units; unit += gridDim.x) {
       const Unit u = unit_of(a, unit);
       const int n = u.last - u.first;
-      const bool alternate = u.rows <= kTileRows;
+      const bool alternate = kAlone || u.rows <= kTileRows;
       const int row = alternate ? r : s * kTileRows + r;  // of the unit
       const bool live = row < u.rows;
       if (n == 0) {  // nothing to see: an empty part
@@ -715,12 +718,12 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         }
       } else {
         // join the streams: each one's warps read both O and store half of the columns.  (m, l)
-        // go through the second Q tile, which such a unit does not use.
-        float2* const join = reinterpret_cast<float2*>(gbase + S::kQ + S::kTile);
+        // go through Q's place: both streams' products are done with it.
+        if (s == 1 || n > 1) wait(o_full(s ^ 1), o_count[s ^ 1]);
+        float2* const join = reinterpret_cast<float2*>(gbase + S::kQ);
         join[s * kTileRows + r] = make_float2(m, poisoned ? -l : l);  // l >= 0: the sign bit is free
         softmax_sync();
         float2 other = join[(s ^ 1) * kTileRows + r];
-        if (n > 1) wait(o_full(s ^ 1), o_count[s ^ 1]);
         tc_fence_after();
         poisoned = poisoned || signbit(other.y);
         other.y = fabsf(other.y);
@@ -934,17 +937,25 @@ int make_kv_map(const char* op, CUtensorMap* map, const void* ptr, int64_t d, in
   return JO_OK;
 }
 
+template <typename T, int D, bool kAlone>
+int launch_units(const CUtensorMap* maps, const AttnArgs& a, cudaStream_t st, const DeviceInfo* di) {
+  const char* op = "shared_prefix_attention";
+  auto kern = prefix_attn_kernel<T, D, kAlone>;
+  constexpr int smem = AttnSmem<D, kAlone>::kBytes;
+  static std::atomic<uint64_t> reserved{0};
+  if (int s = reserve_smem((const void*)kern, smem, reserved, di, op)) return s;
+  if (cudaError_t e = launch_pdl(kern, dim3((unsigned)(a.units < di->sm_count ? a.units : di->sm_count)),
+                                 dim3(kAttnThreads), smem, st, maps[0], maps[1], maps[2], maps[3], a))
+    return launch_failed(e, op);
+  return after_launch("prefix_attn_kernel");
+}
+
 template <typename T, int D>
 int launch_attention(const CUtensorMap* maps, const AttnArgs& a, const Plan& p, cudaStream_t st, const DeviceInfo* di) {
   const char* op = "shared_prefix_attention";
-  auto kern = prefix_attn_kernel<T, D>;
-  constexpr int smem = AttnSmem<D>::kBytes;
-  static std::atomic<uint64_t> reserved{0};
-  if (int s = reserve_smem((const void*)kern, smem, reserved, di, op)) return s;
-  if (cudaError_t e = launch_pdl(kern, dim3((unsigned)(p.units < di->sm_count ? p.units : di->sm_count)), dim3(kAttnThreads), smem, st, maps[0], maps[1],
-                                 maps[2], maps[3], a))
-    return launch_failed(e, op);
-  if (int s = after_launch("prefix_attn_kernel")) return s;
+  if (int s = p.tile_rows <= kTileRows ? launch_units<T, D, true>(maps, a, st, di)
+                                       : launch_units<T, D, false>(maps, a, st, di))
+    return s;
   if (const int64_t joined = (p.items - p.whole) * p.tile_rows) {
     if (cudaError_t e = launch_pdl(prefix_attn_join_kernel<T, D>, dim3((unsigned)joined), dim3(32 * kJoinWarps), 0, st, a))
       return launch_failed(e, op);
