@@ -361,13 +361,17 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     if (warp == 8) {
       // ---------------- TMA producer (lane 0; the warp finds the units together)
       int at = 0;  // loads so far
-      bool ok = true;
+      bool ok = true, first_unit = true;
       for (int unit = blockIdx.x; unit < a.units; unit += gridDim.x) {
         const Unit u = unit_of(a, unit);
         const int n = u.last - u.first;
         if (n == 0) continue;
         const bool alternate = kAlone || u.rows <= kTileRows;
         Walk wk(a, u, u.first), wv(wk);  // of K, of V
+        // The first unit's Q is asked for before any K and V: behind a ring's worth of them on
+        // every SM (24 MB) it would take 4 us.
+        if (first_unit) asm volatile("bar.sync 5, 288;" ::: "memory");
+        first_unit = false;
         for (int j = 0; j < 2 * n && lane == 0 && ok; ++j, ++at) {
           const int slot = at % kRing;
           if (!(ok = mbar_wait(empty(slot), ((at / kRing) & 1) ^ 1u, a.fault))) break;
@@ -508,6 +512,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(bar);
     };
+    bool first_unit = true;
     int count = 0, at = 0, guards = 0, o_count[2] = {0, 0};
     for (int unit = blockIdx.x; unit < a.units; unit += gridDim.x) {
       const Unit u = unit_of(a, unit);
@@ -523,10 +528,9 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         }
         continue;
       }
-      // this row's request, query and head, and how many of the request's own rows it sees
+      // this row's request, query and head
       const int flat = u.row0 + min(row, u.rows - 1), my_b = a.by_request(flat);
       const int in = flat - my_b * per_request, my_i = a.by_group(in), my_g = in - my_i * a.group;
-      const int visible = a.own > 0 ? own_visible(a, own_len(a, my_b), my_i) : 0;
       {
         // Q: a thread loads its row (of a row that both streams use, one half), 32 bytes at a
         // time, all of it before the streams meet; 128-byte swizzle; rows past the last are zero
@@ -542,6 +546,8 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
             v[c][1] = ld_stream(q + c * 16 + 8);
           }
         }
+        if (first_unit) asm volatile("bar.arrive 5, 288;" ::: "memory");  // Q is on its way: K and V may follow
+        first_unit = false;
         softmax_sync();  // both streams are done with the last unit's Q and O
         uint8_t* const dst = gbase + S::kQ + (alternate ? 0 : s * S::kTile) + r * 128;
 #pragma unroll
@@ -556,6 +562,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         arrive_warp(q_full);
       }
+      const int visible = a.own > 0 ? own_visible(a, own_len(a, my_b), my_i) : 0;  // own rows that this row sees
       const bool warp_live = (alternate ? 0 : s * kTileRows) + ((warp & 3) << 5) < u.rows;
       const int steps = alternate ? (n + 1 - s) / 2 : n;
       // of a unit within one request: own rows that all of its rows see
