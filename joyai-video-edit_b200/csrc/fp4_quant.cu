@@ -19,8 +19,6 @@
 // load), so a block's maximum needs no shuffle (MX: one) and its 16 codes leave as
 // one 8-byte store.  One pass: the row stays in registers between its maximum and
 // its codes.  `warps` warps share a row, each lane holding up to kRuns runs.
-#include <cuda_fp4.h>
-
 #include "fp4.cuh"
 #include "quant.cuh"
 
@@ -230,6 +228,18 @@ __global__ void __launch_bounds__(kMaxThreads) quant_fp4_kernel(const QuantArgs 
   }
 }
 
+// Eight codes, the lowest first, as pairs of fp16.
+__device__ __forceinline__ void e2m1x8_to_half(uint32_t w, uint32_t* h) {
+  asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+      "mov.b32 {b0, b1, b2, b3}, %4;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %0, b0;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %1, b1;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %2, b2;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %3, b3;\n\t}"
+      : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
+      : "r"(w));
+}
+
 struct DequantArgs {
   void* out;
   int64_t ldo;
@@ -286,16 +296,25 @@ __global__ void __launch_bounds__(kQuantThreads) dequant_fp4_kernel(const Dequan
     const uint32_t at = u0 + i * kQuantThreads, over = at / (uint32_t)a.runs, u = at - over * a.runs;
     const int64_t m = m0 + over;
     if (base + threadIdx.x + i * kQuantThreads >= a.total) break;
-    const float s = fp4_scale_value<kMx>(scale[i]);
-    const uint32_t w[2] = {code[i].x, code[i].y};
+    uint32_t h[8];  // pairs of fp16
+    e2m1x8_to_half(code[i].x, h);
+    e2m1x8_to_half(code[i].y, h + 4);
     float f[16];
+    if constexpr (kMx) {
+      const float s = fp4_scale_value<true>(scale[i]);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const __half2_raw h =
-          __nv_cvt_fp4x2_to_halfraw2((__nv_fp4x2_storage_t)((w[j / 4] >> (8 * (j % 4))) & 0xffu), __NV_E2M1);
-      const float2 v = __half22float2(__half2(h));
-      f[2 * j] = kMx ? v.x * s : __fmul_rn(v.x * s, row[i]);  // code * s is exact
-      f[2 * j + 1] = kMx ? v.y * s : __fmul_rn(v.y * s, row[i]);
+      for (int j = 0; j < 8; ++j) {
+        const float2 v = __fmul2_rn(__half22float2(*reinterpret_cast<const __half2*>(&h[j])), f2(s));
+        f[2 * j] = v.x, f[2 * j + 1] = v.y;
+      }
+    } else {
+      // code * s has 6 significant bits, from 2^-10 to 2688: exact in fp16
+      const __half2 s = __half2half2(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)scale[i], __NV_E4M3)));
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float2 v = __fmul2_rn(__half22float2(__hmul2(*reinterpret_cast<const __half2*>(&h[j]), s)), f2(row[i]));
+        f[2 * j] = v.x, f[2 * j + 1] = v.y;
+      }
     }
     store16(reinterpret_cast<T*>(a.out) + m * a.ldo + (int64_t)u * 16, f, a.align);
   }
