@@ -42,8 +42,22 @@
 // Warp 9: tcgen05.mma issuer: S = Q K^T (both operands in shared memory), O += P V with P
 //   from tensor memory and V as it lies ([keys, D], the MN-major operand).
 //
-// P is rounded to q's 16-bit type for the tensor cores (its error averages out over the
-// keys: 2^-9 relative for bf16, like the output's own rounding); l sums the unrounded p.
+// P is rounded to q's 16-bit type for the tensor cores, a relative 2^-8 at most for bf16 as
+// the output's own rounding, whose errors average out over the keys; l sums the unrounded p.
+//
+// Bound and measured (B200; us per call, calls in a row).  Many queries: the chain of one
+// stream, S -> softmax -> P V -> S, whose softmax (S in 300 cycles, maximum 150-300,
+// exponentials 1300 at 16 per clock and SM, P 150) is longer than the other stream's products
+// (1024): 2 x 900 queries x 24 heads of 128 over 43200 + 900 rows 890 us = 1.08 PFLOP/s (1050
+// us once the power cap lowers the clock), tensor cores busy 57 %.  Single tokens: bytes, and
+// the start and end of the one unit that each SM has: 32 tokens x 8 k/v heads over 10800
+// shared and 512 own rows 32 us (the first tile arrives 5 us after the launch, the tiles take
+// 15, storing and joining the parts 8), one token over 777 rows 7.9 us.
+//
+// Tried and slower, same 2 x 900 queries: a quarter / half of the exponentials as a polynomial
+// on the FMA units 943 / 1056 us (938 without), two threads per row and 16 softmax warps 1021
+// (928), one tile of 128 rows per CTA and two CTAs per SM 1535; spinning instead of suspended
+// barrier waits and a longer ring for single tokens changed nothing.
 #include "quant.cuh"
 #include "tcgen05.cuh"
 

@@ -16,6 +16,11 @@
 // or in the half layout the two vectors that hold both halves of its pairs) and walks
 // over the heads of q, k (and v), so the table row is read once per token and place
 // and stays in registers, and neither layout needs a shuffle or a second load.
+//
+// Measured (B200, bf16): 10800 tokens x 48 heads of 128, interleaved, 48.9 us (5.5 TB/s, 0.84
+// of the measured copy; 63.9 with a head's load behind the store before it); 4099 x 40 heads,
+// half layout, half of each head, 16.5 us (5.1 TB/s; 23.2 at two CTAs per SM); append of 2043
+// tokens x 72 heads 15.4 us, of 32 tokens 2.4.
 #include "common.cuh"
 
 namespace jo {
