@@ -478,20 +478,29 @@ def fp4_linear(x, mat_b, block_b, scales_b=None, bias: Optional[torch.Tensor] = 
 
 
 class _RotaryEmbed(torch.autograd.Function):
-    """rotary_embed with its gradient; the tables and positions have none."""
+    """The rotation or its inverse, each the other's gradient; the tables and positions have none."""
 
     @staticmethod
-    def forward(ctx, q, k, cos, sin, positions, interleaved):
+    def forward(ctx, q, k, cos, sin, positions, interleaved, inverse):
         ctx.save_for_backward(cos, sin, positions)
-        ctx.interleaved = interleaved
-        qo, ko = _ops.rotary_embed(q, k, cos, sin, positions, interleaved, False)
+        ctx.form = interleaved, inverse
+        qo, ko = _ops.rotary_embed(q, k, cos, sin, positions, interleaved, inverse)
         return qo, ko if k is not None else None
 
     @staticmethod
     def backward(ctx, dq, dk):
-        cos, sin, positions = ctx.saved_tensors
-        dq, dk = rotary_embed_backward(dq, dk, cos, sin, positions, ctx.interleaved)
-        return dq, dk, None, None, None, None
+        interleaved, inverse = ctx.form
+        # the gradient of a sum or a mean comes as one expanded value
+        dq, dk = (g if g is None or g.stride(-1) == 1 else g.contiguous() for g in (dq, dk))
+        dq, dk = _rotate(dq, dk, *ctx.saved_tensors, interleaved, not inverse)
+        return dq, dk, None, None, None, None, None
+
+
+def _rotate(q, k, cos, sin, positions, interleaved, inverse):
+    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+        return _RotaryEmbed.apply(q, k, cos, sin, positions, interleaved, inverse)
+    qo, ko = _ops.rotary_embed(q, k, cos, sin, positions, interleaved, inverse)
+    return qo, ko if k is not None else None
 
 
 def rotary_embed(q, k, cos, sin, positions, interleaved=False):
@@ -499,16 +508,12 @@ def rotary_embed(q, k, cos, sin, positions, interleaved=False):
     [P, R/2]) at positions (int [T]) rotate the first R elements of each head, in pairs (2i, 2i+1) if
     interleaved, else (i, i + R/2); the other elements are copied.  fp32 math, one rounding.  Differentiable
     in q and k.  A position outside the tables gives NaN.  Returns (q, k) (k None if it was)."""
-    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
-        return _RotaryEmbed.apply(q, k, cos, sin, positions, interleaved)
-    qo, ko = _ops.rotary_embed(q, k, cos, sin, positions, interleaved, False)
-    return qo, ko if k is not None else None
+    return _rotate(q, k, cos, sin, positions, interleaved, False)
 
 
 def rotary_embed_backward(dq, dk, cos, sin, positions, interleaved=False):
     """Gradients with respect to rotary_embed's q and k from those of its outputs: the inverse rotation."""
-    qo, ko = _ops.rotary_embed(dq, dk, cos, sin, positions, interleaved, True)
-    return qo, ko if dk is not None else None
+    return _rotate(dq, dk, cos, sin, positions, interleaved, True)
 
 
 def rotary_embed_append(q, k, v, cos, sin, positions, slots, k_cache, v_cache, interleaved=False):

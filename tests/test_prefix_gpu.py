@@ -272,6 +272,29 @@ def test_rotary_gradient(jo, dev, interleaved):
         assert not jo.rotary_embed(q, k, cos, sin, at, interleaved)[0].requires_grad
 
 
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_rotary_gradient_of_broadcast_values(jo, dev, dtype):
+    g = gen(dev, 7)
+    q, k = (normal(g, dev, 6, h, 64).to(dtype).requires_grad_() for h in (3, 1))
+    cos, sin = tables(dev, 9, 64)
+    at = torch.arange(6, device=dev)
+    qo, ko = jo.rotary_embed(q, k, cos, sin, at)
+    (qo.sum() + ko.sum()).backward()  # one value for all elements
+    check_rotary(q.grad, torch.ones_like(q), cos, sin, at, False, inverse=True)
+    check_rotary(k.grad, torch.ones_like(k), cos, sin, at, False, inverse=True)
+    q.grad = k.grad = None
+    row = normal(g, dev, 64).to(dtype)
+    qo, ko = jo.rotary_embed(q, k, cos, sin, at)
+    torch.autograd.backward([qo], [row.expand(6, 3, 64)])  # one row for all heads; none for k
+    check_rotary(q.grad, row.expand(6, 3, 64), cos, sin, at, False, inverse=True)
+    assert not k.grad.any()
+    # twice: the gradient of |dq|^2 with respect to the value that came in is twice its rotation there and back
+    d = normal(g, dev, 6, 3, 64).to(dtype).requires_grad_()
+    dq, = torch.autograd.grad(jo.rotary_embed(q, None, cos, sin, at)[0], q, d, create_graph=True)
+    dd, = torch.autograd.grad(dq, d, dq.detach())
+    check_rotary(dd, dq.detach(), cos, sin, at, False)
+
+
 @pytest.mark.parametrize("interleaved", [True, False])
 def test_rotary_strides_and_places_outside_the_tables(jo, dev, interleaved):
     g = gen(dev, 6)
