@@ -88,8 +88,8 @@ def step(layer: PrefixAttention, x: torch.Tensor, cache: PrefixCache, cos: torch
     i = torch.arange(n, device=x.device, dtype=torch.int32)
     new = cache.lens.new_full((b,), n) if counts is None else counts
     row = cache.lens[:, None] + i - (n - new)[:, None]  # own row of token i; before the first: padding
-    padding = i < (n - new)[:, None]
-    slot = torch.where(padding, -1, row.long() + rows * torch.arange(b, device=x.device)[:, None])
+    kept = (i >= (n - new)[:, None]) & (row < rows)  # a replay beyond the cache's end leaves the next request alone
+    slot = torch.where(kept, row.long() + rows * torch.arange(b, device=x.device)[:, None], -1)
     position = (cache.k_prefix.shape[0] + row.clamp(min=0)).long()
     q = jo.rotary_embed_append(q, k, v, cos, sin, position.view(-1), slot.view(-1), cache.k_own.view(b * rows, hk, d),
                                cache.v_own.view(b * rows, hk, d), layer.interleaved)

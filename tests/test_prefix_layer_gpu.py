@@ -93,3 +93,24 @@ def test_step_in_a_graph(jo, dev):
         held.copy_(x[i])
         graph.replay()
         assert torch.equal(y, want[i])
+
+
+def test_replay_beyond_the_cache_leaves_the_next_request_alone(jo, dev):
+    from joyomni_ops import prefix, rope
+
+    g = torch.Generator(device=dev)
+    g.manual_seed(2)
+    rnd = lambda *s: torch.randn(s, generator=g, device=dev)
+    layer = prefix.PrefixAttention(prefix.quantize_linear_fp4(rnd(384, 128)), prefix.quantize_linear_fp4(rnd(128, 128)),
+                                   2, 2, 64)
+    cos, sin = rope.rotary_tables(200, 64, device=dev)
+    cache = prefix.PrefixCache.allocate(rnd(100, 2, 64).to(BF), rnd(100, 2, 64).to(BF), 3, 50)
+    for x in (cache.k_own, cache.v_own):
+        x.fill_(7)
+    cache.lens[:] = torch.tensor([50, 3, 49], device=dev, dtype=torch.int32)  # the host does not know: filled is 0
+    prefix.step(layer, rnd(3, 2, 128).to(BF), cache, cos, sin)
+    for x in (cache.k_own, cache.v_own):
+        changed = (x != 7).flatten(2).any(2)
+        want = torch.zeros(3, 50, dtype=torch.bool, device=dev)
+        want[1, 3:5], want[2, 49] = True, True
+        assert torch.equal(changed, want)
