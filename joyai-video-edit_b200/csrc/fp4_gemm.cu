@@ -159,8 +159,8 @@ struct PairSmem {
 // 32 accumulator columns of this lane's row: scales, bias, rounding, four 16-byte chunks into
 // the warp's staging box (row = lane, 128-byte swizzle) from chunk `c0` on.
 template <typename OutT>
-__device__ __forceinline__ void stage32(const Fp4GemmArgs& g, const uint32_t* r, int n0, float s_a, uint8_t* box, int lane,
-                                        int c0) {
+__device__ __forceinline__ void stage32(const Fp4GemmArgs& g, const uint32_t* r, int n0, float s_a, uint8_t* box,
+                                        int lane, int c0) {
   const OutT* bias = reinterpret_cast<const OutT*>(g.bias);
 #pragma unroll
   for (int h = 0; h < 4; ++h) {
@@ -431,7 +431,8 @@ struct RowsSmem {
 
 // `count` consecutive rows of A at column n of D: a warp writes 64 contiguous bytes per row.
 template <typename OutT, int kCount>
-__device__ __forceinline__ void store_column(const Fp4GemmArgs& g, const float* v, int m0, int n, float s_b, float bias) {
+__device__ __forceinline__ void store_column(const Fp4GemmArgs& g, const float* v, int m0, int n, float s_b,
+                                             float bias) {
   float s_a[kCount];
 #pragma unroll
   for (int e = 0; e < kCount; ++e) s_a[e] = g.sa && m0 + e < g.m ? __ldg(g.sa + m0 + e) : 1.f;
@@ -694,7 +695,8 @@ int launch_pair(const Operands& o, Fp4GemmArgs g, cudaStream_t st, const DeviceI
   const int tiles = g.tiles_m * g.tiles_n;
   cfg.gridDim = dim3(2 * (unsigned)(tiles < pairs ? tiles : pairs), 1, 1);
   cfg.numAttrs = 2;
-  if (cudaError_t e = cudaLaunchKernelEx(&cfg, kern, maps[0], maps[1], maps[2], maps[3], maps[4], g)) return launch_failed(e, op);
+  if (cudaError_t e = cudaLaunchKernelEx(&cfg, kern, maps[0], maps[1], maps[2], maps[3], maps[4], g))
+    return launch_failed(e, op);
   return after_launch("fp4_gemm_pair_kernel");
 }
 
@@ -708,7 +710,8 @@ int launch_rows(const Operands& o, Fp4GemmArgs g, cudaStream_t st, const DeviceI
   g.tiles_m = (int)cdiv(g.m, kCols);
   g.tiles_n = (int)cdiv(g.n, 128);
   if (kCols < 128 && g.tiles_m > 1) return fail(JO_ERR_SHAPE, "%s: %d rows in a tile of %d", op, g.m, kCols);
-  if (g.tiles_m > 65535 || (int64_t)g.tiles_n * kMaxSplit > INT32_MAX) return fail(JO_ERR_SHAPE, "%s: too many tiles", op);
+  if (g.tiles_m > 65535 || (int64_t)g.tiles_n * kMaxSplit > INT32_MAX)
+    return fail(JO_ERR_SHAPE, "%s: too many tiles", op);
   // K in as many parts as still leave two stages each, until every SM has a CTA
   const int64_t tiles = (int64_t)g.tiles_m * g.tiles_n, kblocks = cdiv(g.k, kKElems);
   int split = 1;
@@ -736,7 +739,10 @@ int launch_rows(const Operands& o, Fp4GemmArgs g, cudaStream_t st, const DeviceI
 
 template <typename OutT, bool kMx>
 int dispatch(const Operands& o, const Fp4GemmArgs& g, cudaStream_t st, const DeviceInfo* di) {
-  // CTA pairs where their 256 x 256 tiles keep most SMs busy
+  // CTA pairs where their 256 x 256 tiles occupy at least half of the SMs; below that the rows
+  // kernel's smaller tiles, split over K, finish sooner. Pairs / rows, microseconds, M x N x K:
+  // 200 x 1024 x 1024 (a twentieth of the SMs) 8.8 / 8.8; 512 x 3072 x 3072 (a third)
+  // 11.7 / 10.6; 1350 x 3072 x 3072 (all, 72 of 74 pairs) 12.3 / 20.9.
   const int64_t pair_tiles = cdiv(g.m, kPairM) * cdiv(g.n, kPairN);
   if (g.m > 128 && pair_tiles * 2 * 2 >= di->sm_count) return launch_pair<OutT, kMx>(o, g, st, di);
   if (g.m <= 16) return launch_rows<OutT, kMx, 16>(o, g, st, di);
@@ -756,7 +762,8 @@ int fp4_mm(const char* op, void* d, int64_t ldd, const Operands& o, const float*
            cudaStream_t st) {
   const DeviceInfo* di;
   if (int s = device_info(&di)) return s;
-  if (format != JO_FP4_NV && format != JO_FP4_MX) return fail(JO_ERR_INVALID, "%s: unknown 4-bit format %d", op, format);
+  if (format != JO_FP4_NV && format != JO_FP4_MX)
+    return fail(JO_ERR_INVALID, "%s: unknown 4-bit format %d", op, format);
   if (m < 0 || n < 0 || k < 0) return fail(JO_ERR_SHAPE, "%s: negative size", op);
   if (out_dtype != JO_BF16 && out_dtype != JO_F16) return fail(JO_ERR_DTYPE, "%s: out dtype must be bf16/fp16", op);
   if (m == 0 || n == 0) return JO_OK;

@@ -364,7 +364,8 @@ int dispatch_quant(QuantArgs a, const DeviceInfo* di, cudaStream_t st) {
 
 int check_fp4(const char* op, const void* q, int64_t ldq, const void* bs, const void* rs, int64_t rows, int64_t cols,
               int format, int dtype) {
-  if (format != JO_FP4_NV && format != JO_FP4_MX) return fail(JO_ERR_INVALID, "%s: unknown 4-bit format %d", op, format);
+  if (format != JO_FP4_NV && format != JO_FP4_MX)
+    return fail(JO_ERR_INVALID, "%s: unknown 4-bit format %d", op, format);
   if (dtype != JO_F32 && dtype != JO_F16 && dtype != JO_BF16)
     return fail(JO_ERR_DTYPE, "%s: values must be fp32, fp16 or bf16", op);
   if (rows < 0 || cols < 0) return fail(JO_ERR_SHAPE, "%s: negative size", op);

@@ -1019,8 +1019,8 @@ int jo_shared_prefix_attention(void* out, float* lse, const void* q, int64_t q_s
   if (batch == 0 || q_len == 0) return JO_OK;
   if (!out || !lse || !q || !lens || (prefix_len && (!k_prefix || !v_prefix)) || (own_len && (!k_own || !v_own)))
     return fail(JO_ERR_INVALID, "%s: null operand", op);
-  if ((reinterpret_cast<uintptr_t>(out) & 31) || !aligned16(q) || !aligned16(k_prefix) || !aligned16(v_prefix) || !aligned16(k_own) ||
-      !aligned16(v_own))
+  if ((reinterpret_cast<uintptr_t>(out) & 31) || !aligned16(q) || !aligned16(k_prefix) || !aligned16(v_prefix) ||
+      !aligned16(k_own) || !aligned16(v_own))
     return fail(JO_ERR_ALIGN, "%s: operands must be 16-byte aligned (out: 32)", op);
   // a stride of a dimension of size 1 is never used
   const struct {
@@ -1035,8 +1035,10 @@ int jo_shared_prefix_attention(void* out, float* lse, const void* q, int64_t q_s
     if (u.size > 1 && (u.stride % 8 || u.stride < 0))
       return fail(JO_ERR_ALIGN, "%s: strides must be multiples of 16 bytes and not negative", op);
   const Plan p = plan_attention(batch, q_len, kv_heads, q_heads / kv_heads, prefix_len, own_len, di->sm_count);
-  if (p.units > INT32_MAX / 2 || (p.items - p.whole) * p.tile_rows > INT32_MAX) return fail(JO_ERR_SHAPE, "%s: size too large", op);
-  if (p.slots && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 31) || workspace_bytes < p.slots * (head_dim + 1) * 4))
+  if (p.units > INT32_MAX / 2 || (p.items - p.whole) * p.tile_rows > INT32_MAX)
+    return fail(JO_ERR_SHAPE, "%s: size too large", op);
+  if (p.slots && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 31) ||
+                  workspace_bytes < p.slots * (head_dim + 1) * 4))
     return fail(JO_ERR_INVALID, "%s: a 32-byte aligned workspace of %lld bytes is needed", op,
                 (long long)(p.slots * (head_dim + 1) * 4));
   AttnArgs a{};
