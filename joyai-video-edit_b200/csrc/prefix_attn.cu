@@ -26,7 +26,9 @@
 // others their p is 0).  For single tokens the tensor cores have time for that: a tile costs
 // its bytes.  Row tiles run across requests or stay within one, whichever costs fewer tiles
 // (plan_attention).  Where the units do not fill the GPU evenly, the last ones' walks are
-// split and joined.
+// split and joined: by a second kernel, or, where all units are parts and few rows are to be
+// joined, by the CTAs of a cluster from each other's shared memory (one launch and no
+// workspace: one token over 777 rows 11.3 -> 8.3 us per call, 8.2 -> 7.2 on the GPU).
 //
 // One CTA per SM goes through its units with two streams, each with its own S, P and O in
 // tensor memory, so that one stream's softmax runs while the other's products do:
@@ -52,7 +54,7 @@
 // us once the power cap lowers the clock), tensor cores busy 57 %.  Single tokens: bytes, and
 // the start and end of the one unit that each SM has: 32 tokens x 8 k/v heads over 10800
 // shared and 512 own rows 32 us (the first tile arrives 5 us after the launch, the tiles take
-// 15, storing and joining the parts 8), one token over 777 rows 7.9 us.
+// 15, storing and joining the parts 8), one token over 777 rows 7.2 us.
 //
 // Tried and slower, same 2 x 900 queries: a quarter / half of the exponentials as a polynomial
 // on the FMA units 943 / 1056 us (938 without), two threads per row and 16 softmax warps 1021
@@ -74,6 +76,17 @@ constexpr int kAttnThreads = 384;  // two softmax warpgroups; producer, issuer a
 constexpr int kSoftmaxRegs = 224, kOtherRegs = 56;
 constexpr int kColO = 256;  // tensor memory: S / P of the streams at 0 and 128, O at 256 and 384
 constexpr float kRaise = 8.f;
+constexpr int kMaxCluster = 8;  // parts that a cluster joins at most (the portable cluster size)
+
+// From a CTA of the cluster (cluster address).
+__device__ __forceinline__ float ld_cluster(uint32_t addr) {
+  float r;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(r) : "r"(addr) : "memory");
+  return r;
+}
+__device__ __forceinline__ void ld_cluster2(uint32_t addr, float* v) {
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v[0]), "=f"(v[1]) : "r"(addr) : "memory");
+}
 
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
@@ -154,12 +167,17 @@ __device__ __forceinline__ void tile_of(const AttnArgs& a, int item, int& grp, i
   }
 }
 
-// Work unit `index`; by a converged warp.
+// Work unit `index`; by a converged warp.  kCluster: a cluster's CTAs take an item's parts.
+template <bool kCluster>
 __device__ __forceinline__ Unit unit_of(const AttnArgs& a, int index) {
   Unit u;
   const int per_request = a.lq * a.group, lane = threadIdx.x & 31;
   int piece = 0, pieces = 1, item = index, grp, t;
-  if (index >= a.whole) {
+  if (kCluster) {
+    pieces = a.splits;
+    item = a.by_splits(index);
+    piece = index - item * pieces;
+  } else if (index >= a.whole) {
     // the parts of full row tiles first, then those of the groups' last tiles
     const int full = a.groups * (a.row_tiles - 1), cut = max(a.whole, full);
     const int j = index - a.whole, tail = cut - a.whole, last = j - tail * a.splits;
@@ -185,7 +203,7 @@ __device__ __forceinline__ Unit unit_of(const AttnArgs& a, int index) {
     u.b0 = a.by_request(u.row0);
     u.b1 = a.by_request(u.row0 + u.rows - 1);
   }
-  u.slot = pieces > 1 ? ((int64_t)(item - a.whole) * pieces + piece) * a.tile_rows : -1;
+  u.slot = !kCluster && pieces > 1 ? ((int64_t)(item - a.whole) * pieces + piece) * a.tile_rows : -1;
   int own = 0;
   if (a.own > 0)
     for (int b = u.b0 + lane; b <= u.b1; b += 32) own += own_tiles(a, u, b);
@@ -326,11 +344,32 @@ struct RowOut {
   }
 };
 
-template <typename T, int D, bool kAlone>
+// Result of a row (of the batch) of k/v head h, whose parts' results (weighted, o: elements
+// lane * D/32 on) add up to o and their weights, relative to 2^top, to sum; by a warp.
+template <typename T, int D>
+__device__ __forceinline__ void store_joined(const AttnArgs& a, int h, int row, const float* o, float sum, float top) {
+  constexpr int E = D / 32;
+  const int lane = threadIdx.x & 31, per_request = a.lq * a.group;
+  const int64_t hq = (int64_t)a.heads * a.group;
+  const int b = a.by_request(row), in = row - b * per_request, i = a.by_group(in), g = in - i * a.group;
+  const int64_t hh = (int64_t)h * a.group + g;
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  T* const at = reinterpret_cast<T*>(a.out) + (((int64_t)b * a.lq + i) * hq + hh) * D + lane * E;
+  uint32_t* const out = reinterpret_cast<uint32_t*>(at);
+#pragma unroll
+  for (int e = 0; e < E; e += 2) out[e / 2] = pack16<T>(o[e] * inv, o[e + 1] * inv);
+  if (lane == 0)
+    a.lse[(b * hq + hh) * a.lq + i] = sum == 0.f ? -INFINITY : (top + __log2f(sum)) * 0.6931471805599453f;
+}
+
+// kCluster: every unit is a part of a walk, each CTA has one, and a cluster's CTAs join
+// theirs through distributed shared memory.
+template <typename T, int D, bool kAlone, bool kCluster>
 __global__ void __launch_bounds__(kAttnThreads, 1)
     prefix_attn_kernel(const __grid_constant__ CUtensorMap map_kp, const __grid_constant__ CUtensorMap map_vp,
                        const __grid_constant__ CUtensorMap map_ko, const __grid_constant__ CUtensorMap map_vo,
                        const AttnArgs a) {
+  static_assert(kAlone || !kCluster, "the parts of a cluster have at most 128 rows");
   using S = AttnSmem<D, kAlone>;
   constexpr int kRing = S::kRing;
   constexpr int kBox = kTileKeys * 128;  // bytes of one 64-element-wide box
@@ -370,6 +409,13 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
   pdl_wait();  // lens, q, k and v may be the previous kernel's
   pdl_trigger();
 
+  // kCluster: this CTA's part, in place of the K and V that it is done with; rows are padded by
+  // 16 bytes, so that the threads of a warp, a row each, store to different banks
+  constexpr int kPartRow = D + 4;
+  static_assert(kTileRows * (kPartRow + 1) * 4 <= kRing * S::kTile, "a part fits into the ring");
+  float* const part = reinterpret_cast<float*>(gbase + S::kKV);
+  float* const part_lse = part + kTileRows * kPartRow;
+
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
     if (warp == 8) {
@@ -377,7 +423,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       int at = 0;  // loads so far
       bool ok = true, first_unit = true;
       for (int unit = blockIdx.x; unit < a.units; unit += gridDim.x) {
-        const Unit u = unit_of(a, unit);
+        const Unit u = unit_of<kCluster>(a, unit);
         const int n = u.last - u.first;
         if (n == 0) continue;
         const bool alternate = kAlone || u.rows <= kTileRows;
@@ -454,7 +500,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         p_phase[s] ^= 1u;
       };
       for (int unit = blockIdx.x; unit < a.units && ok; unit += gridDim.x) {
-        const Unit u = unit_of(a, unit);
+        const Unit u = unit_of<kCluster>(a, unit);
         const int n = u.last - u.first;
         if (n == 0) continue;
         wait(q_full, q_phase);
@@ -510,6 +556,11 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       __syncwarp();
       mbar_wait(done, 0, a.fault);
     }
+    if constexpr (kCluster) {
+      __syncwarp();
+      cluster_sync();
+      cluster_sync();
+    }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
     // ---------------- softmax: stream s, thread r owns a row (tensor-memory lane r)
@@ -527,15 +578,22 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       if (lane == 0) mbar_arrive(bar);
     };
     bool first_unit = true;
+    int part_h = 0, part_row0 = 0, part_rows = 0;  // kCluster: of the one unit
     int count = 0, at = 0, guards = 0, o_count[2] = {0, 0};
     for (int unit = blockIdx.x; unit < a.units; unit += gridDim.x) {
-      const Unit u = unit_of(a, unit);
+      const Unit u = unit_of<kCluster>(a, unit);
       const int n = u.last - u.first;
       const bool alternate = kAlone || u.rows <= kTileRows;
       const int row = alternate ? r : s * kTileRows + r;  // of the unit
       const bool live = row < u.rows;
+      if constexpr (kCluster) part_h = u.h, part_row0 = u.row0, part_rows = u.rows;
       if (n == 0) {  // nothing to see: an empty part
-        if (!alternate || s == 0) {
+        if constexpr (kCluster) {
+          if (s == 0) {
+            part_lse[r] = -INFINITY;
+            for (int c = 0; c < D; ++c) part[r * kPartRow + c] = 0.f;
+          }
+        } else if (!alternate || s == 0) {
           const RowOut<T, D> dst(a, u, row, live, true, 0.f, 0.f);
           const float zero[32] = {};
           for (int c = 0; c < D; c += 32) dst.store32(c, zero);
@@ -751,7 +809,8 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         const float top = fmaxf(m, other.x), shift = top == -INFINITY ? 0.f : top;
         float mine = ex2_approx(m - shift), theirs = ex2_approx(other.x - shift);
         const float sum = mine * l + theirs * other.y;
-        const RowOut<T, D> dst(a, u, row, live && ok, s == 0, shift, sum);
+        const RowOut<T, D> dst(a, u, row, !kCluster && live && ok, s == 0, shift, sum);
+        if (kCluster && s == 0 && ok) part_lse[r] = sum == 0.f ? -INFINITY : shift + __log2f(sum);
         const float inv = poisoned ? __int_as_float(0x7fffffff) : sum == 0.f ? 0.f : rcp_approx(sum);
         const float f0 = (s == 0 ? mine : theirs) * inv, f1 = (s == 0 ? theirs : mine) * inv;
         if (warp_live && ok) {
@@ -768,7 +827,13 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
 #pragma unroll
               for (int e = 0; e < 32; ++e) f[e] = sum == 0.f ? 0.f : fmaf(__uint_as_float(o[e]), f1, f[e]);
             }
-            dst.store32(c, f);
+            if constexpr (kCluster) {
+#pragma unroll
+              for (int e = 0; e < 32; e += 4)
+                *reinterpret_cast<float4*>(part + r * kPartRow + c + e) = make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]);
+            } else {
+              dst.store32(c, f);
+            }
           }
         }
       }
@@ -776,6 +841,38 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       at += 2 * n;
       ++o_count[0];
       if (!alternate || n > 1) ++o_count[1];
+    }
+    if constexpr (kCluster) {
+      __syncwarp();
+      cluster_sync();  // every part is there
+      // the cluster's warps take the rows in turn; parts are added in their order
+      constexpr int E = D / 32;
+      const uint32_t from = smem_u32(part), lse_from = smem_u32(part_lse);
+      for (int row = (int)cluster_rank() + a.splits * warp; row < part_rows; row += a.splits * (kSoftmaxThreads / 32)) {
+        const float lse = lane < a.splits ? ld_cluster(cluster_addr(lse_from + 4u * row, lane)) : -INFINITY;
+        float v[kMaxCluster][E];
+#pragma unroll
+        for (int p = 0; p < kMaxCluster; ++p)
+          if (p < a.splits) {
+            const uint32_t at = cluster_addr(from + 4u * (row * kPartRow + lane * E), p);
+#pragma unroll
+            for (int e = 0; e < E; e += 2) ld_cluster2(at + 4u * e, v[p] + e);
+          }
+        const float top = warp_max(lse), shift = top == -INFINITY ? 0.f : top;
+        const float wgt = ex2_approx(lse - shift);
+        float o[E] = {}, sum = 0.f;
+#pragma unroll
+        for (int p = 0; p < kMaxCluster; ++p)
+          if (p < a.splits) {
+            const float w = __shfl_sync(0xffffffffu, wgt, p);
+            sum += w;
+#pragma unroll
+            for (int e = 0; e < E; ++e) o[e] = fmaf(w, v[p][e], o[e]);
+          }
+        store_joined<T, D>(a, part_h, part_row0 + row, o, sum, top);
+      }
+      __syncwarp();
+      cluster_sync();  // no CTA leaves while another reads its part
     }
   }
   __syncthreads();
@@ -836,32 +933,69 @@ __global__ void __launch_bounds__(32 * kJoinWarps) prefix_attn_join_kernel(const
 #pragma unroll
     for (int e = 0; e < E; ++e) o[e] += sums[w][lane * E + e];
   }
-  const int64_t hq = (int64_t)a.heads * a.group;
-  const int b = a.by_request(row), in = row - b * per_request, i = a.by_group(in), g = in - i * a.group;
-  const int64_t hh = (int64_t)h * a.group + g;
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  uint32_t* out = reinterpret_cast<uint32_t*>(reinterpret_cast<T*>(a.out) + (((int64_t)b * a.lq + i) * hq + hh) * D + lane * E);
-#pragma unroll
-  for (int e = 0; e < E; e += 2) out[e / 2] = pack16<T>(o[e] * inv, o[e + 1] * inv);
-  if (lane == 0)
-    a.lse[(b * hq + hh) * a.lq + i] = sum == 0.f ? -INFINITY : (top + __log2f(sum)) * 0.6931471805599453f;
+  store_joined<T, D>(a, h, row, o, sum, top);
 }
 
 // ------------------------------------------------------------------ host side
 struct Plan {
   bool within_request;
   int64_t tile_rows, groups, row_tiles, items, whole, splits, units, rows, slots;
+  bool clustered;  // the parts of an item are the CTAs of a cluster
   double cost;  // key tiles that the longest-working SM walks, and what joining costs
 };
 
 // What a unit costs beside its tiles (finding it, Q, the pipeline's ends, the results) and
 // what joining costs, in steps of 128 keys and 256 rows.
-constexpr double kUnitTiles = 2.0, kJoinTiles = 1.0;
+constexpr double kUnitTiles = 2.0, kJoinTiles = 1.0, kClusterTiles = 0.7;
+// Rows that a cluster joins at most.  Its CTAs read each other's parts at a few bytes a cycle, where the
+// second kernel has a CTA for every row: with 32 rows 10.9 us per call in clusters and 13.1
+// without, with 64 12.9 and 12.7, with 128 16.0 and 14.9.
+constexpr int64_t kClusterRows = 32;
 // A step of a unit of up to 128 rows takes two tiles, which is as much to load as two steps.
 constexpr double kHalfStep = 0.6;
 
+// Clusters of 2..kMaxCluster CTAs of this kernel that the GPU holds at once: the SMs come in
+// groups that a cluster may not straddle, so a second round can start long before every SM has
+// a CTA (24 clusters of 6: 25 us, where 6 parts and the second kernel take 17).
+struct ClusterRoom {
+  int clusters[kMaxCluster + 1];
+};
+int cluster_room(const DeviceInfo* di, ClusterRoom* room) {
+  static std::atomic<uint64_t> known{0}, reserved{0};
+  static std::atomic<int> held[64][kMaxCluster + 1];
+  const uint64_t bit = 1ull << di->ordinal;
+  if (!(known.load(std::memory_order_acquire) & bit)) {
+    const auto kern = prefix_attn_kernel<__nv_bfloat16, 128, true, true>;
+    constexpr int smem = AttnSmem<128, true>::kBytes;
+    if (int s = reserve_smem((const void*)kern, smem, reserved, di, "shared_prefix_attention")) return s;
+    for (int n = 2; n <= kMaxCluster; ++n) {
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3((unsigned)n, 1, 1);
+      cfg.blockDim = dim3(kAttnThreads, 1, 1);
+      cfg.dynamicSmemBytes = smem;
+      cudaLaunchAttribute at[1];
+      at[0].id = cudaLaunchAttributeClusterDimension;
+      at[0].val.clusterDim.x = (unsigned)n;
+      at[0].val.clusterDim.y = 1;
+      at[0].val.clusterDim.z = 1;
+      cfg.attrs = at;
+      cfg.numAttrs = 1;
+      int count = 0;
+      if (cudaOccupancyMaxActiveClusters(&count, kern, &cfg) != cudaSuccess) {
+        cudaGetLastError();
+        count = 0;
+      }
+      held[di->ordinal][n].store(count, std::memory_order_relaxed);
+    }
+    known.fetch_or(bit, std::memory_order_acq_rel);
+  }
+  room->clusters[0] = room->clusters[1] = 0;
+  for (int n = 2; n <= kMaxCluster; ++n) room->clusters[n] = held[di->ordinal][n].load(std::memory_order_relaxed);
+  return JO_OK;
+}
+
 Plan make_plan(bool within_request, int64_t tile_rows, int64_t batch, int64_t lq, int64_t heads, int64_t group,
-               int64_t prefix, int64_t own, int64_t hold) {
+               int64_t prefix, int64_t own, int64_t hold, const ClusterRoom& room) {
   Plan p{};
   const int64_t per_request = lq * group;
   p.within_request = within_request;
@@ -890,7 +1024,10 @@ Plan make_plan(bool within_request, int64_t tile_rows, int64_t batch, int64_t lq
       const int64_t s = trial <= 16 ? trial : whole < p.items ? (trial - 16) * hold / (p.items - whole) : 1;
       if (s > most || s < 1 || (s > 1 && s > limit) || (s > 1 && whole == p.items)) continue;
       const int64_t cut = whole > full ? whole : full;
-      double cost = s > 1 ? kJoinTiles + 0.05 * (double)s : 0.;
+      // one unit of few rows to a CTA, in as many parts as a cluster may have CTAs
+      const bool clustered = (p.row_tiles > 1 ? tile_rows : last_rows) <= kClusterRows && tile_rows <= kTileRows &&
+                             whole == 0 && s > 1 && s <= kMaxCluster && p.items <= room.clusters[s];
+      double cost = clustered ? kClusterTiles : s > 1 ? kJoinTiles + 0.05 * (double)s : 0.;
       int64_t at = 0;
       auto add = [&](int64_t units, double tiles_each, double per_tile) {
         cost += (double)(cdiv(at + units, hold) - cdiv(at, hold)) * (tiles_each * per_tile + kUnitTiles);
@@ -905,23 +1042,24 @@ Plan make_plan(bool within_request, int64_t tile_rows, int64_t batch, int64_t lq
         p.cost = cost;
         p.whole = whole;
         p.splits = s;
+        p.clustered = clustered;
         any = true;
       }
     }
   if (p.splits == 1) p.whole = p.items;
   p.units = p.whole + (p.items - p.whole) * p.splits;
-  p.slots = (p.items - p.whole) * p.splits * tile_rows;
+  p.slots = p.clustered ? 0 : (p.items - p.whole) * p.splits * tile_rows;
   return p;
 }
 
 // `hold`: CTAs that the GPU holds at once (one per SM).
 Plan plan_attention(int64_t batch, int64_t lq, int64_t heads, int64_t group, int64_t prefix, int64_t own,
-                    int64_t hold) {
+                    int64_t hold, const ClusterRoom& room) {
   Plan best{};
   for (int64_t tile_rows : {(int64_t)kTileRows, (int64_t)kUnitRows})
     for (bool within : {true, false}) {
       if (!within && batch == 1) continue;
-      const Plan p = make_plan(within, tile_rows, batch, lq, heads, group, prefix, own, hold);
+      const Plan p = make_plan(within, tile_rows, batch, lq, heads, group, prefix, own, hold, room);
       if (best.units == 0 || p.cost < best.cost) best = p;
     }
   return best;
@@ -958,28 +1096,41 @@ int make_kv_map(const char* op, CUtensorMap* map, const void* ptr, int64_t d, in
   return JO_OK;
 }
 
-template <typename T, int D, bool kAlone>
+template <typename T, int D, bool kAlone, bool kCluster>
 int launch_units(const CUtensorMap* maps, const AttnArgs& a, cudaStream_t st, const DeviceInfo* di) {
   const char* op = "shared_prefix_attention";
-  auto kern = prefix_attn_kernel<T, D, kAlone>;
+  auto kern = prefix_attn_kernel<T, D, kAlone, kCluster>;
   constexpr int smem = AttnSmem<D, kAlone>::kBytes;
   static std::atomic<uint64_t> reserved{0};
   if (int s = reserve_smem((const void*)kern, smem, reserved, di, op)) return s;
-  if (cudaError_t e = launch_pdl(kern, dim3((unsigned)(a.units < di->sm_count ? a.units : di->sm_count)),
-                                 dim3(kAttnThreads), smem, st, maps[0], maps[1], maps[2], maps[3], a))
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(a.units < di->sm_count ? a.units : di->sm_count), 1, 1);
+  cfg.blockDim = dim3(kAttnThreads, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = (unsigned)a.splits;
+  at[1].val.clusterDim.y = 1;
+  at[1].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = kCluster ? 2 : 1;
+  if (cudaError_t e = cudaLaunchKernelEx(&cfg, kern, maps[0], maps[1], maps[2], maps[3], a))
     return launch_failed(e, op);
   return after_launch("prefix_attn_kernel");
 }
 
 template <typename T, int D>
 int launch_attention(const CUtensorMap* maps, const AttnArgs& a, const Plan& p, cudaStream_t st, const DeviceInfo* di) {
-  const char* op = "shared_prefix_attention";
-  if (int s = p.tile_rows <= kTileRows ? launch_units<T, D, true>(maps, a, st, di)
-                                       : launch_units<T, D, false>(maps, a, st, di))
+  if (p.clustered) return launch_units<T, D, true, true>(maps, a, st, di);
+  if (int s = p.tile_rows <= kTileRows ? launch_units<T, D, true, false>(maps, a, st, di)
+                                       : launch_units<T, D, false, false>(maps, a, st, di))
     return s;
   if (const int64_t joined = (p.items - p.whole) * p.tile_rows) {
     if (cudaError_t e = launch_pdl(prefix_attn_join_kernel<T, D>, dim3((unsigned)joined), dim3(32 * kJoinWarps), 0, st, a))
-      return launch_failed(e, op);
+      return launch_failed(e, "shared_prefix_attention");
     return after_launch("prefix_attn_join_kernel");
   }
   return JO_OK;
@@ -998,7 +1149,9 @@ int64_t jo_shared_prefix_attention_workspace(int64_t batch, int64_t q_len, int64
   if (device_info(&di)) return -1;
   if (check_sizes("shared_prefix_attention", batch, q_len, q_heads, kv_heads, head_dim, prefix_len, own_len)) return -1;
   if (batch == 0 || q_len == 0) return 0;
-  const Plan p = plan_attention(batch, q_len, kv_heads, q_heads / kv_heads, prefix_len, own_len, di->sm_count);
+  ClusterRoom room;
+  if (cluster_room(di, &room)) return -1;
+  const Plan p = plan_attention(batch, q_len, kv_heads, q_heads / kv_heads, prefix_len, own_len, di->sm_count, room);
   return p.slots * (head_dim + 1) * 4;
 }
 
@@ -1034,7 +1187,9 @@ int jo_shared_prefix_attention(void* out, float* lse, const void* q, int64_t q_s
   for (const auto& u : used)
     if (u.size > 1 && (u.stride % 8 || u.stride < 0))
       return fail(JO_ERR_ALIGN, "%s: strides must be multiples of 16 bytes and not negative", op);
-  const Plan p = plan_attention(batch, q_len, kv_heads, q_heads / kv_heads, prefix_len, own_len, di->sm_count);
+  ClusterRoom room;
+  if (int s = cluster_room(di, &room)) return s;
+  const Plan p = plan_attention(batch, q_len, kv_heads, q_heads / kv_heads, prefix_len, own_len, di->sm_count, room);
   if (p.units > INT32_MAX / 2 || (p.items - p.whole) * p.tile_rows > INT32_MAX)
     return fail(JO_ERR_SHAPE, "%s: size too large", op);
   if (p.slots && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 31) ||

@@ -402,6 +402,28 @@ def test_attention(jo, dev, causal, dtype, b, n, hk, g, d, p, s):
     check_attention(jo, *x, causal)
 
 
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("b,n,hk,g", [(1, 1, 1, 1), (4, 1, 3, 2), (2, 3, 1, 5), (1, 8, 2, 4), (1, 11, 1, 3), (3, 1, 24, 1)])
+def test_attention_in_every_number_of_parts(jo, dev, d, b, n, hk, g):
+    # up to 32 rows and more, walks of 4 to 40 tiles, and a request without rows of its own
+    for p in (512, 700, 1024, 1281, 1500, 1793, 2100, 2305, 5000):
+        x = inputs(dev, b, n, hk, g, d, p, 200, BF, p)
+        x[-1][0] = 0
+        spoil(x[-1], x[3], x[4])
+        out, lse = check_attention(jo, *x, True)
+        again = jo.shared_prefix_attention(*x, True)
+        assert torch.equal(out, again[0]) and torch.equal(lse, again[1])
+
+
+def test_attention_parts_without_keys(jo, dev):
+    # the walk is split for full caches, but its requests are short or empty: parts that see nothing
+    for lens in ([0, 0], [1, 0], [0, 130], [2000, 3]):
+        x = inputs(dev, 2, 1, 2, 2, 128, 0, 2000, F16, 1)
+        x[-1][:] = torch.tensor(lens, device=dev, dtype=torch.int32)
+        spoil(x[-1], x[3], x[4])
+        check_attention(jo, *x, True)
+
+
 @pytest.mark.parametrize("causal", [True, False])
 def test_attention_of_nothing(jo, dev, causal):
     q, kp, vp, ko, vo, lens = inputs(dev, 4, 3, 2, 2, 64, 0, 50, BF, 1)
