@@ -27,11 +27,12 @@
 // stays converged 169 (a lone lane took 40 cycles per scale copy and more per product),
 // results by TMA 140.  Walking the tiles in bands of 4, 8 or 16 rows, four stages instead of
 // five, and evict-first stores changed nothing.  1350 x 3072 x 12288 (blocks of 32): 24 us.
-// Few rows: the weight's bytes, and a fixed 4 us: one row x 9216 x 3072 5.1 us, 6.7 with the
-// quantisation of the row; 128 rows 10.7.
+// Few rows: the weight's bytes, and a fixed 4 us: one row x 9216 x 3072 5.1 us, 6.6 with the
+// quantisation of the row, which each CTA does for itself while the weight comes in (7.9 with
+// a kernel before); 128 rows 10.7.
 //
 // Every mbarrier wait is bounded (pipeline.cuh), as in the FP8 product.
-#include "fp4.cuh"
+#include "fp4_quant.cuh"
 #include "tcgen05.cuh"
 
 namespace jo {
@@ -121,6 +122,9 @@ struct Fp4GemmArgs {
   int m, n, k;
   int tiles_m, tiles_n;
   bool b_ready;  // B was complete before the previous kernel of the stream began
+  const void* x;  // rows that the product's kernel quantises itself (null: A is given in 4 bits)
+  int64_t ldx;
+  int x_align;  // bytes that every run's address is a multiple of (Run::load)
   unsigned int* fault;
 };
 
@@ -424,25 +428,111 @@ struct RowsSmem {
   static constexpr int kOffSA = kOffSB + kStages * F::kScale;
   static constexpr int kOffPart = kOffSA + kStages * F::kScale;
   static constexpr int kBars = kOffPart + kPart;
-  static constexpr int kBytes = kBars + 256 + 1024;
+  static constexpr int kRowScale = kBars + 256;        // kFused: per epilogue warp, 16 row scales
+  static constexpr int kRowMax = kRowScale + 4 * 64;   // and of each row the four warps' maxima
+  static constexpr int kBytes = kRowMax + 4 * 64 + 1024;
+  static_assert(kBytes <= 227 * 1024, "shared memory");
   static_assert(kCols / kMaxSplit >= 2, "every CTA of a cluster has columns to add up");
   static constexpr int kTmem = kCols + 64 <= 128 ? 128 : 256;  // accumulator, two stages of scales
 };
 
 // `count` consecutive rows of A at column n of D: a warp writes 64 contiguous bytes per row.
+// row_scale: A's in shared memory, or null.
 template <typename OutT, int kCount>
-__device__ __forceinline__ void store_column(const Fp4GemmArgs& g, const float* v, int m0, int n, float s_b,
-                                             float bias) {
+__device__ __forceinline__ void store_column(const Fp4GemmArgs& g, const float* row_scale, const float* v, int m0,
+                                             int n, float s_b, float bias) {
   float s_a[kCount];
 #pragma unroll
-  for (int e = 0; e < kCount; ++e) s_a[e] = g.sa && m0 + e < g.m ? __ldg(g.sa + m0 + e) : 1.f;
+  for (int e = 0; e < kCount; ++e)
+    s_a[e] = m0 + e >= g.m ? 1.f : row_scale ? row_scale[m0 + e] : g.sa ? __ldg(g.sa + m0 + e) : 1.f;
   OutT* d = reinterpret_cast<OutT*>(g.d) + (int64_t)m0 * g.ldd + n;
 #pragma unroll
   for (int e = 0; e < kCount; ++e)
     if (m0 + e < g.m) d[e * g.ldd] = Elt<OutT>::from_f(v[e] * s_b * s_a[e] + bias);
 }
 
-template <typename OutT, bool kMx, int kCols>
+// quant_fp4 of this CTA's part of K of x, into A's place in every stage, by the epilogue's
+// warps; each CTA finds the maxima of whole rows for itself (a row of 3072 is 6 KB out of L2).
+// Rows past the last stay as they are: they reach only their own columns of the accumulator.
+// Loads go out in batches of four runs: a row at a time costs its latency, 1.1 us, per row.
+template <typename T, bool kMx, typename S>
+__device__ __forceinline__ void quantise_part(const Fp4GemmArgs& g, uint8_t* gbase, int kb0, int kb1) {
+  constexpr int kThreads = 128, kBatch = 4, kRuns = kKElems / 16;  // runs of a stage
+  const int t = threadIdx.x - (kRowsThreads - kThreads), w = t >> 5, lane = t & 31, runs = g.k / 16;
+  const T* const x = reinterpret_cast<const T*>(g.x);
+  float* const row_scale = reinterpret_cast<float*>(gbase + S::kRowScale) + w * 16;
+  uint32_t top_row = 0;  // of row `lane`
+  float rs_row = 0.f;
+  if constexpr (!kMx) {
+    uint32_t* const row_max = reinterpret_cast<uint32_t*>(gbase + S::kRowMax);
+    const int share = g.m == 1 ? 4 : g.m == 2 ? 2 : 1;  // warps to a row
+    for (int m = w / share; m < g.m; m += 4 / share) {
+      uint32_t top = 0;
+      for (int u0 = (w % share) * 32 + lane; u0 < runs; u0 += 32 * share * kBatch) {
+        Run<T> run[kBatch];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+          const int u = u0 + i * 32 * share;
+          if (u < runs)
+            run[i].load(x + m * g.ldx + (int64_t)u * 16, g.x_align);
+          else
+            run[i].clear();
+        }
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) top = max(top, run[i].amax_bits());
+      }
+      top = __reduce_max_sync(0xffffffffu, top);
+      if (lane == 0) row_max[m * 4 + w % share] = top;
+    }
+    asm volatile("bar.sync 1, 128;" ::: "memory");
+    if (lane < g.m) {
+      for (int i = 0; i < share; ++i) top_row = max(top_row, row_max[lane * 4 + i]);
+      rs_row = fp4_row_scale(top_row);
+      row_scale[lane] = top_row >= 0x7f800000u ? __int_as_float(0x7fffffff) : rs_row;
+    }
+  }
+  const int part = (kb1 - kb0) * kRuns, all = g.m * part;
+  for (int i0 = t; i0 - t < all; i0 += kThreads * kBatch) {
+    Run<T> run[kBatch];
+    int row[kBatch], at[kBatch];  // row (g.m: none) and run of this CTA's part
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      row[i] = min(i0 + i * kThreads, all) / max(part, 1);
+      at[i] = i0 + i * kThreads - row[i] * part;
+      if (row[i] < g.m && kb0 * kRuns + at[i] < runs)
+        run[i].load(x + row[i] * g.ldx + (int64_t)(kb0 * kRuns + at[i]) * 16, g.x_align);
+      else
+        run[i].clear();
+    }
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      if (i0 - t + i * kThreads >= all) break;  // the same for all threads
+      uint32_t top = run[i].amax_bits(), code;
+      float rs = 0.f, rc = 0.f;
+      bool bad = false;
+      if constexpr (kMx) {
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      } else {
+        const int from = min(row[i], g.m - 1);
+        bad = __shfl_sync(0xffffffffu, top_row, from) >= 0x7f800000u;
+        rs = __shfl_sync(0xffffffffu, rs_row, from);
+        rc = __frcp_rn(rs);
+      }
+      const uint2 c = run_to_fp4<T, kMx>(run[i], top, bad, rs, rc, code);
+      if (row[i] < g.m) {
+        // 128-byte swizzle; scales: the tile's order (fp4.cuh), the row being one of the first 32
+        const int stage = at[i] / kRuns, j = at[i] % kRuns, b = kMx ? j >> 1 : j;
+        *reinterpret_cast<uint2*>(gbase + S::kOffA + stage * S::kA + row[i] * kKBytes +
+                                  (((j >> 1) ^ (row[i] & 7)) << 4) + (j & 1) * 8) = c;
+        if (!kMx || (j & 1) == 0)
+          gbase[S::kOffSA + stage * S::F::kScale + (b >> 2) * kChunk + row[i] * 16 + (b & 3)] = (uint8_t)code;
+      }
+    }
+  }
+}
+
+// kFused: A's rows come in 16 bits and are quantised here; K's parts fit into the ring.
+template <typename OutT, bool kMx, int kCols, bool kFused>
 __global__ void __launch_bounds__(kRowsThreads, 1)
     fp4_gemm_rows_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                          const __grid_constant__ CUtensorMap map_sa, const __grid_constant__ CUtensorMap map_sb,
@@ -451,6 +541,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
   using F = Fmt<kMx>;
   constexpr int kStages = S::kStages;
   static_assert(kStages >= 3, "ring too short");
+  static_assert(!kFused || kCols == 16, "row scales for 16 rows");
   unsigned int* const fault = args.fault;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_base = smem_u32(smem_raw);
@@ -460,7 +551,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
   auto full_bar = [&](int s) { return bars + 8u * s; };
   auto empty_bar = [&](int s) { return bars + 8u * (kStages + s); };
   const uint32_t tfull = bars + 8u * (2 * kStages);
-  const uint32_t tmem_slot = tfull + 8;
+  const uint32_t tmem_slot = tfull + 8, a_ready = tfull + 16;
 
   const int warp = warp_index(), lane = threadIdx.x & 31;
   const int rank = split > 1 ? (int)cluster_rank() : 0;
@@ -474,6 +565,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
       mbar_init(empty_bar(s), 1);
     }
     mbar_init(tfull, 1);
+    if constexpr (kFused) mbar_init(a_ready, 4);  // one arrival per quantising warp
     mbar_init_fence();
   }
   if (warp == 1) tmem_alloc(tmem_slot, S::kTmem);
@@ -482,7 +574,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
   tc_fence_after();
   const uint32_t tmem = *reinterpret_cast<uint32_t*>(gbase + (tmem_slot - base));
   auto load_b = [&](int stage, int kb) {
-    mbar_expect_tx(full_bar(stage), S::kStage);
+    mbar_expect_tx(full_bar(stage), kFused ? S::kB + F::kScale : S::kStage);
     tma_load_2d(base + S::kOffB + stage * S::kB, &map_b, kb * kKBytes, tn * 128, full_bar(stage));
     tma_load_3d(base + S::kOffSB + stage * F::kScale, &map_sb, 0, kb * F::kTiles, tn, full_bar(stage));
   };
@@ -502,8 +594,10 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
           if (!mbar_wait(empty_bar(stage), phase ^ 1u, fault)) break;
           load_b(stage, kb);
         }
-        tma_load_2d(base + S::kOffA + stage * S::kA, &map_a, kb * kKBytes, tm * kCols, full_bar(stage));
-        tma_load_3d(base + S::kOffSA + stage * F::kScale, &map_sa, 0, kb * F::kTiles, tm, full_bar(stage));
+        if constexpr (!kFused) {
+          tma_load_2d(base + S::kOffA + stage * S::kA, &map_a, kb * kKBytes, tm * kCols, full_bar(stage));
+          tma_load_3d(base + S::kOffSA + stage * F::kScale, &map_sa, 0, kb * F::kTiles, tm, full_bar(stage));
+        }
         ++issued;
         if (++stage == kStages) stage = 0, phase ^= 1u;
       }
@@ -515,7 +609,8 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
     const uint64_t sbd = scale_desc(base + S::kOffSB), sad = scale_desc(base + S::kOffSA);
     int stage = 0;
     uint32_t phase = 0;
-    for (int kb = kb0; kb < kb1; ++kb) {
+    const bool ready = !kFused || __all_sync(0xffffffffu, mbar_wait(a_ready, 0, fault));
+    for (int kb = kb0; kb < kb1 && ready; ++kb) {
       if (!__all_sync(0xffffffffu, mbar_wait(full_bar(stage), phase, fault))) break;
       tc_fence_after();
       if (elect_one()) {
@@ -538,6 +633,14 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
     const bool live = n < args.n;
     const float s_b = live && args.sb ? __ldg(args.sb + n) : 1.f;
     const float bias = live && args.bias ? Elt<OutT>::to_f(reinterpret_cast<const OutT*>(args.bias)[n]) : 0.f;
+    const float* row_scale = nullptr;
+    if constexpr (kFused) {
+      quantise_part<OutT, kMx, S>(args, gbase, kb0, kb1);
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(a_ready);
+      if (!kMx) row_scale = reinterpret_cast<const float*>(gbase + S::kRowScale) + (warp - 2) * 16;
+    }
     const bool ok = mbar_wait(tfull, 0, fault);
     tc_fence_after();
     // each CTA of the cluster adds up kCols / split of the columns (both powers of two)
@@ -557,7 +660,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
         float v[16];
 #pragma unroll
         for (int e = 0; e < 16; ++e) v[e] = __uint_as_float(r[e]);
-        if (live) store_column<OutT, 16>(args, v, tm * kCols + c, n, s_b, bias);
+        if (live) store_column<OutT, 16>(args, row_scale, v, tm * kCols + c, n, s_b, bias);
       } else {
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
@@ -577,7 +680,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
         for (int r = 0; r < split; ++r)
 #pragma unroll
           for (int e = 0; e < kCount; ++e) v[e] += from[((r << shift) + c + e) * 128];
-        if (live) store_column<OutT, kCount>(args, v, tm * kCols + rank * share + c, n, s_b, bias);
+        if (live) store_column<OutT, kCount>(args, row_scale, v, tm * kCols + rank * share + c, n, s_b, bias);
       };
       if (share >= 8)
         for (int c = 0; c < share; c += 8) sums(std::integral_constant<int, 8>{}, c);
@@ -650,9 +753,11 @@ template <bool kMx>
 int make_maps(CUtensorMap* maps, const Operands& o, const Fp4GemmArgs& g, int rows_a, int rows_b, int groups_b) {
   using F = Fmt<kMx>;
   const int64_t tk = fp4_tiles_k(g.k, kMx ? JO_FP4_MX : JO_FP4_NV);
-  if (int s = make_code_map(&maps[0], o.a, g.m, g.k / 2, o.lda, rows_a)) return s;
+  if (g.x == nullptr) {  // else A is not read
+    if (int s = make_code_map(&maps[0], o.a, g.m, g.k / 2, o.lda, rows_a)) return s;
+    if (int s = make_scale_map(&maps[2], o.block_a, cdiv(g.m, 128), tk, F::kTiles, 1)) return s;
+  }
   if (int s = make_code_map(&maps[1], o.b, g.n, g.k / 2, o.ldb, rows_b)) return s;
-  if (int s = make_scale_map(&maps[2], o.block_a, cdiv(g.m, 128), tk, F::kTiles, 1)) return s;
   return make_scale_map(&maps[3], o.block_b, cdiv(g.n, 128), tk, F::kTiles, groups_b);
 }
 
@@ -700,11 +805,19 @@ int launch_pair(const Operands& o, Fp4GemmArgs g, cudaStream_t st, const DeviceI
   return after_launch("fp4_gemm_pair_kernel");
 }
 
-template <typename OutT, bool kMx, int kCols>
+// K in as many parts as still leave two stages each, until every SM has a CTA.
+int rows_split(int64_t tiles, int64_t k, int sm_count) {
+  const int64_t kblocks = cdiv(k, kKElems);
+  int split = 1;
+  while (split < kMaxSplit && tiles * split * 2 <= sm_count && kblocks >= split * 4) split *= 2;
+  return split;
+}
+
+template <typename OutT, bool kMx, int kCols, bool kFused>
 int launch_rows(const Operands& o, Fp4GemmArgs g, cudaStream_t st, const DeviceInfo* di) {
   const char* op = "fp4_scaled_mm";
   using S = RowsSmem<kMx, kCols>;
-  auto kern = fp4_gemm_rows_kernel<OutT, kMx, kCols>;
+  auto kern = fp4_gemm_rows_kernel<OutT, kMx, kCols, kFused>;
   static std::atomic<uint64_t> reserved{0};
   if (int s = reserve_smem((const void*)kern, S::kBytes, reserved, di, op)) return s;
   g.tiles_m = (int)cdiv(g.m, kCols);
@@ -712,11 +825,8 @@ int launch_rows(const Operands& o, Fp4GemmArgs g, cudaStream_t st, const DeviceI
   if (kCols < 128 && g.tiles_m > 1) return fail(JO_ERR_SHAPE, "%s: %d rows in a tile of %d", op, g.m, kCols);
   if (g.tiles_m > 65535 || (int64_t)g.tiles_n * kMaxSplit > INT32_MAX)
     return fail(JO_ERR_SHAPE, "%s: too many tiles", op);
-  // K in as many parts as still leave two stages each, until every SM has a CTA
-  const int64_t tiles = (int64_t)g.tiles_m * g.tiles_n, kblocks = cdiv(g.k, kKElems);
-  int split = 1;
-  while (split < kMaxSplit && tiles * split * 2 <= di->sm_count && kblocks >= split * 4) split *= 2;
-  CUtensorMap maps[4];
+  const int split = rows_split((int64_t)g.tiles_m * g.tiles_n, g.k, di->sm_count);
+  CUtensorMap maps[4] = {};
   if (int s = make_maps<kMx>(maps, o, g, kCols, 128, 1)) return s;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(g.tiles_n * split), (unsigned)g.tiles_m, 1);
@@ -745,10 +855,11 @@ int dispatch(const Operands& o, const Fp4GemmArgs& g, cudaStream_t st, const Dev
   // 11.7 / 10.6; 1350 x 3072 x 3072 (all, 72 of 74 pairs) 12.3 / 20.9.
   const int64_t pair_tiles = cdiv(g.m, kPairM) * cdiv(g.n, kPairN);
   if (g.m > 128 && pair_tiles * 2 * 2 >= di->sm_count) return launch_pair<OutT, kMx>(o, g, st, di);
-  if (g.m <= 16) return launch_rows<OutT, kMx, 16>(o, g, st, di);
-  if (g.m <= 32) return launch_rows<OutT, kMx, 32>(o, g, st, di);
-  if (g.m <= 64) return launch_rows<OutT, kMx, 64>(o, g, st, di);
-  return launch_rows<OutT, kMx, 128>(o, g, st, di);
+  if (g.x) return launch_rows<OutT, kMx, 16, true>(o, g, st, di);
+  if (g.m <= 16) return launch_rows<OutT, kMx, 16, false>(o, g, st, di);
+  if (g.m <= 32) return launch_rows<OutT, kMx, 32, false>(o, g, st, di);
+  if (g.m <= 64) return launch_rows<OutT, kMx, 64, false>(o, g, st, di);
+  return launch_rows<OutT, kMx, 128, false>(o, g, st, di);
 }
 
 }  // namespace
@@ -759,7 +870,7 @@ namespace {
 
 int fp4_mm(const char* op, void* d, int64_t ldd, const Operands& o, const float* scale_a, const float* scale_b,
            const void* bias, int64_t m, int64_t n, int64_t k, int format, int out_dtype, bool b_ready,
-           cudaStream_t st) {
+           const void* x, int64_t ldx, cudaStream_t st) {
   const DeviceInfo* di;
   if (int s = device_info(&di)) return s;
   if (format != JO_FP4_NV && format != JO_FP4_MX)
@@ -788,11 +899,26 @@ int fp4_mm(const char* op, void* d, int64_t ldd, const Operands& o, const float*
   g.n = (int)n;
   g.k = (int)k;
   g.b_ready = b_ready;
+  g.x = x;
+  g.ldx = ldx;
+  const uint64_t at = reinterpret_cast<uintptr_t>(x) | (uint64_t)(m > 1 ? ldx * 2 : 0);
+  g.x_align = at % 32 == 0 ? 32 : at % 16 == 0 ? 16 : 2;
   g.fault = di->fault;
   const bool mx = format == JO_FP4_MX;
   if (out_dtype == JO_BF16)
     return mx ? dispatch<__nv_bfloat16, true>(o, g, st, di) : dispatch<__nv_bfloat16, false>(o, g, st, di);
   return mx ? dispatch<__half, true>(o, g, st, di) : dispatch<__half, false>(o, g, st, di);
+}
+
+// Whether the product's kernel quantises x itself: where each part of K fits into the ring, for
+// few rows, as every CTA does it again and the wait for the weight hides only so much.  us
+// per call (and on the GPU), 9216 x 3072, one kernel / two, JO_FP4_NV: 1 row 8.0 / 9.4 (6.6 /
+// 7.9), 4 rows 8.5 / 9.4 (8.3 / 7.9), 8 rows 10.5 / 9.3; JO_FP4_MX: 1 row 7.1 / 9.3 (5.8 /
+// 7.8), 8 rows 7.1 / 9.2 (7.0 / 8.0), 16 rows 8.6 / 9.4 (8.6 / 8.0).
+int64_t most_fused_rows(int format) { return format == JO_FP4_MX ? 8 : 4; }
+bool quantises_itself(int64_t n, int64_t k, int format, int sm_count) {
+  const int stages = format == JO_FP4_MX ? RowsSmem<true, 16>::kStages : RowsSmem<false, 16>::kStages;
+  return cdiv(cdiv(k, kKElems), rows_split(cdiv(n, 128), k, sm_count)) <= stages;
 }
 
 // fp4_linear's workspace: codes, block scales and row scales of x, each from 512 bytes on.
@@ -818,7 +944,7 @@ int jo_fp4_scaled_mm(void* d, int64_t ldd, const void* a, int64_t lda, const voi
                      const void* block_a, const void* block_b, const float* scale_a, const float* scale_b,
                      const void* bias, int64_t m, int64_t n, int64_t k, int format, int out_dtype, void* stream) {
   return fp4_mm("fp4_scaled_mm", d, ldd, Operands{a, b, block_a, block_b, lda, ldb}, scale_a, scale_b, bias, m, n, k,
-                format, out_dtype, false, (cudaStream_t)stream);
+                format, out_dtype, false, nullptr, 0, (cudaStream_t)stream);
 }
 
 int64_t jo_fp4_linear_workspace(int64_t m, int64_t k, int format) {
@@ -840,10 +966,20 @@ int jo_fp4_linear(void* d, int64_t ldd, const void* x, int64_t x_row_stride, con
   const LinearWork w = linear_work(m, k, format);
   uint8_t* const q = (uint8_t*)workspace;
   float* const rows = format == JO_FP4_NV ? reinterpret_cast<float*>(q + w.rows) : nullptr;
+  const DeviceInfo* di = nullptr;
+  if (m <= most_fused_rows(format))
+    if (int s = device_info(&di)) return s;
+  if (di && quantises_itself(n, k, format, di->sm_count)) {
+    if (!x) return fail(JO_ERR_INVALID, "%s: null operand", op);
+    if (m > 1 && x_row_stride < k) return fail(JO_ERR_SHAPE, "%s: row stride smaller than the row", op);
+    if (reinterpret_cast<uintptr_t>(x) % 2) return fail(JO_ERR_ALIGN, "%s: x must be aligned to its elements", op);
+    return fp4_mm(op, d, ldd, Operands{q, b, q + w.scales, block_b, k / 2, ldb}, nullptr, scale_b, bias, m, n, k,
+                  format, dtype, false, x, x_row_stride, (cudaStream_t)stream);
+  }
   if (int s = jo_quant_fp4(q, k / 2, q + w.scales, rows, x, x_row_stride, m, k, format, dtype, stream)) return s;
   // the quantisation releases the product's launch only once everything before it is complete
   return fp4_mm(op, d, ldd, Operands{q, b, q + w.scales, block_b, k / 2, ldb}, rows, scale_b, bias, m, n, k, format,
-                dtype, true, (cudaStream_t)stream);
+                dtype, true, nullptr, 0, (cudaStream_t)stream);
 }
 
 }  // extern "C"

@@ -208,6 +208,24 @@ def test_linear_is_quantisation_and_product(jo, dev, dtype, fmt, m):
     assert torch.equal(jo.fp4_linear(x, *w, add), jo.fp4_scaled_mm(a[0], w[0], a[1], w[1], a[2], w[2], dtype, add))
 
 
+@pytest.mark.parametrize("dtype", [BF, F16])
+@pytest.mark.parametrize("fmt", ["nvfp4", "mxfp4"])
+@pytest.mark.parametrize("n,k", [(520, 32), (136, 288), (264, 2080), (1032, 4096), (9600, 3072), (72, 16384), (8, 20000)])
+def test_linear_of_few_rows(jo, dev, dtype, fmt, n, k):
+    g = gen(dev, n)
+    w, add = held(jo, normal(g, dev, n, k), fmt)[0], normal(g, dev, n).to(dtype)
+    for m in (1, 2, 3, 4, 5, 8, 9, 16):
+        for shift in (0, 1, 8):  # rows on 32 bytes, on their elements, on 16 bytes
+            x = normal(g, dev, m, k + 16 + shift).to(dtype)[:, shift:shift + k]
+            if m > 2:  # the smallest values, a row of zeros, and rows with an infinity or a NaN
+                x[0] *= 2.0 ** -14
+                x[1] = 0
+                x[2, k - 1] = math.nan if shift else math.inf
+            a = jo.quant_fp4(x, fmt)
+            want = jo.fp4_scaled_mm(a[0], w[0], a[1], w[1], a[2], w[2], dtype, add)
+            torch.testing.assert_close(jo.fp4_linear(x, *w, add), want, rtol=0, atol=0, equal_nan=True)
+
+
 def test_no_rows(jo, dev):
     x = torch.empty(0, 64, device=dev, dtype=BF)
     q, block, row = jo.quant_fp4(x)
