@@ -414,19 +414,20 @@ __global__ void __launch_bounds__(kPairThreads, 1)
 constexpr int kRowsThreads = 192;
 constexpr int kMaxSplit = 8;
 
-template <bool kMx, int kCols>
+// kFused: A's part of K lies beside the ring, which then holds the weight alone.
+template <bool kMx, int kCols, bool kFused>
 struct RowsSmem {
   using F = Fmt<kMx>;
   static constexpr int kB = 128 * kKBytes;    // the weight's codes
   static constexpr int kA = kCols * kKBytes;  // kCols rows of A
-  static constexpr int kStage = kB + kA + 2 * F::kScale;
+  static constexpr int kStage = kFused ? kB + F::kScale : kB + kA + 2 * F::kScale;
   static constexpr int kPart = 128 * kCols * 4;  // received parts
-  static constexpr int kStages = (int)((227 * 1024 - 2048 - kPart) / kStage) < 8
-                                     ? (int)((227 * 1024 - 2048 - kPart) / kStage)
-                                     : 8;
-  static constexpr int kOffB = 0, kOffA = kStages * kB, kOffSB = kOffA + kStages * kA;
+  static constexpr int kRoom = 227 * 1024 - 2048 - kPart;
+  static constexpr int kStages = kFused ? 6 : kRoom / kStage < 8 ? kRoom / kStage : 8;
+  static constexpr int kAStages = kFused ? (kRoom - kStages * kStage) / (kA + F::kScale) : kStages;
+  static constexpr int kOffB = 0, kOffA = kStages * kB, kOffSB = kOffA + kAStages * kA;
   static constexpr int kOffSA = kOffSB + kStages * F::kScale;
-  static constexpr int kOffPart = kOffSA + kStages * F::kScale;
+  static constexpr int kOffPart = kOffSA + kAStages * F::kScale;
   static constexpr int kBars = kOffPart + kPart;
   static constexpr int kRowScale = kBars + 256;        // kFused: per epilogue warp, 16 row scales
   static constexpr int kRowMax = kRowScale + 4 * 64;   // and of each row the four warps' maxima
@@ -451,7 +452,7 @@ __device__ __forceinline__ void store_column(const Fp4GemmArgs& g, const float* 
     if (m0 + e < g.m) d[e * g.ldd] = Elt<OutT>::from_f(v[e] * s_b * s_a[e] + bias);
 }
 
-// quant_fp4 of this CTA's part of K of x, into A's place in every stage, by the epilogue's
+// quant_fp4 of this CTA's part of K of x, into the place of A's codes and scales, by the epilogue's
 // warps; each CTA finds the maxima of whole rows for itself (a row of 3072 is 6 KB out of L2).
 // Rows past the last stay as they are: they reach only their own columns of the accumulator.
 // Loads go out in batches of four runs: a row at a time costs its latency, 1.1 us, per row.
@@ -531,13 +532,13 @@ __device__ __forceinline__ void quantise_part(const Fp4GemmArgs& g, uint8_t* gba
   }
 }
 
-// kFused: A's rows come in 16 bits and are quantised here; K's parts fit into the ring.
+// kFused: A's rows come in 16 bits and are quantised here; K's parts fit into kAStages.
 template <typename OutT, bool kMx, int kCols, bool kFused>
 __global__ void __launch_bounds__(kRowsThreads, 1)
     fp4_gemm_rows_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                          const __grid_constant__ CUtensorMap map_sa, const __grid_constant__ CUtensorMap map_sb,
                          const Fp4GemmArgs args, const int split) {
-  using S = RowsSmem<kMx, kCols>;
+  using S = RowsSmem<kMx, kCols, kFused>;
   using F = Fmt<kMx>;
   constexpr int kStages = S::kStages;
   static_assert(kStages >= 3, "ring too short");
@@ -574,7 +575,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
   tc_fence_after();
   const uint32_t tmem = *reinterpret_cast<uint32_t*>(gbase + (tmem_slot - base));
   auto load_b = [&](int stage, int kb) {
-    mbar_expect_tx(full_bar(stage), kFused ? S::kB + F::kScale : S::kStage);
+    mbar_expect_tx(full_bar(stage), S::kStage);
     tma_load_2d(base + S::kOffB + stage * S::kB, &map_b, kb * kKBytes, tn * 128, full_bar(stage));
     tma_load_3d(base + S::kOffSB + stage * F::kScale, &map_sb, 0, kb * F::kTiles, tn, full_bar(stage));
   };
@@ -614,9 +615,10 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
       if (!__all_sync(0xffffffffu, mbar_wait(full_bar(stage), phase, fault))) break;
       tc_fence_after();
       if (elect_one()) {
+        const int at = kFused ? kb - kb0 : stage;
         stage_products<false, kMx, 128, kCols, 1>(
-            tmem, bd + stage * (S::kB >> 4), ad + stage * (S::kA >> 4), sbd + stage * (F::kScale >> 4),
-            sad + stage * (F::kScale >> 4), tmem + kCols + ((kb - kb0) & 1) * 2 * F::kCols, steps_of(args.k, kb),
+            tmem, bd + stage * (S::kB >> 4), ad + at * (S::kA >> 4), sbd + stage * (F::kScale >> 4),
+            sad + at * (F::kScale >> 4), tmem + kCols + ((kb - kb0) & 1) * 2 * F::kCols, steps_of(args.k, kb),
             kb == kb0);
         tc_commit(empty_bar(stage));
       }
@@ -816,7 +818,7 @@ int rows_split(int64_t tiles, int64_t k, int sm_count) {
 template <typename OutT, bool kMx, int kCols, bool kFused>
 int launch_rows(const Operands& o, Fp4GemmArgs g, cudaStream_t st, const DeviceInfo* di) {
   const char* op = "fp4_scaled_mm";
-  using S = RowsSmem<kMx, kCols>;
+  using S = RowsSmem<kMx, kCols, kFused>;
   auto kern = fp4_gemm_rows_kernel<OutT, kMx, kCols, kFused>;
   static std::atomic<uint64_t> reserved{0};
   if (int s = reserve_smem((const void*)kern, S::kBytes, reserved, di, op)) return s;
@@ -910,15 +912,25 @@ int fp4_mm(const char* op, void* d, int64_t ldd, const Operands& o, const float*
   return mx ? dispatch<__half, true>(o, g, st, di) : dispatch<__half, false>(o, g, st, di);
 }
 
-// Whether the product's kernel quantises x itself: where each part of K fits into the ring, for
-// few rows, as every CTA does it again and the wait for the weight hides only so much.  us
-// per call (and on the GPU), 9216 x 3072, one kernel / two, JO_FP4_NV: 1 row 8.0 / 9.4 (6.6 /
-// 7.9), 4 rows 8.5 / 9.4 (8.3 / 7.9), 8 rows 10.5 / 9.3; JO_FP4_MX: 1 row 7.1 / 9.3 (5.8 /
-// 7.8), 8 rows 7.1 / 9.2 (7.0 / 8.0), 16 rows 8.6 / 9.4 (8.6 / 8.0).
-int64_t most_fused_rows(int format) { return format == JO_FP4_MX ? 8 : 4; }
-bool quantises_itself(int64_t n, int64_t k, int format, int sm_count) {
-  const int stages = format == JO_FP4_MX ? RowsSmem<true, 16>::kStages : RowsSmem<false, 16>::kStages;
-  return cdiv(cdiv(k, kKElems), rows_split(cdiv(n, 128), k, sm_count)) <= stages;
+// Whether the product's kernel quantises x itself: where each part of K fits beside the ring,
+// and the runs of 16 that each of a CTA's 128 threads goes through are few: m K / 2048 over
+// the parts of K, and for the maxima of whole rows (JO_FP4_NV) as many as a third of m K /
+// 2048, once for every tile of the SM.  us per call (and on the GPU), one kernel / two:
+//   JO_FP4_NV  9216 x 3072   1 row (1.2) 8.2 / 9.4 (6.7 / 7.8), 4 rows (4.8) 8.5 / 9.4 (8.3 / 7.7),
+//                            8 rows (9.6) 10.5 / 9.3 (10.4 / 8.0)
+//              12288 x 3072  2 rows (3.9) 8.9 / 9.2 (8.1 / 8.6), 4 rows (7.8) 10.7 / 9.3 (10.2 / 8.7)
+//   JO_FP4_MX  9216 x 3072   1 row (0.8) 7.1 / 9.3 (5.8 / 7.8), 8 rows (6) 7.2 / 9.3 (6.9 / 8.0),
+//                            16 rows (12) 8.6 / 9.4 (8.6 / 8.0)
+//              28672 x 4096  2 rows (8) 16.1 / 18.5 (15.7 / 18.3), 4 rows (16) 18.7 / 18.6 (18.4 / 17.7)
+constexpr int64_t kMostFused = 16;  // rows
+bool quantises_itself(int64_t m, int64_t n, int64_t k, int format, int sm_count) {
+  const bool mx = format == JO_FP4_MX;
+  const int64_t tiles = cdiv(n, 128);
+  const int split = rows_split(tiles, k, sm_count);
+  if (cdiv(cdiv(k, kKElems), split) > (mx ? RowsSmem<true, 16, true>::kAStages : RowsSmem<false, 16, true>::kAStages))
+    return false;
+  const double runs = (double)(cdiv(tiles * split, sm_count) * m * k) / 2048.;
+  return m <= kMostFused && (mx ? runs / split <= 8. : runs * (0.3 + 1. / split) <= 5.);
 }
 
 // fp4_linear's workspace: codes, block scales and row scales of x, each from 512 bytes on.
@@ -967,9 +979,9 @@ int jo_fp4_linear(void* d, int64_t ldd, const void* x, int64_t x_row_stride, con
   uint8_t* const q = (uint8_t*)workspace;
   float* const rows = format == JO_FP4_NV ? reinterpret_cast<float*>(q + w.rows) : nullptr;
   const DeviceInfo* di = nullptr;
-  if (m <= most_fused_rows(format))
+  if (m <= kMostFused)
     if (int s = device_info(&di)) return s;
-  if (di && quantises_itself(n, k, format, di->sm_count)) {
+  if (di && quantises_itself(m, n, k, format, di->sm_count)) {
     if (!x) return fail(JO_ERR_INVALID, "%s: null operand", op);
     if (m > 1 && x_row_stride < k) return fail(JO_ERR_SHAPE, "%s: row stride smaller than the row", op);
     if (reinterpret_cast<uintptr_t>(x) % 2) return fail(JO_ERR_ALIGN, "%s: x must be aligned to its elements", op);

@@ -210,7 +210,8 @@ def test_linear_is_quantisation_and_product(jo, dev, dtype, fmt, m):
 
 @pytest.mark.parametrize("dtype", [BF, F16])
 @pytest.mark.parametrize("fmt", ["nvfp4", "mxfp4"])
-@pytest.mark.parametrize("n,k", [(520, 32), (136, 288), (264, 2080), (1032, 4096), (9600, 3072), (72, 16384), (8, 20000)])
+@pytest.mark.parametrize("n,k", [(520, 32), (136, 288), (264, 2080), (1032, 4096), (9600, 3072), (72, 16384), (8, 20000), (3072, 12288),
+                                 (20000, 1024)])
 def test_linear_of_few_rows(jo, dev, dtype, fmt, n, k):
     g = gen(dev, n)
     w, add = held(jo, normal(g, dev, n, k), fmt)[0], normal(g, dev, n).to(dtype)
