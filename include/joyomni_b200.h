@@ -446,9 +446,10 @@ JO_API int jo_fp4_scaled_mm(void* d, int64_t ldd, const void* a, int64_t lda, co
 
 /* A Linear layer in 4 bits: jo_quant_fp4 of x [M, K] (F16/BF16) in the weight's format
  * into the workspace, then jo_fp4_scaled_mm with the weight b [N, K] (packed codes, its
- * block scales and row scales); D and bias of x's dtype.  Two kernels: the product's
- * starts loading the weight while the quantisation runs, so nothing else may be writing
- * the weight by then but work that was queued on `stream` before this call.
+ * block scales and row scales); D and bias of x's dtype.  Few rows are quantised inside the
+ * product's kernel; else the product starts loading the weight while the quantisation runs,
+ * so nothing else may be writing the weight by then but work that was queued on `stream`
+ * before this call.
  * workspace: 16-byte aligned, jo_fp4_linear_workspace(m, k, format) bytes (-1: bad
  * arguments). */
 JO_API int64_t jo_fp4_linear_workspace(int64_t m, int64_t k, int format);
