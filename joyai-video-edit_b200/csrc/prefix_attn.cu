@@ -385,6 +385,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
   auto p_full = [&](int s, int half) { return q_full + 24u + 16u * half + 8u * s; };
   auto o_full = [&](int s) { return q_full + 56u + 8u * s; };
   const uint32_t done = q_full + 72u, tmem_slot = q_full + 80u;
+  auto guarded_by_0 = [&](int i) { return q_full + 88u + 8u * i; };
   const int warp = warp_index(), lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
@@ -399,6 +400,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       mbar_init(p_full(s, 0), kTileRows / 32);  // one arrival per warp
       mbar_init(p_full(s, 1), kTileRows / 32);
       mbar_init(o_full(s), 1);
+      mbar_init(guarded_by_0(s), kTileRows / 32);
     }
     mbar_init_fence();
   }
@@ -579,7 +581,8 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     };
     bool first_unit = true;
     int part_h = 0, part_row0 = 0, part_rows = 0;  // kCluster: of the one unit
-    int count = 0, at = 0, guards = 0, o_count[2] = {0, 0};
+    int count = 0, at = 0, o_count[2] = {0, 0};
+    int guards = 0, shared_guards = 0;  // guarded tiles so far: a stream's own, and those that both use
     for (int unit = blockIdx.x; unit < a.units; unit += gridDim.x) {
       const Unit u = unit_of<kCluster>(a, unit);
       const int n = u.last - u.first;
@@ -659,7 +662,8 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
           const int len = own_len(a, w.b);
           const bool guarded = u.b0 != u.b1 || key0 + kTileKeys > seen_by_all;
           const bool ends = len < a.own && key0 + kTileKeys > len;
-          int* const first_bad = reinterpret_cast<int*>(gbase + S::kGuard) + (guards & 1) * 8 + (alternate ? s * 4 : 0);
+          const int turn = alternate ? guards & 1 : shared_guards & 1;
+          int* const first_bad = reinterpret_cast<int*>(gbase + S::kGuard) + turn * 8 + (alternate ? s * 4 : 0);
           if ((guarded || ends) && (alternate || s == 0)) {
             const int idx = at + v_index(alternate, alternate ? 2 * t + s : t, n), slot = idx % kRing;
             wait(full(slot), idx / kRing);
@@ -686,16 +690,27 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
             }
           }
           if (guarded) {
-            if (!alternate && s == 0) asm volatile("bar.arrive 4, 256;" ::: "memory");
-            if (s == 0)
-              asm volatile("bar.sync 2, 128;" ::: "memory");
-            else if (alternate)
-              asm volatile("bar.sync 3, 128;" ::: "memory");
-            else  // what stream 0 found
-              asm volatile("bar.sync 4, 256;" ::: "memory");
+            // Stream 1 takes what stream 0 found in a tile that both use.  Stream 0 goes on without
+            // waiting for it and may be one such tile ahead, not two: S(t + 2) of stream 0 is
+            // issued after O += P V of stream 1's tile t, whose P comes after this.  So two barriers
+            // in turn do, and waits that are bounded as all others.
+            if (alternate) {
+              if (s == 0)
+                asm volatile("bar.sync 2, 128;" ::: "memory");
+              else
+                asm volatile("bar.sync 3, 128;" ::: "memory");
+              ++guards;
+            } else {
+              if (s == 0) {
+                arrive_warp(guarded_by_0(turn));
+                asm volatile("bar.sync 2, 128;" ::: "memory");
+              } else {
+                wait(guarded_by_0(turn), shared_guards >> 1);
+              }
+              ++shared_guards;
+            }
             const int low = min(min(first_bad[0], first_bad[1]), min(first_bad[2], first_bad[3]));
             poisoned = poisoned || low < limit;
-            ++guards;
           }
         }
         if (!ok) {

@@ -140,3 +140,26 @@ def shared_prefix_attention(q, k_prefix, v_prefix, k_own, v_own, lens, causal=Tr
             out[r, i] = torch.einsum("hk,khd->hd", w, v)
             mass[r, i] = torch.einsum("hk,khd->hd", w, v.abs())
     return out, lse, mass
+
+
+def shared_prefix_attention_by_request(q, k_prefix, v_prefix, k_own, v_own, lens, causal=True, scale=None):
+    """``shared_prefix_attention`` with a request's queries all at once, for sizes at which one by one takes too long."""
+    b, n, h, d = q.shape
+    hk, p = k_prefix.shape[1], k_prefix.shape[0]
+    scale = d ** -0.5 if scale is None else scale
+    out = torch.zeros(b, n, hk, h // hk, d, dtype=torch.float64, device=q.device)
+    mass = torch.zeros_like(out)
+    lse = torch.full((b, hk, h // hk, n), -math.inf, dtype=torch.float64, device=q.device)
+    i = torch.arange(n, device=q.device)[:, None]
+    for r, length in enumerate(torch.as_tensor(lens).clamp(0, k_own.shape[1]).tolist()):
+        k, v = (torch.cat((a, o[r, :length])).double() for a, o in ((k_prefix, k_own), (v_prefix, v_own)))
+        if p + length == 0:
+            continue
+        x = torch.einsum("nhgd,khd->hgnk", q[r].double().view(n, hk, -1, d), k) * scale
+        if causal:
+            j = torch.arange(p + length, device=q.device) - p
+            x = x.masked_fill((j >= 0) & (j > length - n + i), -math.inf)
+        lse[r] = torch.logsumexp(x, 3)
+        w = torch.exp(x - torch.where(torch.isneginf(lse[r]), 0.0, lse[r])[..., None])
+        out[r], mass[r] = torch.einsum("hgnk,khd->nhgd", w, v), torch.einsum("hgnk,khd->nhgd", w, v.abs())
+    return out.view(b, n, h, d), lse.view(b, h, n), mass.view(b, n, h, d)

@@ -91,3 +91,18 @@ def test_oracle_attention_is_softmax():
     x = x.masked_fill(torch.ones(5, 5).triu(1).bool(), -math.inf)
     assert torch.allclose(o[0], torch.einsum("hnm,mhd->nhd", x.softmax(-1), v[0].double()), atol=1e-6)
     assert torch.allclose(lse[0], x.logsumexp(-1), atol=1e-6)
+
+
+@pytest.mark.parametrize("causal", [True, False])
+def test_oracle_attention_by_request(causal):
+    g = torch.Generator().manual_seed(3)
+    q = torch.randn(5, 4, 6, 8, generator=g)
+    kp, vp = (torch.randn(7, 2, 8, generator=g) for _ in range(2))
+    ko, vo = (torch.randn(5, 9, 2, 8, generator=g) for _ in range(2))
+    lens = [9, 2, 0, 4, 20]
+    for r, n in enumerate(lens):
+        ko[r, n:], vo[r, n:] = math.nan, math.inf
+    for p in (7, 0):
+        x = q, kp[:p], vp[:p], ko, vo, lens, causal
+        for one, all_ in zip(ref.shared_prefix_attention(*x), ref.shared_prefix_attention_by_request(*x)):
+            assert torch.allclose(one, all_, rtol=1e-12, atol=1e-12)
