@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from oracle import prefix as ref
-from test_prefix_gpu import BF, F16, ROUND, inputs, spoil, within
+from test_prefix_gpu import BF, F16, F32, ROUND, check_product, check_quant, gen, inputs, normal, spoil, within
 
 pytestmark = pytest.mark.gpu
 
@@ -50,3 +50,60 @@ def test_attention_of_units_with_idle_requests(jo, dev, d, b, n, hk, g, p, s):
         spoil(x[5], x[3], x[4])
         check_attention(jo, *x, True)
     no_faults()
+
+
+# Every way in which walks of 256-row units are cut: none, all of them, only the last units'; requests that a unit
+# straddles, and several units to a request; last row tiles of more and of fewer than 128 rows.
+SHARED = [
+    (2, 130, 40, 2, 0, 60), (40, 130, 2, 2, 0, 60), (2, 130, 40, 1, 150, 60),                  # whole
+    (20, 7, 24, 1, 0, 60), (20, 3, 8, 8, 700, 60), (40, 40, 3, 1, 700, 60),                    # all in parts
+    (1, 130, 40, 1, 130, 600), (5, 130, 3, 4, 130, 600), (1, 300, 8, 4, 130, 600),
+    (40, 40, 24, 1, 0, 60), (100, 130, 3, 1, 130, 60), (2, 300, 16, 4, 130, 300), (5, 40, 40, 4, 130, 300),  # the last
+]
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("dtype,d", [(BF, 128), (F16, 64)])
+@pytest.mark.parametrize("b,n,hk,g,p,s", SHARED)
+def test_attention_of_shared_units(jo, dev, causal, dtype, d, b, n, hk, g, p, s):
+    x = inputs(dev, b, n, hk, g, d, p, s, dtype, seed=b + n + p)
+    x[5][0] = s
+    if b > 2:
+        x[5][1], x[5][2] = 0, 1
+    spoil(x[5], x[3], x[4])
+    check_attention(jo, *x, causal)
+    no_faults()
+
+
+@pytest.mark.parametrize("dtype,d", [(F16, 128), (BF, 64)])
+@pytest.mark.parametrize("b,n,hk,g,p,s", [(40, 40, 3, 1, 700, 60), (5, 130, 3, 4, 130, 600), (2, 300, 16, 4, 130, 300)])
+def test_attention_of_shared_units_keeps_a_bad_value_to_the_rows_that_see_it(jo, dev, dtype, d, b, n, hk, g, p, s):
+    q, kp, vp, ko, vo, lens = inputs(dev, b, n, hk, g, d, p, s, dtype, seed=3)
+    lens[:] = s
+    clean = jo.shared_prefix_attention(q, kp, vp, ko, vo, lens, True)
+    at = s - n // 2  # of request 1; its queries from n - n // 2 on see it
+    vo[1, at, 0, 5] = math.inf
+    vo[1, at + 3, 1] = math.nan
+    out, lse = jo.shared_prefix_attention(q, kp, vp, ko, vo, lens, True)
+    first = n - n // 2
+    sees = torch.zeros(b, n, hk * g, dtype=torch.bool, device=dev)
+    sees[1, first:, :g], sees[1, first + 3:, g:2 * g] = True, True
+    assert torch.equal(out[~sees], clean[0][~sees]) and torch.equal(lse, clean[1])
+    assert not torch.isfinite(out[1, first:, :g, 5]).any() and torch.isnan(out[1, first + 3:, g:2 * g]).all()
+    no_faults()
+
+
+# More tiles than the GPU holds CTA pairs (74): the second accumulator, and the ring's state from tile to tile.
+@pytest.mark.parametrize("fmt", ["nvfp4", "mxfp4"])
+@pytest.mark.parametrize("out", [BF, F16])
+@pytest.mark.parametrize("m,n,k", [(2600, 2568, 288), (4000, 4008, 64), (2300, 2560, 2080), (5400, 3080, 32), (257, 20488, 1568)])
+def test_product_of_several_tiles_per_pair(jo, dev, fmt, out, m, n, k):
+    check_product(jo, dev, m, n, k, fmt, out, bias=m % 200 == 0)
+    no_faults()
+
+
+@pytest.mark.parametrize("fmt", ["nvfp4", "mxfp4"])
+@pytest.mark.parametrize("dtype", [BF, F16, F32])
+@pytest.mark.parametrize("m,k", [(400, 12288), (250, 20480)])  # four and (16 bits) six runs per lane
+def test_quant_of_long_rows(jo, dev, fmt, dtype, m, k):
+    check_quant(jo, normal(gen(dev, k), dev, m, k).to(dtype), fmt)
