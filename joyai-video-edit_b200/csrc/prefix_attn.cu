@@ -44,8 +44,13 @@
 // Warp 9: tcgen05.mma issuer: S = Q K^T (both operands in shared memory), O += P V with P
 //   from tensor memory and V as it lies ([keys, D], the MN-major operand).
 //
-// P is rounded to q's 16-bit type for the tensor cores, a relative 2^-8 at most for bf16 as
-// the output's own rounding, whose errors average out over the keys; l sums the unrounded p.
+// P is rounded to q's 16-bit type for the tensor cores, whose errors average out over the keys; l
+// sums the unrounded p.  bf16: a relative 2^-8 at most, as the output's own rounding.  fp16:
+// 2^-11, but below 2^-14 an absolute 2^-25, and p under that vanishes, which does not
+// average out (43200 keys 26 bits below one more would lose their 6e-4 of the weight).  So
+// fp16 has p = 2^(s_j c - m + 7): at most 2^15 with m raised as above (the format ends at
+// 65504), and n keys lose less than n 2^-32 of a weight whose sum is at least 1.  l carries
+// the same 2^7, and the log-sum-exp takes it back.
 //
 // Bound and measured (B200; us per call, calls in a row).  Many queries: the chain of one
 // stream, S -> softmax -> P V -> S, whose softmax (S in 300 cycles, maximum 150-300,
@@ -76,6 +81,8 @@ constexpr int kAttnThreads = 384;  // two softmax warpgroups; producer, issuer a
 constexpr int kSoftmaxRegs = 224, kOtherRegs = 56;
 constexpr int kColO = 256;  // tensor memory: S / P of the streams at 0 and 128, O at 256 and 384
 constexpr float kRaise = 8.f;
+template <typename T>
+constexpr float kBias = std::is_same<T, __half>::value ? 7.f : 0.f;  // of p's exponent
 constexpr int kMaxCluster = 8;  // parts that a cluster joins at most (the portable cluster size)
 
 // From a CTA of the cluster (cluster address).
@@ -763,7 +770,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
               tmem_st16(t_o + c, o);
             }
           }
-          const float shift = m == -INFINITY ? 0.f : m;
+          const float shift = m == -INFINITY ? 0.f : m - kBias<T>;
           const float2 scale2 = make_float2(a.scale_log2, a.scale_log2), shift2 = make_float2(-shift, -shift);
           float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
@@ -794,6 +801,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         w.next(a, u);
         if (alternate) w.next(a, u);
       }
+      m -= kBias<T>;  // l and O are in these units
       if (steps > 0) wait(o_full(s), o_count[s]);
       if (!alternate) {
         tc_fence_after();

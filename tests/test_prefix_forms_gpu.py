@@ -107,3 +107,22 @@ def test_product_of_several_tiles_per_pair(jo, dev, fmt, out, m, n, k):
 @pytest.mark.parametrize("m,k", [(400, 12288), (250, 20480)])  # four and (16 bits) six runs per lane
 def test_quant_of_long_rows(jo, dev, fmt, dtype, m, k):
     check_quant(jo, normal(gen(dev, k), dev, m, k).to(dtype), fmt)
+
+
+# One key 26 bits above 43200 equal ones, which have 6.4e-4 of the weight between them.  Bound in fp16: every weight is
+# rounded, a relative 2^-11 and an absolute 2^-32 of a sum of at least 1 (the kernel keeps weights up to 2^15).
+@pytest.mark.parametrize("dtype", [BF, F16])
+@pytest.mark.parametrize("n,hk,place", [(1, 2, 0), (256, 74, 0), (256, 74, 43199), (128, 74, 20000)])
+def test_attention_weights_far_below_the_largest_keep_their_share(jo, dev, dtype, n, hk, place):
+    p = 43200
+    k, v = torch.zeros(p, hk, 64, device=dev, dtype=dtype), torch.ones(p, hk, 64, device=dev, dtype=dtype)
+    k[place, :, 0], v[place] = 26 * math.log(2), 0
+    q = torch.zeros(1, n, hk, 64, device=dev, dtype=dtype)
+    q[..., 0] = 1
+    own = torch.zeros(1, 8, hk, 64, device=dev, dtype=dtype)
+    lens = torch.zeros(1, device=dev, dtype=torch.int32)
+    out, lse = jo.shared_prefix_attention(q, k, v, own, own, lens, True, 1.0)
+    want, wlse, mass = ref.shared_prefix_attention_by_request(q[:, :1], k, v, own, own, lens, True, 1.0)
+    u = ROUND[dtype]
+    within(out, want.expand_as(out), u * want.abs() + (u + 2.0 ** -16) * mass + p * 2.0 ** -32, "out")
+    within(lse, wlse.expand_as(lse), 2.0 ** -20 * (1 + 2 * wlse.abs()), "lse")
