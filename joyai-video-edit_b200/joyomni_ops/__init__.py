@@ -24,6 +24,7 @@ import os
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 _here = os.path.dirname(__file__)
 _so = glob.glob(os.path.join(_here, "_C*.so"))
@@ -481,22 +482,53 @@ class _RotaryEmbed(torch.autograd.Function):
     """The rotation or its inverse, each the other's gradient; the tables and positions have none."""
 
     @staticmethod
-    def forward(ctx, q, k, cos, sin, positions, interleaved, inverse):
-        ctx.save_for_backward(cos, sin, positions)
-        ctx.form = interleaved, inverse
+    def forward(q, k, cos, sin, positions, interleaved, inverse):
         qo, ko = _ops.rotary_embed(q, k, cos, sin, positions, interleaved, inverse)
         return qo, ko if k is not None else None
 
     @staticmethod
+    def setup_context(ctx, inputs, output):
+        _, k, cos, sin, positions, interleaved, inverse = inputs
+        ctx.save_for_backward(cos, sin, positions)
+        ctx.form = interleaved, inverse, k is not None
+
+    @staticmethod
     def backward(ctx, dq, dk):
-        interleaved, inverse = ctx.form
-        # the gradient of a sum or a mean comes as one expanded value
-        dq, dk = (g if g is None or g.stride(-1) == 1 else g.contiguous() for g in (dq, dk))
-        dq, dk = _rotate(dq, dk, *ctx.saved_tensors, interleaved, not inverse)
+        interleaved, inverse, has_k = ctx.form
+        dq, dk = _rotate(_rows(dq), _rows(dk) if has_k else None, *ctx.saved_tensors, interleaved, not inverse)
         return dq, dk, None, None, None, None, None
 
 
+class _RotaryEmbedForward(_RotaryEmbed):
+    """The same with forward derivatives, for dual tensors and torch.func (torch.compile takes no function that has them)."""
+
+    generate_vmap_rule = True
+
+    @staticmethod
+    def setup_context(ctx, inputs, output):
+        _RotaryEmbed.setup_context(ctx, inputs, output)
+        ctx.save_for_forward(*inputs[2:5])
+
+    @staticmethod
+    def jvp(ctx, dq, dk, *_):
+        interleaved, inverse, has_k = ctx.form
+        # linear: the tangents turn as the values do
+        return _rotate(_rows(dq), _rows(dk) if has_k else None, *ctx.saved_tensors, interleaved, inverse)
+
+
+def _rows(g):
+    """g with contiguous rows (the gradient of a sum or a mean comes as one expanded value)."""
+    return g if g.stride(-1) == 1 else g.contiguous()
+
+
+def _is_dual(x) -> bool:
+    return x is not None and forward_ad.unpack_dual(x).tangent is not None
+
+
 def _rotate(q, k, cos, sin, positions, interleaved, inverse):
+    # the cheap conditions first: outside a dual level (-1) there are no dual tensors
+    if torch._C._are_functorch_transforms_active() or forward_ad._current_level >= 0 and (_is_dual(q) or _is_dual(k)):
+        return _RotaryEmbedForward.apply(q, k, cos, sin, positions, interleaved, inverse)
     if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
         return _RotaryEmbed.apply(q, k, cos, sin, positions, interleaved, inverse)
     qo, ko = _ops.rotary_embed(q, k, cos, sin, positions, interleaved, inverse)
@@ -507,7 +539,7 @@ def rotary_embed(q, k, cos, sin, positions, interleaved=False):
     """Rotary position embedding of q [T, H, D] and k [T, HK, D] (or None): the tables' rows cos/sin (fp32
     [P, R/2]) at positions (int [T]) rotate the first R elements of each head, in pairs (2i, 2i+1) if
     interleaved, else (i, i + R/2); the other elements are copied.  fp32 math, one rounding.  Differentiable
-    in q and k.  A position outside the tables gives NaN.  Returns (q, k) (k None if it was)."""
+    in q and k, backward and forward, not in the tables.  A position outside the tables gives NaN.  Returns (q, k) (k None if it was)."""
     return _rotate(q, k, cos, sin, positions, interleaved, False)
 
 

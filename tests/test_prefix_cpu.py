@@ -106,3 +106,46 @@ def test_oracle_attention_by_request(causal):
         x = q, kp[:p], vp[:p], ko, vo, lens, causal
         for one, all_ in zip(ref.shared_prefix_attention(*x), ref.shared_prefix_attention_by_request(*x)):
             assert torch.allclose(one, all_, rtol=1e-12, atol=1e-12)
+
+
+def test_rotary_derivatives(jo):
+    """Forward and backward derivatives, alone and through torch.func, over a stand-in for the kernel."""
+    import torch.autograd.forward_ad as fw
+
+    g = torch.Generator().manual_seed(4)
+    rnd = lambda *s: torch.randn(s, generator=g, dtype=torch.float64)
+    q, k, dq, dk = rnd(6, 3, 16), rnd(6, 1, 16), rnd(6, 3, 16), rnd(6, 1, 16)
+    cos, sin, at = rnd(9, 6), rnd(9, 6), torch.arange(6) + 2
+    f = lambda x: jo.rotary_embed(x, None, cos, sin, at)[0]
+    both = lambda x, y: jo.rotary_embed(x, y, cos, sin, at)
+    want, back = ref.rotary(dq, cos, sin, at, False), ref.rotary(dq, cos, sin, at, False, True)
+    same = lambda x, y: torch.allclose(x, y, rtol=1e-12, atol=1e-12)
+
+    def turn(q, k, cos, sin, positions, interleaved, inverse):
+        assert q.stride(-1) == 1 and (k is None or k.stride(-1) == 1)
+        r = lambda x: ref.rotary(x, cos, sin, positions, interleaved, inverse)
+        return r(q), q.new_empty(0) if k is None else r(k)
+
+    with torch.library._scoped_library("joyomni_ops", "IMPL") as lib:
+        lib.impl("rotary_embed", turn, "CPU")
+        for enabled in (True, False):
+            with torch.set_grad_enabled(enabled), fw.dual_level():
+                o, p = both(fw.make_dual(q, dq), fw.make_dual(k, dk))
+                assert same(fw.unpack_dual(o).tangent, want)
+                assert same(fw.unpack_dual(p).tangent, ref.rotary(dk, cos, sin, at, False))
+                o, p = both(fw.make_dual(q, dq), k)
+                assert same(fw.unpack_dual(o).tangent, want) and not fw.unpack_dual(p).tangent.any()
+                assert same(fw.unpack_dual(f(fw.make_dual(q, dq))).tangent, want)
+        assert same(torch.func.jvp(f, (q,), (dq,))[1], want)
+        assert same(torch.func.grad(lambda x: (f(x) * dq).sum())(q), back)
+        assert torch.func.grad(lambda x: f(x).sum())(q).shape == q.shape
+        assert same(torch.func.jacfwd(f)(q), torch.func.jacrev(f)(q))
+        assert same(torch.func.vmap(torch.func.grad(lambda x: (f(x) * dq).sum()))(rnd(4, 6, 3, 16))[1], back)
+        assert same(torch.func.vmap(both)(rnd(2, 6, 3, 16), torch.stack((dk, k)))[1][0], ref.rotary(dk, cos, sin, at, False))
+        a, b = q.clone().requires_grad_(), k.clone().requires_grad_()
+        assert torch.autograd.gradcheck(both, (a, b), check_forward_ad=True)
+        assert torch.autograd.gradgradcheck(f, (a,), check_fwd_over_rev=True)
+        for x in (q, a):  # compiled, without and with a gradient
+            o, _ = torch.compile(lambda y: both(y, k), backend="eager", fullgraph=True)(x)
+            assert same(o, ref.rotary(q, cos, sin, at, False)) and o.requires_grad == x.requires_grad
+        assert same(torch.autograd.grad(o, a, dq)[0], back)

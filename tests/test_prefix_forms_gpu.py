@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from oracle import prefix as ref
-from test_prefix_gpu import BF, F16, F32, ROUND, check_product, check_quant, gen, inputs, normal, spoil, within
+from test_prefix_gpu import BF, F16, F32, ROUND, check_product, check_quant, check_rotary, gen, inputs, normal, spoil, tables, within
 
 pytestmark = pytest.mark.gpu
 
@@ -126,3 +126,23 @@ def test_attention_weights_far_below_the_largest_keep_their_share(jo, dev, dtype
     u = ROUND[dtype]
     within(out, want.expand_as(out), u * want.abs() + (u + 2.0 ** -16) * mass + p * 2.0 ** -32, "out")
     within(lse, wlse.expand_as(lse), 2.0 ** -20 * (1 + 2 * wlse.abs()), "lse")
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("interleaved", [True, False])
+def test_rotary_forward_derivative(jo, dev, dtype, interleaved):
+    import torch.autograd.forward_ad as fw
+
+    g = gen(dev, 11)
+    q, k, dq, dk = (normal(g, dev, 6, h, 64).to(dtype) for h in (3, 1, 3, 1))
+    cos, sin = tables(dev, 9, 48)
+    at = torch.arange(6, device=dev)
+    with fw.dual_level():
+        out = jo.rotary_embed(fw.make_dual(q, dq), fw.make_dual(k, dk), cos, sin, at, interleaved)
+        for o, x, t in zip(out, (q, k), (dq, dk)):
+            value, tangent = fw.unpack_dual(o)
+            check_rotary(value, x, cos, sin, at, interleaved)
+            check_rotary(tangent, t, cos, sin, at, interleaved)
+    f = lambda x: jo.rotary_embed(x, None, cos, sin, at, interleaved)[0]
+    check_rotary(torch.func.jvp(f, (q,), (dq,))[1], dq, cos, sin, at, interleaved)
+    check_rotary(torch.func.grad(lambda x: (f(x) * dq).sum())(q), dq, cos, sin, at, interleaved, inverse=True)
