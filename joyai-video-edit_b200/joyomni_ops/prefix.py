@@ -49,7 +49,7 @@ class PrefixCache:
     k_own: torch.Tensor     # [B, S, HK, D], contiguous
     v_own: torch.Tensor
     lens: torch.Tensor      # int32 [B], rows of each request
-    filled: int = 0         # the most rows that any request has, as the host knows it
+    filled: int = 0         # what the host knows of lens: no request has more rows (step keeps it)
 
     @classmethod
     def allocate(cls, k_prefix: torch.Tensor, v_prefix: torch.Tensor, batch: int, rows: int) -> "PrefixCache":
@@ -71,17 +71,21 @@ class PrefixAttention:
 
 
 def step(layer: PrefixAttention, x: torch.Tensor, cache: PrefixCache, cos: torch.Tensor, sin: torch.Tensor,
-         counts: Optional[torch.Tensor] = None) -> torch.Tensor:
+         counts: Optional[torch.Tensor] = None, most: Optional[int] = None) -> torch.Tensor:
     """L new tokens of each request through the layer: x [B, L, hidden] -> [B, L, hidden]; the cache grows.
 
     Token i of request b stands at position P + lens[b] + i of the tables (``rope.rotary_tables``).  counts
     (int32 [B], at most L): how many of the L tokens request b really has, the last counts[b] of its rows; the
-    padding in front of them is not cached and its outputs mean nothing.
+    padding in front of them is not cached and its outputs mean nothing.  most: the largest of counts, which the host
+    cannot see in them (L if not given); the cache's room is reckoned by it.
     """
     b, n, hidden = x.shape
     rows = cache.k_own.shape[1]
-    if cache.filled + n > rows:
-        raise ValueError(f"the cache holds {rows} rows per request: {cache.filled} are used and {n} come in")
+    most = n if most is None else most
+    if not 0 <= most <= n:
+        raise ValueError(f"of {n} tokens per request the largest count cannot be {most}")
+    if cache.filled + most > rows:
+        raise ValueError(f"the cache holds {rows} rows per request: up to {cache.filled} are used and {most} come in")
     h, hk, d = layer.heads, layer.kv_heads, layer.head_dim
     qkv = layer.qkv(x.reshape(b * n, hidden)).view(b * n, h + 2 * hk, d)
     q, k, v = qkv.split((h, hk, hk), 1)
@@ -94,7 +98,7 @@ def step(layer: PrefixAttention, x: torch.Tensor, cache: PrefixCache, cos: torch
     q = jo.rotary_embed_append(q, k, v, cos, sin, position.view(-1), slot.view(-1), cache.k_own.view(b * rows, hk, d),
                                cache.v_own.view(b * rows, hk, d), layer.interleaved)
     cache.lens += new
-    cache.filled += n
+    cache.filled += most
     o, _ = jo.shared_prefix_attention(q.view(b, n, h, d), cache.k_prefix, cache.v_prefix, cache.k_own, cache.v_own,
                                       cache.lens)
     return layer.out(o.view(b * n, h * d)).view(b, n, -1)

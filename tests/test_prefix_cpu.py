@@ -149,3 +149,31 @@ def test_rotary_derivatives(jo):
             o, _ = torch.compile(lambda y: both(y, k), backend="eager", fullgraph=True)(x)
             assert same(o, ref.rotary(q, cos, sin, at, False)) and o.requires_grad == x.requires_grad
         assert same(torch.autograd.grad(o, a, dq)[0], back)
+
+
+def test_step_reckons_the_room_by_the_rows_that_come_in(jo, monkeypatch):
+    from joyomni_ops import prefix
+
+    def append(q, k, v, cos, sin, positions, slots, k_cache, v_cache, interleaved=False):
+        live = slots >= 0
+        k_cache[slots[live]], v_cache[slots[live]] = k[live], v[live]
+        return q
+
+    monkeypatch.setattr(jo, "rotary_embed_append", append)
+    monkeypatch.setattr(jo, "shared_prefix_attention", lambda q, *a: (q, None))
+    layer = prefix.PrefixAttention(lambda x: torch.ones(x.shape[0], 3 * 2 * 8), lambda x: x, 2, 2, 8)
+    cache = prefix.PrefixCache.allocate(torch.zeros(5, 2, 8), torch.zeros(5, 2, 8), 3, 20)
+    x = torch.zeros(3, 16, 16)
+    for i in range(6):  # padded to 16 tokens, 3 at most are there
+        assert prefix.step(layer, x, cache, None, None, torch.tensor([3, 0, 2], dtype=torch.int32), 3).shape == (3, 16, 16)
+    assert cache.filled == 18 and cache.lens.tolist() == [18, 0, 12]
+    prefix.step(layer, x[:, :2], cache, None, None)  # two more for each
+    assert cache.filled == 20 and cache.lens.tolist() == [20, 2, 14]
+    assert all((cache.k_own[r, :n] == 1).all() for r, n in enumerate((20, 2, 14)))
+    with pytest.raises(ValueError):
+        prefix.step(layer, x[:, :1], cache, None, None)
+    for most in (-1, 3):
+        with pytest.raises(ValueError):
+            prefix.step(layer, x[:, :2], cache, None, None, None, most)
+    prefix.step(layer, x[:, :2], cache, None, None, torch.zeros(3, dtype=torch.int32), 0)
+    assert cache.filled == 20 and cache.lens.tolist() == [20, 2, 14]
