@@ -413,7 +413,8 @@ JO_API int jo_peer_copy(void* dst, const void* src, int64_t bytes, void* stream)
  * for JO_FP4_NV, 32 for JO_FP4_MX).  -1: bad arguments. */
 JO_API int64_t jo_fp4_scale_bytes(int64_t rows, int64_t cols, int format);
 
-/* Rows to 4 bits.  x: F32/F16/BF16 [rows, cols], cols a multiple of 32; q: packed
+/* Rows to 4 bits.  x: F32/F16/BF16 [rows, cols], cols a multiple of 32 and at most
+ * 98304 (F32: 65536); q: packed
  * codes [rows, cols/2] bytes (row stride in bytes, a multiple of 8); block_scale:
  * jo_fp4_scale_bytes(rows, cols, format) bytes, every one written (zero where there
  * is no row or block); row_scale: fp32 [rows], JO_FP4_NV only.
@@ -450,8 +451,8 @@ JO_API int jo_fp4_scaled_mm(void* d, int64_t ldd, const void* a, int64_t lda, co
  * product's kernel; else the product starts loading the weight while the quantisation runs,
  * so nothing else may be writing the weight by then but work that was queued on `stream`
  * before this call.
- * workspace: 16-byte aligned, jo_fp4_linear_workspace(m, k, format) bytes (-1: bad
- * arguments). */
+ * K at most 98304.  workspace: 16-byte aligned, jo_fp4_linear_workspace(m, k, format) bytes
+ * (-1: bad arguments). */
 JO_API int64_t jo_fp4_linear_workspace(int64_t m, int64_t k, int format);
 JO_API int jo_fp4_linear(void* d, int64_t ldd, const void* x, int64_t x_row_stride, const void* b, int64_t ldb,
                          const void* block_b, const float* scale_b, const void* bias, int64_t m, int64_t n, int64_t k,

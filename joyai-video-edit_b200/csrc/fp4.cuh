@@ -16,6 +16,8 @@
 namespace jo {
 
 constexpr int fp4_block(int format) { return format == JO_FP4_NV ? 16 : 32; }
+// Longest row that is quantised: one CTA of 32 warps holds it, six runs of 16 per lane (four of fp32).
+constexpr int64_t fp4_longest_row(int dtype) { return (int64_t)32 * 32 * 16 * (dtype == JO_F32 ? 4 : 6); }
 // 512-byte tiles along K.
 inline int64_t fp4_tiles_k(int64_t k, int format) { return cdiv(cdiv(k, fp4_block(format)), 4); }
 

@@ -960,7 +960,9 @@ int jo_fp4_scaled_mm(void* d, int64_t ldd, const void* a, int64_t lda, const voi
 }
 
 int64_t jo_fp4_linear_workspace(int64_t m, int64_t k, int format) {
-  if (m < 0 || k <= 0 || k % 32 || (format != JO_FP4_NV && format != JO_FP4_MX)) return -1;
+  if (m < 0 || m > INT32_MAX || k <= 0 || k % 32 || (m > 0 && k > fp4_longest_row(JO_BF16)) ||
+      (format != JO_FP4_NV && format != JO_FP4_MX))
+    return -1;
   return linear_work(m, k, format).bytes;
 }
 
@@ -971,7 +973,9 @@ int jo_fp4_linear(void* d, int64_t ldd, const void* x, int64_t x_row_stride, con
   if (dtype != JO_BF16 && dtype != JO_F16) return fail(JO_ERR_DTYPE, "%s: x must be bf16 or fp16", op);
   if (m < 0 || n < 0) return fail(JO_ERR_SHAPE, "%s: negative size", op);
   const int64_t bytes = jo_fp4_linear_workspace(m, k, format);
-  if (bytes < 0) return fail(JO_ERR_SHAPE, "%s: K must be a positive multiple of 32, in a 4-bit format", op);
+  if (bytes < 0)
+    return fail(JO_ERR_SHAPE, "%s: K must be a positive multiple of 32 and at most %lld, in a 4-bit format", op,
+                (long long)fp4_longest_row(dtype));
   if (m == 0 || n == 0) return JO_OK;
   if (!workspace || !aligned16(workspace) || workspace_bytes < bytes)
     return fail(JO_ERR_INVALID, "%s: a 16-byte aligned workspace of %lld bytes is needed", op, (long long)bytes);

@@ -219,7 +219,7 @@ int dispatch_quant(QuantArgs a, const DeviceInfo* di, cudaStream_t st) {
   // another's arithmetic.  Measured, bf16: 10800 x 3072 with 1 / 2 / 4 / 6 runs 21.4 / 18.8 /
   // 18.8 / 20.1 us, 10800 x 12288 101 / 77 / 65 / 65, 1350 x 3072 3.8 / 4.1 / 4.7 / 4.8.
   const int full = (int)cdiv(a.runs, 32);
-  constexpr int kMost = sizeof(T) == 4 ? 4 : 6;
+  constexpr int kMost = sizeof(T) == 4 ? 4 : 6;  // fp4_longest_row
   int runs = 1;
   if (a.rows * full >= (int64_t)64 * di->sm_count || full > 32)
     for (int r : {2, 4, 6}) {
@@ -229,7 +229,6 @@ int dispatch_quant(QuantArgs a, const DeviceInfo* di, cudaStream_t st) {
     }
   if (runs > full) runs = full;
   a.warps = (int)cdiv(full, runs);
-  if (a.warps > 32) return fail(JO_ERR_SHAPE, "quant_fp4: rows of at most %d elements", 32 * 32 * 16 * kMost);
   switch (runs) {
     case 1: return launch_quant<T, kMx, 1>(a, st);
     case 2: return launch_quant<T, kMx, 2>(a, st);
@@ -276,6 +275,8 @@ int jo_quant_fp4(void* q, int64_t q_row_stride, void* block_scale, float* row_sc
   if (int s = device_info(&di)) return s;
   if (int s = check_fp4(op, q, q_row_stride, block_scale, row_scale, rows, cols, format, dtype)) return s;
   if (rows == 0) return JO_OK;
+  if (cols > fp4_longest_row(dtype))
+    return fail(JO_ERR_SHAPE, "%s: rows of at most %lld elements", op, (long long)fp4_longest_row(dtype));
   if (!x) return fail(JO_ERR_INVALID, "%s: null operand", op);
   if (rows > 1 && x_row_stride < cols) return fail(JO_ERR_SHAPE, "%s: row stride smaller than the row", op);
   const int64_t esize = dtype == JO_F32 ? 4 : 2;

@@ -117,6 +117,7 @@ torch::Tensor fp4_linear(const torch::Tensor& x, const torch::Tensor& mat_b, con
   const c10::cuda::CUDAGuard guard(x.device());
   auto out = new_empty({M, N}, x.scalar_type(), x);
   const int64_t bytes = jo_fp4_linear_workspace(M, K, format);
+  TORCH_CHECK(bytes >= 0, "joyomni_ops::fp4_linear: rows of x of at most 98304 elements");
   auto work = new_empty({bytes}, at::kByte, x);
   jo_check(jo_fp4_linear(out.data_ptr(), N, x.data_ptr(), x.stride(0), mat_b.data_ptr(), mat_b.stride(0),
                          block_b.data_ptr(), (const float*)opt_ptr(scales_b), opt_ptr(bias), M, N, K, format,

@@ -451,7 +451,8 @@ def _fp4_code(format: str) -> int:
 
 
 def quant_fp4(x, format="nvfp4"):
-    """Rows of x [M, K] (bf16, fp16 or fp32; K a multiple of 32) in 4 bits: (q, block_scale, row_scale).
+    """Rows of x [M, K] (bf16, fp16 or fp32; K a multiple of 32, at most 98304, or 65536 in fp32) in 4 bits:
+    (q, block_scale, row_scale).
 
     q: uint8 [M, K/2], two e2m1 codes to a byte (the even element low).  "nvfp4": blocks of 16 with e4m3
     block scales and an fp32 row scale [M, 1]; "mxfp4": blocks of 32 with power-of-two block scales,
@@ -474,7 +475,7 @@ def fp4_scaled_mm(mat_a, mat_b, block_a, block_b, scales_a, scales_b, out_dtype,
 
 def fp4_linear(x, mat_b, block_b, scales_b=None, bias: Optional[torch.Tensor] = None):
     """A Linear layer in 4 bits: quant_fp4 of x [M, K] in the weight's format, then fp4_scaled_mm with the
-    weight (mat_b, block_b, scales_b = quant_fp4(weight [N, K])); [M, N] of x's dtype (bf16 or fp16)."""
+    weight (mat_b, block_b, scales_b = quant_fp4(weight [N, K])); [M, N] of x's dtype (bf16 or fp16).  K at most 98304."""
     return _ops.fp4_linear(x, mat_b, block_b, scales_b, bias)
 
 

@@ -146,3 +146,27 @@ def test_rotary_forward_derivative(jo, dev, dtype, interleaved):
     f = lambda x: jo.rotary_embed(x, None, cos, sin, at, interleaved)[0]
     check_rotary(torch.func.jvp(f, (q,), (dq,))[1], dq, cos, sin, at, interleaved)
     check_rotary(torch.func.grad(lambda x: (f(x) * dq).sum())(q), dq, cos, sin, at, interleaved, inverse=True)
+
+
+def test_longest_rows(jo, dev):
+    from joyomni_ops import cabi
+
+    room = cabi.lib().jo_fp4_linear_workspace
+    for f, fmt in enumerate(("nvfp4", "mxfp4")):
+        for dtype, most in ((BF, 98304), (F16, 98304), (F32, 65536)):
+            check_quant(jo, normal(gen(dev, f), dev, 3, most).to(dtype), fmt)
+            longer = torch.zeros(3, most + 32, device=dev, dtype=dtype)
+            with pytest.raises(RuntimeError, match=f"at most {most}"):
+                jo.quant_fp4(longer, fmt)
+            assert jo.quant_fp4(longer[:0], fmt)[0].shape == (0, most // 2 + 16)
+        assert room(20, 98304, f) > 0 and room(20, 98336, f) == -1 and room(2 ** 31, 64, f) == -1
+        w = normal(gen(dev, 5), dev, 16, 98304).to(BF)
+        for m in (1, 20):
+            x = normal(gen(dev, m), dev, m, 98304).to(BF)
+            a, b = jo.quant_fp4(x, fmt), jo.quant_fp4(w, fmt)
+            assert torch.equal(jo.fp4_linear(x, *b), jo.fp4_scaled_mm(a[0], b[0], a[1], b[1], a[2], b[2], BF))
+        # a block of 32 more than that
+        tiles = b[1].new_zeros(1, 1537 if fmt == "nvfp4" else 769, 32, 4, 4)
+        wide = torch.zeros(8, 49168, device=dev, dtype=torch.uint8), tiles, None if b[2] is None else b[2][:8]
+        with pytest.raises(RuntimeError, match="at most 98304"):
+            jo.fp4_linear(torch.zeros(1, 98336, device=dev, dtype=BF), *wide)
