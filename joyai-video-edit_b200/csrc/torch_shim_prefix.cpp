@@ -23,6 +23,9 @@ std::vector<int64_t> scale_shape(int64_t rows, int64_t cols, int format) {
 }
 at::ScalarType scale_type(int format) { return format == JO_FP4_NV ? at::kFloat8_e4m3fn : at::kFloat8_e8m0fnu; }
 
+// Row stride of a matrix with contiguous rows (of a single row, whose stride may be anything: its length).
+int64_t row_stride(const torch::Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
+
 // One matrix in 4 bits: packed codes [rows, K/2], its block scales, and its row scales
 // ([rows] or [rows, 1]; none for the power-of-two format).  Returns the format.
 int check_fp4(const torch::Tensor& q, const torch::Tensor& block, const c10::optional<torch::Tensor>& row,
@@ -56,7 +59,7 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> quant_fp4(const torch::T
   auto block = new_empty(scale_shape(M, K, (int)format), scale_type((int)format), x);
   auto row = new_empty({format == JO_FP4_NV ? M : 0, 1}, at::kFloat, x);
   jo_check(jo_quant_fp4(q.data_ptr(), K / 2, block.data_ptr(), row.numel() ? row.data_ptr<float>() : nullptr,
-                        x.data_ptr(), x.stride(0), M, K, (int)format, dt_code(x.scalar_type()), stream_of(x)),
+                        x.data_ptr(), row_stride(x), M, K, (int)format, dt_code(x.scalar_type()), stream_of(x)),
            "quant_fp4");
   return {q, block, row};
 }
@@ -68,7 +71,7 @@ torch::Tensor dequant_fp4(const torch::Tensor& q, const torch::Tensor& block, co
   const int64_t M = q.size(0), K = 2 * q.size(1);
   const c10::cuda::CUDAGuard guard(q.device());
   auto out = new_empty({M, K}, dtype, q);
-  jo_check(jo_dequant_fp4(out.data_ptr(), K, q.data_ptr(), q.stride(0), block.data_ptr(),
+  jo_check(jo_dequant_fp4(out.data_ptr(), K, q.data_ptr(), row_stride(q), block.data_ptr(),
                           (const float*)opt_ptr(row), M, K, format, dt_code(dtype), stream_of(q)),
            "dequant_fp4");
   return out;
@@ -97,7 +100,7 @@ torch::Tensor fp4_scaled_mm(const torch::Tensor& mat_a, const torch::Tensor& mat
   check_product(mat_a, N, out_dtype, bias);
   const c10::cuda::CUDAGuard guard(mat_a.device());
   auto out = new_empty({M, N}, out_dtype, mat_a);
-  jo_check(jo_fp4_scaled_mm(out.data_ptr(), N, mat_a.data_ptr(), mat_a.stride(0), mat_b.data_ptr(), mat_b.stride(0),
+  jo_check(jo_fp4_scaled_mm(out.data_ptr(), N, mat_a.data_ptr(), row_stride(mat_a), mat_b.data_ptr(), row_stride(mat_b),
                             block_a.data_ptr(), block_b.data_ptr(), (const float*)opt_ptr(scales_a),
                             (const float*)opt_ptr(scales_b), opt_ptr(bias), M, N, 2 * mat_a.size(1), format,
                             dt_code(out_dtype), stream_of(mat_a)),
@@ -119,7 +122,7 @@ torch::Tensor fp4_linear(const torch::Tensor& x, const torch::Tensor& mat_b, con
   const int64_t bytes = jo_fp4_linear_workspace(M, K, format);
   TORCH_CHECK(bytes >= 0, "joyomni_ops::fp4_linear: rows of x of at most 98304 elements");
   auto work = new_empty({bytes}, at::kByte, x);
-  jo_check(jo_fp4_linear(out.data_ptr(), N, x.data_ptr(), x.stride(0), mat_b.data_ptr(), mat_b.stride(0),
+  jo_check(jo_fp4_linear(out.data_ptr(), N, x.data_ptr(), row_stride(x), mat_b.data_ptr(), row_stride(mat_b),
                          block_b.data_ptr(), (const float*)opt_ptr(scales_b), opt_ptr(bias), M, N, K, format,
                          dt_code(x.scalar_type()), work.data_ptr(), bytes, stream_of(x)),
            "fp4_linear");

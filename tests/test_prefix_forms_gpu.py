@@ -170,3 +170,17 @@ def test_longest_rows(jo, dev):
         wide = torch.zeros(8, 49168, device=dev, dtype=torch.uint8), tiles, None if b[2] is None else b[2][:8]
         with pytest.raises(RuntimeError, match="at most 98304"):
             jo.fp4_linear(torch.zeros(1, 98336, device=dev, dtype=BF), *wide)
+
+
+@pytest.mark.parametrize("fmt", ["nvfp4", "mxfp4"])
+def test_one_row_with_any_row_stride(jo, dev, fmt):
+    g = gen(dev, 12)
+    x, w = normal(g, dev, 1, 64).to(BF), jo.quant_fp4(normal(g, dev, 8, 64), fmt)
+    a = jo.quant_fp4(x, fmt)
+    want = jo.fp4_scaled_mm(a[0], w[0], a[1], w[1], a[2], w[2], BF)
+    turned = a[0].view(32, 1).clone().t()  # [1, 32], contiguous, row stride 1
+    assert turned.stride() == (1, 1)
+    assert torch.equal(jo.fp4_scaled_mm(turned, w[0], a[1], w[1], a[2], w[2], BF), want)
+    assert torch.equal(jo.dequant_fp4(turned, *a[1:]), jo.dequant_fp4(*a))
+    column = x.view(64, 1).clone().t()
+    assert torch.equal(jo.fp4_linear(column, *w), want) and torch.equal(jo.quant_fp4(column, fmt)[0], a[0])
