@@ -660,23 +660,21 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         const int limit = min(kTileKeys, (own ? (my_b == w.b ? visible : 0) : a.prefix) - key0);
         wait(s_full(s), count);
         tc_fence_after();
-        if (own) {
-          // Value rows that not every row here sees must not reach the others' products, where
-          // p is 0 but 0 * inf is not: cache rows past the request's length, which hold
-          // anything, and rows with an infinity or a NaN where requests or causal limits
-          // differ.  They are zeroed (a tile that both streams use: by stream 0, whose product
-          // comes first); a row that does see such a value gives NaN.
+        // Value rows that not every row here sees must not reach the others' products, where p is 0
+        // but 0 * inf is not: cache rows past the request's length, which hold anything, and rows
+        // with an infinity or a NaN where requests or causal limits differ.  They are zeroed (a tile
+        // that both streams use: by stream 0, whose product comes first); a row that does see such a
+        // value gives NaN.  Every other tile ends before seen_by_all, which is at most the length.
+        if (own && (u.b0 != u.b1 || key0 + kTileKeys > seen_by_all)) {
           const int len = own_len(a, w.b);
-          const bool guarded = u.b0 != u.b1 || key0 + kTileKeys > seen_by_all;
-          const bool ends = len < a.own && key0 + kTileKeys > len;
           const int turn = alternate ? guards & 1 : shared_guards & 1;
           int* const first_bad = reinterpret_cast<int*>(gbase + S::kGuard) + turn * 8 + (alternate ? s * 4 : 0);
-          if ((guarded || ends) && (alternate || s == 0)) {
+          if (alternate || s == 0) {
             const int idx = at + v_index(alternate, alternate ? 2 * t + s : t, n), slot = idx % kRing;
             wait(full(slot), idx / kRing);
             uint8_t* const vrow = gbase + S::kKV + slot * S::kTile + r * 128;
             bool zero = ok && key0 + r >= len, bad = false;
-            if (ok && guarded && !zero) {
+            if (ok && !zero) {
               uint32_t mag = 0;
 #pragma unroll
               for (int c = 0; c < D / 8; ++c) {
@@ -691,34 +689,30 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
                 *reinterpret_cast<uint4*>(vrow + (c / 8) * kBox + (((c ^ r) & 7) << 4)) = make_uint4(0, 0, 0, 0);
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            if (guarded) {
-              const int low = __reduce_min_sync(0xffffffffu, bad ? r : kTileKeys);
-              if (lane == 0) first_bad[warp & 3] = low;
-            }
+            const int low = __reduce_min_sync(0xffffffffu, bad ? r : kTileKeys);
+            if (lane == 0) first_bad[warp & 3] = low;
           }
-          if (guarded) {
-            // Stream 1 takes what stream 0 found in a tile that both use.  Stream 0 goes on without
-            // waiting for it and may be one such tile ahead, not two: S(t + 2) of stream 0 is
-            // issued after O += P V of stream 1's tile t, whose P comes after this.  So two barriers
-            // in turn do, and waits that are bounded as all others.
-            if (alternate) {
-              if (s == 0)
-                asm volatile("bar.sync 2, 128;" ::: "memory");
-              else
-                asm volatile("bar.sync 3, 128;" ::: "memory");
-              ++guards;
+          // Stream 1 takes what stream 0 found in a tile that both use.  Stream 0 goes on without
+          // waiting for it and may be one such tile ahead, not two: S(t + 2) of stream 0 is issued
+          // after O += P V of stream 1's tile t, whose P comes after this.  So two barriers in turn
+          // do, and waits that are bounded as all others.
+          if (alternate) {
+            if (s == 0)
+              asm volatile("bar.sync 2, 128;" ::: "memory");
+            else
+              asm volatile("bar.sync 3, 128;" ::: "memory");
+            ++guards;
+          } else {
+            if (s == 0) {
+              arrive_warp(guarded_by_0(turn));
+              asm volatile("bar.sync 2, 128;" ::: "memory");
             } else {
-              if (s == 0) {
-                arrive_warp(guarded_by_0(turn));
-                asm volatile("bar.sync 2, 128;" ::: "memory");
-              } else {
-                wait(guarded_by_0(turn), shared_guards >> 1);
-              }
-              ++shared_guards;
+              wait(guarded_by_0(turn), shared_guards >> 1);
             }
-            const int low = min(min(first_bad[0], first_bad[1]), min(first_bad[2], first_bad[3]));
-            poisoned = poisoned || low < limit;
+            ++shared_guards;
           }
+          const int low = min(min(first_bad[0], first_bad[1]), min(first_bad[2], first_bad[3]));
+          poisoned = poisoned || low < limit;
         }
         if (!ok) {
           // a wait ran out: the rest of the walk is only gone through, for the barriers in it
