@@ -643,7 +643,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
       if (lane == 0) mbar_arrive(a_ready);
       if (!kMx) row_scale = reinterpret_cast<const float*>(gbase + S::kRowScale) + (warp - 2) * 16;
     }
-    const bool ok = mbar_wait(tfull, 0, fault);
+    const bool ok = __all_sync(0xffffffffu, mbar_wait(tfull, 0, fault));
     tc_fence_after();
     // each CTA of the cluster adds up kCols / split of the columns (both powers of two)
     const int shift = 31 - __clz(kCols / split), share = 1 << shift;
