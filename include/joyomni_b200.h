@@ -503,9 +503,12 @@ JO_API int jo_rotary_embed_append(void* q_out, int64_t qo_stride_t, int64_t qo_s
  * (natural log-sum-exp of the scaled scores) fp32 [batch, q_heads, q_len]; a query
  * that sees nothing gives 0 and -inf.  An infinity or a NaN in a key or a value reaches
  * the queries that see its row and no others; one in an own row's value may make all of
- * those queries' out NaN.  dtype F16/BF16, head_dim 64 or 128; scale > 0.  Pointers and
- * strides of q, k and v: multiples of 16 bytes; out and workspace: 32-byte aligned;
- * workspace: jo_shared_prefix_attention_workspace(...) bytes (-1: bad arguments). */
+ * those queries' out NaN.  The softmax weights are rounded to dtype for the product with
+ * the values: relative 2^-8 (BF16) or 2^-11 (F16, where also an absolute 2^-32 of the
+ * largest weight); scores, sums and out are held in fp32 until out's one rounding.  dtype
+ * F16/BF16, head_dim 64 or 128; scale > 0.  Pointers and strides of q, k and v: multiples
+ * of 16 bytes; out and workspace: 32-byte aligned; workspace:
+ * jo_shared_prefix_attention_workspace(...) bytes (-1: bad arguments). */
 JO_API int64_t jo_shared_prefix_attention_workspace(int64_t batch, int64_t q_len, int64_t q_heads, int64_t kv_heads,
                                                     int64_t head_dim, int64_t prefix_len, int64_t own_len);
 JO_API int jo_shared_prefix_attention(void* out, float* lse, const void* q, int64_t q_stride_b, int64_t q_stride_t,

@@ -852,9 +852,11 @@ int launch_rows(const Operands& o, Fp4GemmArgs g, cudaStream_t st, const DeviceI
 template <typename OutT, bool kMx>
 int dispatch(const Operands& o, const Fp4GemmArgs& g, cudaStream_t st, const DeviceInfo* di) {
   // CTA pairs where their 256 x 256 tiles occupy at least half of the SMs; below that the rows
-  // kernel's smaller tiles, split over K, finish sooner. Pairs / rows, microseconds, M x N x K:
-  // 200 x 1024 x 1024 (a twentieth of the SMs) 8.8 / 8.8; 512 x 3072 x 3072 (a third)
-  // 11.7 / 10.6; 1350 x 3072 x 3072 (all, 72 of 74 pairs) 12.3 / 20.9.
+  // kernel's 128 x 128 tiles take one round of the SMs, above it two. Pairs / rows, microseconds,
+  // M x N x K, pair tiles of the 74 that the GPU holds: JO_FP4_NV 200 x 1024 x 1024 (4) 8.8 / 8.8;
+  // 512 x 3072 x 3072 (24) 11.5 / 10.4; 768 x 3072 x 3072 (36) 11.8 / 10.5; 1024 x 2560 x 3072
+  // (40) 12.1 / 19.8; 512 x 4864 x 1024 (38) 9.3 / 15.3; 1350 x 3072 x 3072 (72) 12.3 / 20.9.
+  // JO_FP4_MX 768 x 3072 x 3072 9.0 / 9.3; 1024 x 2560 x 3072 9.5 / 17.4.
   const int64_t pair_tiles = cdiv(g.m, kPairM) * cdiv(g.n, kPairN);
   if (g.m > 128 && pair_tiles * 2 * 2 >= di->sm_count) return launch_pair<OutT, kMx>(o, g, st, di);
   if (g.x) return launch_rows<OutT, kMx, 16, true>(o, g, st, di);

@@ -20,8 +20,9 @@
 // one 8-byte store.  One pass: the row stays in registers between its maximum and
 // its codes.  `warps` warps share a row, each lane holding up to kRuns runs.
 //
-// Measured (B200, bf16): 10800 x 3072 to 4 bits 18.0 us (JO_FP4_NV, 85 MB at 4.7 TB/s, issue
-// slots 68 % busy) and 13.9 (JO_FP4_MX, 5.9 TB/s), back 13.1 (6.5 TB/s); one row 1.6 us.
+// Measured (B200, bf16): 10800 x 3072 to 4 bits 18.1 us (JO_FP4_NV, 85 MB at 4.7 TB/s, issue
+// slots 68 % busy) and 14.2 (JO_FP4_MX, 5.9 TB/s), back 14.4 (5.9 TB/s; 13.4 with the codes in
+// L2); one row 1.5 us.
 #include "fp4_quant.cuh"
 
 namespace jo {

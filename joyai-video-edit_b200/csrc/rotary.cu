@@ -11,16 +11,18 @@
 // tables' own scale a (c^2 + s^2 = a^2, a stretched context's attention factor),
 // so its gradient is the same map with -s: dx = (dy0 c + dy1 s, dy1 c - dy0 s).
 //
-// Bound: HBM (each element read once and written once; 6 flops per pair).  One CTA
+// Bound: HBM (each element read once and written once; 6 flops per pair); with few tokens
+// per CTA their latency, as a token's loads wait for the last one's stores.  One CTA
 // holds one token at a time: a thread keeps one place of the head (a 16-byte vector,
 // or in the half layout the two vectors that hold both halves of its pairs) and walks
 // over the heads of q, k (and v), so the table row is read once per token and place
 // and stays in registers, and neither layout needs a shuffle or a second load.
 //
-// Measured (B200, bf16): 10800 tokens x 48 heads of 128, interleaved, 48.9 us (5.5 TB/s, 0.84
-// of the measured copy; 63.9 with a head's load behind the store before it); 4099 x 40 heads,
-// half layout, half of each head, 16.5 us (5.1 TB/s; 23.2 at two CTAs per SM); append of 2043
-// tokens x 72 heads 15.4 us, of 32 tokens 2.4.
+// Measured (B200, bf16, inputs from memory): 10800 tokens x 48 heads of 128, interleaved, 48.6 us
+// (5.5 TB/s, 0.84 of the measured copy; 63.9 with a head's load behind the store before it); 4099
+// x 40 heads, half layout, half of each head, 18.4 us (4.6 TB/s, seven tokens to a CTA one after
+// the other; interleaved whole heads of that size take as long); append of 2043 tokens x 72 heads
+// 16.8 us (13.5 with all of it in L2), of 32 tokens 2.4.
 #include "common.cuh"
 
 namespace jo {

@@ -561,7 +561,9 @@ def shared_prefix_attention(q, k_prefix, v_prefix, k_own, v_own, lens, causal=Tr
     each request's own rows (the first lens [B] (int32) of k_own / v_own [B, S, HK, D]; what lies after them
     is not used, whatever it holds).  Every query sees the whole prefix; causal: the L queries are the last
     rows of their request, so query i sees own rows up to lens - L + i.  H a multiple of HK, D 64 or 128,
-    bf16 or fp16; scale: 1/sqrt(D) by default.  Returns (out [B, L, H, D], lse fp32 [B, H, L], the natural
+    bf16 or fp16; scale: 1/sqrt(D) by default.  The softmax weights are rounded to q's dtype for the product
+    with the values (relative 2^-8 in bf16, 2^-11 in fp16), everything else is held in fp32.  An infinity or a
+    NaN in an own value row reaches the queries that see the row and may make all of their out NaN.  Returns (out [B, L, H, D], lse fp32 [B, H, L], the natural
     log-sum-exp of the scaled scores); a query that sees nothing gives 0 and -inf."""
     return _ops.shared_prefix_attention(q, k_prefix, v_prefix, k_own, v_own, lens, causal,
                                         q.shape[-1] ** -0.5 if scale is None else scale)

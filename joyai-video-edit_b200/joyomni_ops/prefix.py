@@ -9,6 +9,9 @@ request has its own rows after them.  One step of L new tokens per request:
                      -> attention over prefix and own rows    shared_prefix_attention
                      -> output projection in 4 bits         fp4_linear
 
+The layer has what these operators need and no more: no normalisation of q and k before the rotation, and one
+position per token.
+
 Nothing is read back to the host: lengths, positions and cache slots stay on the GPU, so a step can be
 captured into a CUDA graph (capture it with ``cache.filled`` left to the caller).
 """
@@ -75,8 +78,8 @@ def step(layer: PrefixAttention, x: torch.Tensor, cache: PrefixCache, cos: torch
     """L new tokens of each request through the layer: x [B, L, hidden] -> [B, L, hidden]; the cache grows.
 
     Token i of request b stands at position P + lens[b] + i of the tables (``rope.rotary_tables``).  counts
-    (int32 [B], at most L): how many of the L tokens request b really has, the last counts[b] of its rows; the
-    padding in front of them is not cached and its outputs mean nothing.  most: the largest of counts, which the host
+    (int32 [B], at most L): how many of the L tokens request b really has, the last counts[b] of its rows (the
+    first of them is its token 0); the padding in front of them is not cached and its outputs mean nothing.  most: the largest of counts, which the host
     cannot see in them (L if not given); the cache's room is reckoned by it.
     """
     b, n, hidden = x.shape

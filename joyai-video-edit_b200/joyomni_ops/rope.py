@@ -76,8 +76,9 @@ def scaled_freqs(dim: int, theta: float = 10000.0, scaling: str = "none", factor
     ``"none"``: theta^(-2i/dim).  ``"linear"``: positions divided by factor.  ``"ntk"``: theta times
     factor^(dim / (dim - 2)), so the lowest frequency is divided by factor and the highest stays.
     ``"yarn"`` (Peng et al., "YaRN", 2023): frequencies that turn more than beta[0] times within the
-    ``original`` context stay, those below beta[1] turns are divided by factor, a ramp in between; the
-    tables are scaled by 0.1 ln(factor) + 1.
+    ``original`` context stay, those below beta[1] turns are divided by factor, a ramp in between that is
+    linear in the turns, as in the paper; the tables are scaled by 0.1 ln(factor) + 1.  (Many programs have a
+    ramp that is linear in the frequency's index: weights tuned with it expect other frequencies in between.)
     """
     if dim % 2 or dim <= 0:
         raise ValueError(f"RoPE dimension must be even and positive, got {dim}")
